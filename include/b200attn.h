@@ -266,6 +266,54 @@ int b200attn_rope_norm_bwd_qk(const void* dyq, const void* dyk, int y_layout, co
                               size_t workspace_bytes, void* stream);
 
 /*
+ * Rotary positions in every layout, for q and k in one launch each way (the reference has one: all of the head, neighbouring pairs,
+ * the token's index as its position, the norm always, llm/src/model/rope.cu:25-65; that one is b200attn_rope_norm_fwd_qk).
+ *
+ *   The first R of a head's D elements turn (R a multiple of 16, at most D); a pair is (x[2i], x[2i+1]) with
+ *   B200ATTN_PAIRS_INTERLEAVED or (x[i], x[i + R/2]) with B200ATTN_PAIRS_HALF; the other elements are taken as they are.
+ *   pos: [B, T] (device, int32) the tokens' positions, or NULL: token t has position t.  cos_t, sin_t: [n_pos, R / 2] FP32, 16-byte
+ *   aligned.  A token whose position is not in [0, n_pos) is skipped (its outputs are not written) and sets the device status word to 106.
+ *   gamma_q and gamma_k: the QK-norm behind the rotation, with rstd_* [B, H, T] written (forward) or read (backward); both NULL:
+ *   no norm, and then rstd_*, d_gamma_* and, in the backward, xq and xk are not used and may be NULL.
+ *
+ * Layouts, types and d_gamma (accumulated into, in a fixed order) as for b200attn_rope_norm_fwd / _bwd; the workspace, of
+ * b200attn_rope_norm_bwd_workspace_bytes(D), is only needed with the norm.
+ *
+ * b200attn_rotary_table fills DEVICE tables [T, R / 2] of angles computed in 64 bits, position * f(i) with
+ *   B200ATTN_SCALING_NONE    f = base^(-2i/R)
+ *   B200ATTN_SCALING_LINEAR  f / factor: positions pressed together
+ *   B200ATTN_SCALING_BASE    f of the base base * factor^(R/(R-2)): the fastest pair as it was, the slowest slowed by the factor
+ *   B200ATTN_SCALING_PARTS   pairs that turn more than turns_fast times within `trained` positions as they were, those that turn less
+ *                            than turns_slow times slowed by the factor, linear in the number of turns between
+ * (factor, trained and turns_* are ignored where the scaling has no use for them.)
+ */
+enum { B200ATTN_PAIRS_INTERLEAVED = 0, B200ATTN_PAIRS_HALF = 1 };
+enum { B200ATTN_SCALING_NONE = 0, B200ATTN_SCALING_LINEAR = 1, B200ATTN_SCALING_BASE = 2, B200ATTN_SCALING_PARTS = 3 };
+int b200attn_rotary_table(int T, int R, double base, int scaling, double factor, double trained, double turns_fast,
+                          double turns_slow, float* cos_t, float* sin_t, void* stream);
+int b200attn_rotary_fwd(const void* xq, const void* xk, int x_dtype, int x_layout, void* yq, void* yk, int y_layout,
+                        float* rstd_q, float* rstd_k, const float* gamma_q, const float* gamma_k, const float* cos_t,
+                        const float* sin_t, const int* pos, int n_pos, int R, int pairs, int B, int T, int Hq, int Hkv,
+                        int D, float eps, void* stream);
+int b200attn_rotary_bwd(const void* dyq, const void* dyk, int y_layout, const void* xq, const void* xk, int x_dtype,
+                        int x_layout, const float* rstd_q, const float* rstd_k, const float* gamma_q,
+                        const float* gamma_k, const float* cos_t, const float* sin_t, const int* pos, int n_pos, int R,
+                        int pairs, void* dxq, void* dxk, float* d_gamma_q, float* d_gamma_k, int B, int T, int Hq,
+                        int Hkv, int D, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * b200attn_kv_append with those rotations, for caches whose rows and positions part ways (behind a shared prompt, after an
+ * eviction).  The n_new tokens of sequence b get the positions pos[b] + t and the cache rows rows[b] + t; pos and rows are [B]
+ * (device, int32) or NULL: pos0 and row0 for every sequence.  positions: [B, Hkv, L_cap] int32, where the k rows' positions are
+ * noted, or NULL.  gamma_q and gamma_k may both be NULL (no norm).  A sequence whose rows exceed L_cap (status word 105) or whose
+ * positions exceed the tables (106) is skipped.
+ */
+int b200attn_kv_append_rotary(const void* xq, const void* xk, const void* xv, int x_dtype, void* q_out, void* kcache,
+                              void* vcache, int* positions, const float* gamma_q, const float* gamma_k,
+                              const float* cos_t, const float* sin_t, int n_pos, int R, int pairs, const int* pos,
+                              int pos0, const int* rows, int row0, int B, int n_new, int L_cap, int Hq, int Hkv, int D,
+                              float eps, void* stream);
+
+/*
  * Diagnostics for benchmarks (no counterpart in the reference): when three CUDA events are
  * set, every following b200attn_bwd records them on its stream before the dQ pass (which also
  * computes D = rowsum(o * dout)), after it, and after the dK/dV pass, so a caller can time each
@@ -291,7 +339,7 @@ int b200attn_item_deal(int n_groups, int n_qtiles, int T, int n_ctas, int item_c
  * Synchronises `stream` and returns the device status word of the current device:
  * 0, or the code of the first bounded wait that gave up since the last call (101 load,
  * 102 tensor core, 103 softmax hand-off, 104 buffer free), or 105 when b200attn_kv_append_at met a
- * position beyond the cache capacity (the word is then cleared).  The reference surfaces execution errors at a later
+ * position beyond the cache capacity, or 106 when a position was not a row of the rotary tables (the word is then cleared).  The reference surfaces execution errors at a later
  * synchronisation too (llm/src/core/cuda_check.h:31-45).
  */
 int b200attn_last_device_status(void* stream);

@@ -24,6 +24,7 @@ from .rope_norm import (  # noqa: F401
     rope_qknorm_forward,
     rope_qknorm_forward_qk,
 )
+from .rotary import make_rotary_cache, rotary_backward, rotary_forward  # noqa: F401
 
 __all__ = [
     "flash_attn_forward",
@@ -38,4 +39,7 @@ __all__ = [
     "rope_qknorm_backward",
     "rope_qknorm_forward_qk",
     "rope_qknorm_backward_qk",
+    "make_rotary_cache",
+    "rotary_forward",
+    "rotary_backward",
 ]

@@ -31,6 +31,9 @@ LAYOUT_BHTD = 0
 LAYOUT_BTHD = 1
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+PAIRS_INTERLEAVED = 0
+PAIRS_HALF = 1
+SCALINGS = {"none": 0, "linear": 1, "base": 2, "parts": 3}
 BWD_AUTO = 0
 BWD_TWO_PASS = 1
 BWD_ONE_PASS = 2
@@ -61,6 +64,10 @@ SYMBOLS = (
     "b200attn_rope_norm_bwd_workspace_bytes",
     "b200attn_rope_norm_fwd_qk",
     "b200attn_rope_norm_bwd_qk",
+    "b200attn_rotary_table",
+    "b200attn_rotary_fwd",
+    "b200attn_rotary_bwd",
+    "b200attn_kv_append_rotary",
     "b200attn_last_device_status",
     "b200attn_strerror",
     "b200attn_version",
@@ -148,6 +155,15 @@ def load() -> ctypes.CDLL:
     L.b200attn_rope_norm_bwd_qk.restype = i
     L.b200attn_rope_norm_bwd_workspace_bytes.argtypes = [i]
     L.b200attn_rope_norm_bwd_workspace_bytes.restype = sz
+    d = ctypes.c_double
+    L.b200attn_rotary_table.argtypes = [i, i, d, i, d, d, d, d, vp, vp, vp]
+    L.b200attn_rotary_table.restype = i
+    L.b200attn_rotary_fwd.argtypes = [vp, vp, i, i, vp, vp, i] + [vp] * 7 + [i] * 8 + [f, vp]
+    L.b200attn_rotary_fwd.restype = i
+    L.b200attn_rotary_bwd.argtypes = [vp, vp, i, vp, vp, i, i] + [vp] * 7 + [i] * 3 + [vp] * 4 + [i] * 5 + [vp, sz, vp]
+    L.b200attn_rotary_bwd.restype = i
+    L.b200attn_kv_append_rotary.argtypes = [vp] * 3 + [i] + [vp] * 8 + [i] * 3 + [vp, i, vp, i] + [i] * 6 + [f, vp]
+    L.b200attn_kv_append_rotary.restype = i
     L.b200attn_last_device_status.argtypes = [vp]
     L.b200attn_last_device_status.restype = i
     L.b200attn_strerror.argtypes = [i]

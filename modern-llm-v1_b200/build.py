@@ -1,4 +1,4 @@
-"""Builds the native code in-tree: csrc/b200attn_api.cu -> libb200attn.so (CUDA, sm_100a only) and
+"""Builds the native code in-tree: csrc/*.cu -> libb200attn.so (CUDA, sm_100a only) and
 csrc/host_binding.cc -> _host.so (the Python module over its C ABI).
 
 nvcc cross-compiles without a GPU, so this also runs on a CPU-only machine.
@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -18,8 +19,9 @@ HOST = os.path.join(HERE, "_host.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
+CUDA_SOURCES = ["b200attn_api.cu", "rotary_api.cu"]
 
 
 def sources() -> list[str]:
@@ -60,11 +62,16 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not is_stale():
         return LIB
     nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc, *NVCC_FLAGS]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", LIB, os.path.join(CSRC, "b200attn_api.cu")]
-    subprocess.check_call(cmd)
+    with tempfile.TemporaryDirectory() as tmp:  # one object per source, side by side
+        jobs = []
+        for src in CUDA_SOURCES:
+            obj = os.path.join(tmp, src + ".o")
+            cmd = [nvcc, *NVCC_FLAGS, "-c", "-o", obj, os.path.join(CSRC, src)]
+            jobs.append((cmd, obj, subprocess.Popen(cmd + (["-Xptxas", "-v"] if verbose else []))))
+        for cmd, _, job in jobs:
+            if job.wait() != 0:
+                raise subprocess.CalledProcessError(job.returncode, cmd)
+        subprocess.check_call([nvcc, *NVCC_FLAGS, "-shared", "-o", LIB, *(obj for _, obj, _ in jobs)])
     subprocess.check_call(_host_command())
     return LIB
 

@@ -16,10 +16,11 @@
 #include "attn_bwd.cuh"
 #include "attn_bwd_onepass.cuh"
 #include "attn_bwd_tile.cuh"
-#include "attn_decode.cuh"
 #include "attn_fwd.cuh"
+#include "decode_plan.h"
+#include "host_common.h"
 #include "kv_cache.cuh"
-#include "rope_norm.cuh"
+#include "rope_norm_host.h"
 #include "tmap.h"
 
 using namespace b200attn;
@@ -30,7 +31,6 @@ namespace {
 // off the word (see decode_count).
 __device__ int g_status_word[2];
 
-constexpr int kMaxDevices = 64;
 std::atomic<int*> g_status_ptr[kMaxDevices] = {};  // (the words are zero at load)
 
 // Item counters of the persistent kernels (two words per launch, see ptx.cuh), also in the device
@@ -49,6 +49,9 @@ std::atomic<unsigned> g_sched_seq{0};
 // What tells a decode launch's counters from those of every other launch (see decode_count).  The sequence starts anywhere, so
 // that the counters of another process in recycled memory are as unlikely to pass as anything else.
 std::atomic<unsigned long long> g_decode_seq{0};
+}  // namespace
+
+namespace b200attn {
 unsigned long long next_decode_tag() {
     static const unsigned long long start = [] {
         unsigned long long x = (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count() +
@@ -81,6 +84,9 @@ int* status_ptr(int* err) {
     }
     return status;
 }
+}  // namespace b200attn
+
+namespace {
 
 // The counter pair for the next launch of a persistent kernel on the current device (status_ptr()
 // has resolved the device's addresses before).
@@ -162,6 +168,9 @@ const ItemTable& item_table_for(long long n_items, unsigned n_ctas, int n_groups
     return e.tab;
 }
 
+}  // namespace
+
+namespace b200attn {
 // SM count of the current device (cached per device).
 int sm_count() {
     static int cached[kMaxDevices] = {0};
@@ -174,74 +183,9 @@ int sm_count() {
     }
     return cached[dev];
 }
+}  // namespace b200attn
 
-struct Strides {
-    long long t, h, b;  // element strides
-};
-
-inline Strides strides_for(int layout, int H, int T, int D) {
-    Strides s;
-    if (layout == B200ATTN_LAYOUT_BHTD) {
-        s.t = D;
-        s.h = (long long)T * D;
-        s.b = (long long)H * T * D;
-    } else {
-        s.t = (long long)H * D;
-        s.h = D;
-        s.b = (long long)T * H * D;
-    }
-    return s;
-}
-
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-int check_common(int B, int T, int Hq, int Hkv, int D, int layout) {
-    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return B200ATTN_ERR_INVALID_ARG;
-    if (Hq % Hkv != 0) return B200ATTN_ERR_INVALID_ARG;
-    if (layout != B200ATTN_LAYOUT_BHTD && layout != B200ATTN_LAYOUT_BTHD) return B200ATTN_ERR_INVALID_ARG;
-    if (D != 64 && D != 128) return B200ATTN_ERR_UNSUPPORTED;
-    return B200ATTN_OK;
-}
-
-// Launch with programmatic stream serialization: the kernel may become resident while the
-// previous kernel of the stream drains; it calls griddepcontrol.wait before touching global memory.
-// cluster > 1: in thread-block clusters of that many blocks.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, int cluster,
-                           Args&&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args) {
-    return launch_cluster(kernel, grid, block, smem, st, 1, args...);
-}
-
-template <typename K>
-int set_smem_once(K kernel, int bytes, bool* done) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (!done[dev]) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-            cudaGetLastError();
-            return B200ATTN_ERR_CUDA;
-        }
-        done[dev] = true;
-    }
-    return B200ATTN_OK;
-}
+namespace {
 
 // The SMs that clusters can have: those of four and eight do not fill the last SMs of a GPC and get 132 and 120 of 148.
 double cluster_slots(int cluster) { return sm_count() * (cluster <= 2 ? 1.0 : cluster <= 4 ? 0.892 : 0.811); }
@@ -611,40 +555,6 @@ int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
 // ---------------------------------------------------------------------------------------
 namespace {
 
-constexpr int kRopeNormMaxCtasPerSm = 8;  // of the backward, as far as its workspace goes
-static_assert(kRopeNormBwdBlocks <= kRopeNormMaxCtasPerSm, "a partial sum per CTA");
-
-int rope_norm_check(int B, int T, int H, int D, int x_dtype, int x_layout, int y_layout) {
-    if (B <= 0 || T <= 0 || H <= 0 || D <= 0) return B200ATTN_ERR_INVALID_ARG;
-    if (x_dtype != B200ATTN_DTYPE_BF16 && x_dtype != B200ATTN_DTYPE_F32) return B200ATTN_ERR_INVALID_ARG;
-    for (int l : {x_layout, y_layout})
-        if (l != B200ATTN_LAYOUT_BHTD && l != B200ATTN_LAYOUT_BTHD) return B200ATTN_ERR_INVALID_ARG;
-    if (D != 64 && D != 128) return B200ATTN_ERR_UNSUPPORTED;
-    if ((long long)B * T * H >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;  // rows are counted in 32 bits
-    return B200ATTN_OK;
-}
-
-// Heads per item: eight of them share a token's cosines and sines and addresses, fewer when that leaves less than four items
-// for a resident warp (one eighth of a wave is then the most that the last round can waste).
-void rope_norm_plan(RopeNormParams* p, int n_tensors, int D, unsigned warps) {
-    int chunk = 8;
-    auto items = [&](const RopeNormParams& q) { return (long long)((q.n_tokens + 256u / D - 1) / (256u / D)) * ((q.H + chunk - 1) / chunk); };
-    auto all = [&] { return items(p[0]) + (n_tensors > 1 ? items(p[1]) : 0); };
-    while (chunk > 1 && all() < (chunk > 4 ? 4LL : 1LL) * warps) chunk /= 2;
-    for (int i = 0; i < n_tensors; ++i) {
-        p[i].chunk = chunk;
-        p[i].n_items = (unsigned)items(p[i]);
-        p[i].div_chunks = fastdiv_make((unsigned)((p[i].H + chunk - 1) / chunk));
-    }
-}
-
-// CTAs that the device keeps resident at once, never more than the items need
-inline unsigned rope_norm_grid(const RopeNormParams* p, int n_tensors, int blocks) {
-    const long long items = (long long)p[0].n_items + (n_tensors > 1 ? p[1].n_items : 0);
-    const long long need = (items + kRopeNormThreads / 32 - 1) / (kRopeNormThreads / 32);
-    return (unsigned)std::min<long long>(need, (long long)blocks * sm_count());
-}
-
 template <int D, bool F32>
 void rope_norm_launch_fwd(RopeNormParams* p, int n_tensors, cudaStream_t st) {
     rope_norm_plan(p, n_tensors, D, (unsigned)(kRopeNormFwdBlocks * (kRopeNormThreads / 32) * sm_count()));
@@ -661,17 +571,6 @@ void rope_norm_launch_bwd(RopeNormParams* p, int n_tensors, float* workspace, cu
     const float* part1 = p[1].partial;
     launch_pdl(rope_norm_dgamma_kernel<D>, dim3(n_tensors * (D / 8)), kDgammaThreads, 0, st, part0, p[0].d_gamma, part1,
                p[1].d_gamma, (int)grid);
-}
-
-void rope_norm_fill(RopeNormParams& p, int B, int T, int H, int D, int x_layout, int y_layout) {
-    const Strides sx = strides_for(x_layout, H, T, D), sy = strides_for(y_layout, H, T, D);
-    p.B = B;
-    p.T = T;
-    p.H = H;
-    p.n_tokens = (unsigned)B * (unsigned)T;
-    p.x_st = sx.t, p.x_sh = sx.h, p.x_sb = sx.b;
-    p.y_st = sy.t, p.y_sh = sy.h, p.y_sb = sy.b;
-    p.div_t = fastdiv_make((unsigned)T);
 }
 
 struct RopeNormTensor {  // what differs between q and k
@@ -955,92 +854,6 @@ extern "C" int b200attn_bwd_static(const void* q, const void* k, const void* v, 
 
 namespace {
 
-// Query heads served per decode CTA: the largest divisor of the group size that is <= 16
-// (the row count of the kernel's MMA shape).
-inline int decode_heads_per_cta(int group) {
-    for (int g = 16; g >= 1; --g)
-        if (group % g == 0) return g;
-    return 1;
-}
-
-inline int decode_tile_keys(int D) { return D == 64 ? DecodeCfg<64>::kKeys : DecodeCfg<128>::kKeys; }
-inline int decode_max_ctas() { return std::min(2 * sm_count(), kDecodeMaxCtas); }  // two fit an SM: all are resident at once
-
-struct DecodePlan {
-    int G, n_chunks;
-    int slots;    // workspace slots per unit for partial results
-    int splits;   // and with the room for the counters behind them
-    int shares;   // CTAs per unit, or 0: ranges of tiles
-    int cluster;  // CTAs per cluster
-    bool whole;   // ranges of whole units
-    int n_ctas, slot_mode;
-};
-
-// The deal (see attn_decode.cuh).
-//
-// Ranges cost about 3 us at the end (partial results through memory, a counter, the last CTA's additions), clusters
-// about 1 us, whole units nothing.  So units stay whole or in clusters unless that leaves the memory system idle for longer
-// than that: some 60 SMs saturate HBM, so what counts is how many CTAs the last round has (all, where the units are fewer
-// than the SMs) and how long a unit is, and, for sequences of different lengths, how much memory there is to read at all.
-// kRangesBytes is what HBM delivers in those 3 us.
-//
-// A cluster is the smallest that leaves a CTA at most two tiles, as far as that is one CTA per SM: more of them saturate
-// HBM by themselves.
-//
-// n_splits > 0 asks for that many shares per unit (at most 64, none empty): a cluster where it can have that size.
-constexpr long long kRangesBytes = 16ll << 20;
-constexpr int kSaturatingCtas = 60;
-
-DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits, bool ragged) {
-    DecodePlan d;
-    const int group = Hq / Hkv, cap = decode_max_ctas();
-    d.G = decode_heads_per_cta(group);
-    d.n_chunks = group / d.G;
-    const long long units = (long long)B * Hkv * d.n_chunks;
-    const int keys = decode_tile_keys(D), n_all = (L + keys - 1) / keys, n_128 = (L + 127) / 128;
-    const long long unit_bytes = 4ll * L * D, tiles = units * n_all;
-    d.shares = d.cluster = 1;
-    d.whole = false;
-    d.slot_mode = kDecodeSlotTile;
-    long long counters = 0;
-    if (n_splits > 0) {
-        const int want = std::min(std::min(n_splits, n_128), 64), per = (n_128 + want - 1) / want;
-        d.slots = d.shares = (n_128 + per - 1) / per;
-        if (d.shares <= kDecodeMaxCluster && (d.shares & (d.shares - 1)) == 0) {
-            d.cluster = d.shares;
-        } else {
-            d.slot_mode = kDecodeSlotCta;
-            counters = units * d.shares;
-        }
-    } else {
-        d.slots = (int)std::min<long long>(n_all, (2 * cap + units - 1) / units);
-        if (n_all > 1) counters = std::min<long long>(tiles, cap);  // (a single tile is never shared)
-        while (d.cluster < kDecodeMaxCluster && units * d.cluster * 2 <= sm_count() && n_all > 2 * d.cluster) d.cluster *= 2;
-        d.shares = d.cluster;
-        const long long ctas = units * d.cluster, last = ctas % cap ? ctas % cap : cap;
-        const long long idle = last < kSaturatingCtas ? unit_bytes / d.cluster * (kSaturatingCtas - last) : 0;
-        if (tiles > d.cluster * units && (idle > kRangesBytes || (ragged && units * unit_bytes > kRangesBytes))) {
-            d.shares = 0;
-            d.cluster = 1;
-            d.slot_mode = d.slots == n_all ? kDecodeSlotTile : kDecodeSlotTwo;
-        }
-    }
-    // the counters behind the slots, in units of a slot of every (batch, query head)
-    const long long slot_bytes = (long long)B * Hq * (D + 2) * 4;
-    d.splits = d.slots + (int)((8 * counters + slot_bytes - 1) / slot_bytes);
-    if (d.shares == 0) {
-        d.n_ctas = (int)std::min<long long>(tiles, cap);
-        return d;
-    }
-    d.n_ctas = (int)std::min<long long>(units * d.shares, 1ll << 30);
-    if (d.shares == 1 && units > cap && !ragged) {  // the ring of a CTA then runs on from unit to unit
-        d.shares = 0;
-        d.whole = true;
-        d.n_ctas = cap;
-    }
-    return d;
-}
-
 template <int D, int NH, int PF>
 int launch_decode_pf(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p, int n_ctas, cudaStream_t st) {
     using Cfg = DecodeCfg<D>;
@@ -1298,6 +1111,7 @@ extern "C" const char* b200attn_strerror(int status) {
         case DEV_WAIT_TIMEOUT_SOFTMAX: return "device: a softmax hand-off barrier never completed";
         case DEV_WAIT_TIMEOUT_FREE: return "device: a buffer-free barrier never completed";
         case DEV_KV_CACHE_OVERFLOW: return "device: a KV-cache position plus the new tokens exceeds the cache capacity";
+        case DEV_ROTARY_POSITION: return "device: a position is not a row of the rotary tables";
         default: return "unknown status";
     }
 }

@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <cstdarg>
 #include <cstring>
@@ -65,7 +66,7 @@ const at::Tensor& unpack(PyObject* o) { return THPVariable_Unpack(o); }
 void* ptr(PyObject* o) { return unpack(o).data_ptr(); }
 int64_t numel(PyObject* o) { return unpack(o).numel(); }
 
-const char* type_name(ScalarType t) { return t == ScalarType::BFloat16 ? "BF16" : "FP32"; }
+const char* type_name(ScalarType t) { return t == ScalarType::BFloat16 ? "BF16" : t == ScalarType::Int ? "INT32" : "FP32"; }
 
 // every dtype first, then every device, then contiguity
 bool check_tensors(const char* fn, const Item* items, int n) {
@@ -90,6 +91,29 @@ bool check_tensors(const char* fn, const Item* items, int n) {
             return false;
         }
     return true;
+}
+
+// The same for arguments that may be left out (None), and all of them on one device.
+struct Items {
+    std::array<Item, 20> list;
+    int n = 0;
+    void add(PyObject* o, const char* name, ScalarType t) {
+        if (o != Py_None) list[n++] = {o, name, t};
+    }
+    bool check(const char* fn) const {
+        if (!check_tensors(fn, list.data(), n)) return false;
+        for (int i = 1; i < n; ++i)
+            if (unpack(list[i].obj).device() != unpack(list[0].obj).device()) {
+                value_error("%s: %s and %s must be on one device", fn, list[0].name, list[i].name);
+                return false;
+            }
+        return true;
+    }
+};
+// a tensor's data, or nullptr for None
+template <typename T = void>
+T* opt_ptr(PyObject* o) {
+    return o == Py_None ? nullptr : static_cast<T*>(ptr(o));
 }
 
 // the element type of a projection: BF16 or FP32
@@ -660,12 +684,167 @@ PyObject* rope_bwd_qk(PyObject*, PyObject* const* a, Py_ssize_t n) {
     B200ATTN_CATCH
 }
 
+// What the rotary calls share: B, T, Hq, Hkv, D, rotary_dim, pairs, positions or None, x_layout, y_layout (the last ten arguments)
+struct RotaryArgs {
+    NormArgs n;
+    int Hq, Hkv, R, pairs, n_pos;
+    int64_t rows_q, rows_k;
+    const int* pos;
+};
+bool rotary_sizes(const char* fn, PyObject* const* a, RotaryArgs* r) {
+    int d[6];
+    if (!ints(a, 6, d)) return false;
+    if (!norm_args(fn, a[8], a[9], d[0], d[1], d[4], &r->n)) return false;
+    r->Hq = d[2], r->Hkv = d[3], r->R = d[5];
+    if (std::min({d[0], d[1], d[2], d[3], d[4]}) <= 0) return value_error("%s: sizes must be positive", fn), false;
+    if (r->R <= 0 || r->R > d[4] || r->R % 16 != 0) return value_error("%s: rotary_dim must be a multiple of 16, at most d_h", fn), false;
+    r->pairs = -1;
+    if (PyUnicode_Check(a[6])) {
+        if (PyUnicode_CompareWithASCIIString(a[6], "interleaved") == 0) r->pairs = B200ATTN_PAIRS_INTERLEAVED;
+        else if (PyUnicode_CompareWithASCIIString(a[6], "half") == 0) r->pairs = B200ATTN_PAIRS_HALF;
+    }
+    if (r->pairs < 0) return value_error("%s: pairs must be interleaved or half", fn), false;
+    r->rows_q = int64_t(d[0]) * d[1] * d[2], r->rows_k = int64_t(d[0]) * d[1] * d[3];
+    return true;
+}
+// behind the tensor checks
+bool rotary_tables(const char* fn, PyObject* cos_t, PyObject* sin_t, PyObject* pos, RotaryArgs* r) {
+    const at::Tensor &c = unpack(cos_t), &s = unpack(sin_t);
+    if (c.dim() != 2 || c.size(1) != r->R / 2 || c.sizes() != s.sizes() || c.size(0) <= 0 || c.size(0) > INT32_MAX)
+        return value_error("%s: cos and sin must be [positions, rotary_dim / 2]", fn), false;
+    r->n_pos = int(c.size(0));
+    r->n.cos_t = static_cast<float*>(c.data_ptr());
+    r->n.sin_t = static_cast<float*>(s.data_ptr());
+    r->pos = nullptr;
+    if (pos == Py_None) {
+        if (r->n_pos < r->n.T) return value_error("%s: cos and sin have fewer positions than T", fn), false;
+    } else {
+        if (numel(pos) != int64_t(r->n.B) * r->n.T) return value_error("%s: positions must be [B, T]", fn), false;
+        r->pos = static_cast<const int*>(ptr(pos));
+    }
+    return true;
+}
+bool all_or_none(const char* fn, const char* what, std::initializer_list<PyObject*> objs, bool want) {
+    for (PyObject* o : objs)
+        if ((o != Py_None) != want) return value_error("%s: %s", fn, what), false;
+    return true;
+}
+
+// xq, xk, cos, sin, gamma_q, gamma_k, eps, yq, yk, rstd_q, rstd_k, B, T, Hq, Hkv, D, rotary_dim, pairs, positions, x_layout, y_layout
+PyObject* rotary_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "rotary_forward";
+    B200ATTN_TRY
+    if (!arg_count(n, 21)) return nullptr;
+    ScalarType xt;
+    int xd;
+    if (!x_dtype(fn, a[0], &xt, &xd)) return nullptr;
+    const ScalarType f = ScalarType::Float, bf = ScalarType::BFloat16;
+    const bool norm = a[4] != Py_None;
+    if (!all_or_none(fn, "gamma_q, gamma_k, rstd_q and rstd_k belong together", {a[5], a[9], a[10]}, norm)) return nullptr;
+    Items items;
+    items.add(a[0], "xq", xt), items.add(a[1], "xk", xt), items.add(a[7], "yq", bf), items.add(a[8], "yk", bf);
+    items.add(a[2], "cos", f), items.add(a[3], "sin", f), items.add(a[4], "gamma_q", f), items.add(a[5], "gamma_k", f);
+    items.add(a[9], "rstd_q", f), items.add(a[10], "rstd_k", f), items.add(a[18], "positions", ScalarType::Int);
+    for (int i : {1, 2, 3, 7, 8})
+        if (a[i] == Py_None) return value_error("%s: xk, cos, sin, yq and yk are needed", fn);
+    RotaryArgs r;
+    if (!items.check(fn) || !rotary_sizes(fn, a + 11, &r) || !rotary_tables(fn, a[2], a[3], a[18], &r)) return nullptr;
+    const int D = r.n.D;
+    if (numel(a[0]) != r.rows_q * D || numel(a[7]) != r.rows_q * D || numel(a[1]) != r.rows_k * D || numel(a[8]) != r.rows_k * D)
+        return value_error("%s: shape mismatch (xq/xk/yq/yk)", fn);
+    if (norm && (numel(a[4]) != D || numel(a[5]) != D)) return value_error("%s: gamma must have d_h elements", fn);
+    if (norm && (numel(a[9]) != r.rows_q || numel(a[10]) != r.rows_k)) return value_error("%s: rstd must have B * H * T elements", fn);
+    const double eps = PyFloat_AsDouble(a[6]);
+    if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+    const Call c(a[0]);
+    void *xq = ptr(a[0]), *xk = ptr(a[1]), *yq = ptr(a[7]), *yk = ptr(a[8]), *st = c.st();
+    float *gq = opt_ptr<float>(a[4]), *gk = opt_ptr<float>(a[5]), *sq = opt_ptr<float>(a[9]), *sk = opt_ptr<float>(a[10]);
+    int rc;
+    {
+        const NoGil no_gil;
+        rc = b200attn_rotary_fwd(xq, xk, xd, r.n.x_layout, yq, yk, r.n.y_layout, sq, sk, gq, gk, r.n.cos_t, r.n.sin_t, r.pos, r.n_pos, r.R,
+                                 r.pairs, r.n.B, r.n.T, r.Hq, r.Hkv, D, static_cast<float>(eps), st);
+    }
+    return finish(rc, fn);
+    B200ATTN_CATCH
+}
+
+// d_yq, d_yk, xq or None, xk or None, cos, sin, gamma_q, gamma_k, rstd_q, rstd_k, d_xq, d_xk, d_gamma_q, d_gamma_k, B, T, Hq, Hkv, D,
+// rotary_dim, pairs, positions, x_layout, y_layout
+PyObject* rotary_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "rotary_backward";
+    B200ATTN_TRY
+    if (!arg_count(n, 24)) return nullptr;
+    ScalarType xt;
+    int xd;
+    if (!x_dtype(fn, a[10], &xt, &xd)) return nullptr;
+    const ScalarType f = ScalarType::Float, bf = ScalarType::BFloat16;
+    const bool norm = a[6] != Py_None;
+    if (!all_or_none(fn, "gamma_q, gamma_k, rstd_q, rstd_k, d_gamma_q and d_gamma_k belong together", {a[7], a[8], a[9], a[12], a[13]}, norm))
+        return nullptr;
+    if (norm && (a[2] == Py_None || a[3] == Py_None)) return value_error("%s: xq and xk are needed with the norm", fn);
+    for (int i : {0, 1, 4, 5, 11})
+        if (a[i] == Py_None) return value_error("%s: d_yq, d_yk, cos, sin and d_xk are needed", fn);
+    Items items;
+    items.add(a[0], "d_yq", bf), items.add(a[1], "d_yk", bf), items.add(a[2], "xq", xt), items.add(a[3], "xk", xt);
+    items.add(a[10], "d_xq", xt), items.add(a[11], "d_xk", xt), items.add(a[4], "cos", f), items.add(a[5], "sin", f);
+    items.add(a[6], "gamma_q", f), items.add(a[7], "gamma_k", f), items.add(a[8], "rstd_q", f), items.add(a[9], "rstd_k", f);
+    items.add(a[12], "d_gamma_q", f), items.add(a[13], "d_gamma_k", f), items.add(a[21], "positions", ScalarType::Int);
+    RotaryArgs r;
+    if (!items.check(fn) || !rotary_sizes(fn, a + 14, &r) || !rotary_tables(fn, a[4], a[5], a[21], &r)) return nullptr;
+    const int D = r.n.D;
+    for (int i : {0, 2, 10})
+        if (a[i] != Py_None && numel(a[i]) != r.rows_q * D) return value_error("%s: shape mismatch (d_yq/xq/d_xq)", fn);
+    for (int i : {1, 3, 11})
+        if (a[i] != Py_None && numel(a[i]) != r.rows_k * D) return value_error("%s: shape mismatch (d_yk/xk/d_xk)", fn);
+    for (int i : {6, 7, 12, 13})
+        if (norm && numel(a[i]) != D) return value_error("%s: gamma and d_gamma must have d_h elements", fn);
+    if (norm && (numel(a[8]) != r.rows_q || numel(a[9]) != r.rows_k)) return value_error("%s: rstd must have B * H * T elements", fn);
+    const Call c(a[10]);
+    void *dyq = ptr(a[0]), *dyk = ptr(a[1]), *xq = opt_ptr(a[2]), *xk = opt_ptr(a[3]), *dxq = ptr(a[10]), *dxk = ptr(a[11]), *st = c.st();
+    float *gq = opt_ptr<float>(a[6]), *gk = opt_ptr<float>(a[7]), *sq = opt_ptr<float>(a[8]), *sk = opt_ptr<float>(a[9]),
+          *dgq = opt_ptr<float>(a[12]), *dgk = opt_ptr<float>(a[13]);
+    auto go = [&](void* wp, size_t wn) {
+        return b200attn_rotary_bwd(dyq, dyk, r.n.y_layout, xq, xk, xd, r.n.x_layout, sq, sk, gq, gk, r.n.cos_t, r.n.sin_t, r.pos, r.n_pos, r.R,
+                                   r.pairs, dxq, dxk, dgq, dgk, r.n.B, r.n.T, r.Hq, r.Hkv, D, wp, wn, st);
+    };
+    if (norm) return finish(with_scratch(c, b200attn_rope_norm_bwd_workspace_bytes(D), go), fn);
+    int rc;
+    {
+        const NoGil no_gil;
+        rc = go(nullptr, 0);
+    }
+    return finish(rc, fn);
+    B200ATTN_CATCH
+}
+
+// T_max, rotary_dim, base, scaling (a number), factor, trained, turns_fast, turns_slow, cos, sin
+PyObject* rotary_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "make_rotary_cache";
+    B200ATTN_TRY
+    if (!arg_count(n, 10)) return nullptr;
+    int d[2], scaling;
+    double v[5];
+    if (!ints(a, 2, d) || !ints(a + 3, 1, &scaling)) return nullptr;
+    for (int i = 0; i < 5; ++i) {
+        v[i] = PyFloat_AsDouble(a[i == 0 ? 2 : 3 + i]);
+        if (v[i] == -1.0 && PyErr_Occurred()) return nullptr;
+    }
+    const Item items[] = {{a[8], "cos", ScalarType::Float}, {a[9], "sin", ScalarType::Float}};
+    if (!check_tensors(fn, items, 2)) return nullptr;
+    if (numel(a[8]) != int64_t(d[0]) * (d[1] / 2) || numel(a[9]) != numel(a[8])) return value_error("%s: shape mismatch", fn);
+    const Call c(a[8]);
+    return finish(b200attn_rotary_table(d[0], d[1], v[0], scaling, v[1], v[2], v[3], v[4], static_cast<float*>(ptr(a[8])),
+                                        static_cast<float*>(ptr(a[9])), c.st()), fn);
+    B200ATTN_CATCH
+}
+
 #define B200ATTN_FAST(name) \
     { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
     B200ATTN_FAST(fwd),      B200ATTN_FAST(bwd),      B200ATTN_FAST(decode),      B200ATTN_FAST(kv_append),
     B200ATTN_FAST(kv_attend), B200ATTN_FAST(rope_fwd), B200ATTN_FAST(rope_bwd),    B200ATTN_FAST(rope_fwd_qk),
-    B200ATTN_FAST(rope_bwd_qk), {"release_scratch", release_scratch, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    B200ATTN_FAST(rope_bwd_qk), B200ATTN_FAST(rotary_fwd), B200ATTN_FAST(rotary_bwd), B200ATTN_FAST(rotary_table), {"release_scratch", release_scratch, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

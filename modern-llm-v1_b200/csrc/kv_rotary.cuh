@@ -1,0 +1,104 @@
+// KV-cache append for caches whose rows and positions part ways: behind a prompt that several sequences share a token's position
+// is the prompt's length plus its own row, and an eviction takes rows away, not positions.  kv_append_kernel (kv_cache.cuh) has
+// one number for both, the reference's rotation and the norm always; here are all forms of rotary.cuh, and every k row's position
+// is noted where the cache keeps positions.
+//
+//   q rows [B, n_new, Hq, D]  -> rotated at pos + t (norm) -> BF16 q_out [B, Hq, n_new, D]
+//   k rows [B, n_new, Hkv, D] -> rotated at pos + t (norm) -> BF16 kcache[b, h, row + t, :],  positions[b, h, row + t] = pos + t
+//   v rows                    -> BF16 vcache[b, h, row + t, :]
+//
+// The same deal of rows to lanes as kv_append_kernel: latency at one token, HBM bytes for a prompt.  The row arithmetic is rotary.cuh's,
+// so a cache filled token by token has the bits of one filled from rotary_forward.
+#pragma once
+
+#include "kv_cache.cuh"
+#include "rotary.cuh"
+
+namespace b200attn {
+
+struct KvRotaryParams : KvAppendParams {
+    const int* rows;  // [B] first cache row per sequence, or nullptr: row0
+    int* positions;   // [B, Hkv, L_cap] or nullptr
+    int row0, n_pos, R;
+};
+
+template <int D, bool F32, bool HALF, bool NORM>
+__global__ void __launch_bounds__(kKvAppendThreads)
+kv_rotary_kernel(const __grid_constant__ KvRotaryParams p) {
+    constexpr int LPR = D / 8, RPS = 32 / LPR;
+    const int lane = threadIdx.x & 31, sub = lane / LPR, li = lane % LPR;
+    const unsigned warp0 = (blockIdx.x * kKvAppendThreads + threadIdx.x) >> 5, n_warps = (gridDim.x * kKvAppendThreads) >> 5;
+    const unsigned n_rows = p.rows_q + 2u * p.rows_kv;
+    RotaryLane<D, HALF> rl(p.R, lane, li);
+    if (p.n_new == 1) grid_dep_launch();  // (as in kv_append_kernel)
+    grid_dep_wait();
+
+    for (unsigned long long r0 = static_cast<unsigned long long>(warp0) * RPS; r0 < n_rows; r0 += static_cast<unsigned long long>(n_warps) * RPS) {
+        const bool live = r0 + sub < n_rows;
+        unsigned r = unsigned(r0 + sub);
+        int which = 0;  // 0 q, 1 k, 2 v
+        if (live && r >= p.rows_q) {
+            r -= p.rows_q;
+            which = 1;
+            if (r >= p.rows_kv) r -= p.rows_kv, which = 2;
+        }
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, rot[8], gm[8];
+        int b = 0, t = 0, h = 0;
+        long long pos = 0, row = 0;
+        int bad = 0;
+        if (live) {
+            const int H = which == 0 ? p.Hq : p.Hkv;
+            const unsigned bt = fastdiv(r, which == 0 ? p.div_hq : p.div_hkv);
+            h = int(r - bt * unsigned(H));
+            b = int(fastdiv(bt, p.div_n));
+            t = int(bt - unsigned(b) * unsigned(p.n_new));
+            pos = p.pos ? __ldg(p.pos + b) : p.pos0;
+            row = p.rows ? __ldg(p.rows + b) : p.row0;
+            // (all of a sequence's new tokens or none)
+            if (row < 0 || row + p.n_new > p.L_cap) bad = DEV_KV_CACHE_OVERFLOW;
+            else if (pos < 0 || pos + p.n_new > p.n_pos) bad = DEV_ROTARY_POSITION;
+            if (bad) pos = row = 0;
+            pos += t, row += t;
+            rn_load8<F32>(which == 0 ? p.xq : which == 1 ? p.xk : p.xv, static_cast<long long>(r) * D + li * 8, v);
+            if (NORM && which != 2) {
+                const float* gamma = which == 0 ? p.gamma_q : p.gamma_k;
+                const float4 g0 = *reinterpret_cast<const float4*>(gamma + li * 8), g1 = *reinterpret_cast<const float4*>(gamma + li * 8 + 4);
+                gm[0] = g0.x, gm[1] = g0.y, gm[2] = g0.z, gm[3] = g0.w, gm[4] = g1.x, gm[5] = g1.y, gm[6] = g1.z, gm[7] = g1.w;
+            }
+        }
+        // (a position that the tables do not have reads their first rows: t < n_new <= n_pos was checked by the host)
+        rl.load(p.cos_t, p.sin_t, p.R, li, pos);
+        rl.template rotate<false>(v, rot);  // every lane takes part in the shuffles
+        float ss = 0.f;
+        if constexpr (NORM) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) ss += rot[e] * rot[e] + rot[e + 1] * rot[e + 1];
+            ss = rn_row_sum<LPR>(ss);
+        }
+        if (!live) continue;
+        if (bad) {
+            if (li == 0) atomicCAS(p.status, 0, bad);
+            continue;
+        }
+        const long long at = (static_cast<long long>(b) * p.Hkv + h) * p.L_cap + row;  // of k and v rows
+        if (which == 2) {
+            rn_store8<false>(p.vcache, at * D + li * 8, v);
+            continue;
+        }
+        if constexpr (NORM) {
+            const float rstd = rn_rstd<D>(ss, p.eps);
+            float out[8];
+            rn_scale8(rot, rstd, gm, out);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rot[e] = out[e];
+        }
+        if (which == 0) {
+            rn_store8<false>(p.q_out, ((static_cast<long long>(b) * p.Hq + h) * p.n_new + t) * D + li * 8, rot);
+        } else {
+            rn_store8<false>(p.kcache, at * D + li * 8, rot);
+            if (p.positions && li == 0) p.positions[at] = int(pos);
+        }
+    }
+}
+
+}  // namespace b200attn

@@ -1,0 +1,271 @@
+// Rotary positions in every layout a model may have been trained with, on the way into the attention kernels and back: pairs of
+// neighbours or of the two halves, the first R of a head's D elements, a position per token, with or without the QK-norm behind.
+// (rope_norm.cuh is the reference's one form of it: all of the head, neighbours, the norm always, llm/src/model/rope.cu:25-65.)
+//
+//   the pair i < R / 2 of a row at position p is  (a, b) = (x[2i], x[2i+1])  or  (x[i], x[i + R/2])
+//   r: (a cos - b sin, a sin + b cos) with cos, sin = tables[p][i];  elements >= R stay
+//   y = r, or with the norm  rstd = rsqrt(mean r^2 + eps), y = r rstd gamma
+//   back, with the norm:  g = dy gamma, s = sum g r, dr = rstd g - rstd^3 / D s r, d_gamma += sum over rows of dy r rstd;
+//   without it dr = dy (x is not read);  dx: (da cos + db sin, -da sin + db cos)
+//
+// Bound by HBM like rope_norm.cuh, whose deal of the work this is: a lane owns 8 consecutive elements, a warp 256 / D tokens and a
+// chunk of heads, so that a token's cosines and sines stay in registers.  Where the halves are paired, an element's partner lies
+// R / 16 lanes further (R is a multiple of 16: never inside a lane) and comes by shuffle; loading it a second time instead would
+// double the requests to L1.
+#pragma once
+
+#include "rope_norm.cuh"
+
+namespace b200attn {
+
+struct RotaryParams : RopeNormParams {
+    const int* pos;  // [B, T] positions, or nullptr: token t has position t
+    int n_pos;       // rows of the tables [n_pos, R / 2]
+    int R;
+    int* status;     // set to DEV_ROTARY_POSITION when a position is not a row of the tables (the token's rows are skipped)
+};
+
+// A lane's share of one row of the tables
+template <int D, bool HALF>
+struct RotaryLane {
+    float c[HALF ? 8 : 4], s[HALF ? 8 : 4];
+    bool turns;   // the lane's elements are rotated
+    int partner;  // HALF: the lane that has the pairs' other elements
+    // li: the lane within its row's D / 8
+    __device__ __forceinline__ RotaryLane(int R, int lane, int li) {
+        turns = li * 8 < R;
+        const int half = R / 16;  // lanes
+        partner = !turns ? lane : li < half ? lane + half : lane - half;
+    }
+    __device__ __forceinline__ void load(const float* cos_t, const float* sin_t, int R, int li, long long pos) {
+        if (!turns) {
+#pragma unroll
+            for (int e = 0; e < (HALF ? 8 : 4); ++e) c[e] = 1.f, s[e] = 0.f;
+            return;
+        }
+        const int half = R / 16;
+        const bool first = li < half;
+        const long long at = pos * (R / 2) + (HALF ? (first ? li : li - half) * 8 : li * 4);
+#pragma unroll
+        for (int e = 0; e < (HALF ? 8 : 4); e += 4) {
+            const float4 cv = *reinterpret_cast<const float4*>(cos_t + at + e), sv = *reinterpret_cast<const float4*>(sin_t + at + e);
+            c[e] = cv.x, c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
+            s[e] = sv.x, s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
+            if (HALF && first) {  // (the first half of a pair: a cos - b sin)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[e + k] = -s[e + k];
+            }
+        }
+    }
+    // BACK: by the opposite angle.  Every lane of the warp takes part.
+    template <bool BACK>
+    __device__ __forceinline__ void rotate(const float (&v)[8], float (&out)[8]) const {
+        if constexpr (HALF) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float o = __shfl_sync(0xffffffffu, v[e], partner);
+                // (elements that do not turn are copied: times one plus zero times another would make NaN of infinities)
+                out[e] = !turns ? v[e] : BACK ? v[e] * c[e] - o * s[e] : v[e] * c[e] + o * s[e];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = v[2 * i], b = v[2 * i + 1];
+                out[2 * i] = !turns ? a : BACK ? a * c[i] + b * s[i] : a * c[i] - b * s[i];
+                out[2 * i + 1] = !turns ? b : BACK ? b * c[i] - a * s[i] : a * s[i] + b * c[i];
+            }
+        }
+    }
+};
+
+// The position of a lane's token; a token whose position the tables do not have is dropped (live = false).
+template <int D>
+__device__ __forceinline__ int rotary_position(const RotaryParams& p, RnItem<D>& it) {
+    if (!p.pos || !it.live) return it.live ? it.t : 0;
+    const int pos = __ldg(p.pos + static_cast<long long>(it.b) * p.T + it.t);
+    if (pos >= 0 && pos < p.n_pos) return pos;
+    it.live = false;
+    atomicCAS(p.status, 0, int(DEV_ROTARY_POSITION));
+    return 0;
+}
+
+template <int D, bool F32, bool HALF, bool NORM>
+__device__ __forceinline__ unsigned rotary_fwd_tensor(const RotaryParams& p, unsigned item, unsigned n_warps) {
+    constexpr int LPR = D / 8;
+    constexpr int kUnroll = 4;
+    const int lane = threadIdx.x & 31;
+    const int sub = lane / LPR, li = lane % LPR;
+    RotaryLane<D, HALF> rl(p.R, lane, li);
+    float gm[8];
+    if constexpr (NORM) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gm[e] = p.gamma[li * 8 + e];
+    }
+    for (; item < p.n_items; item += n_warps) {
+        RnItem<D> it(p, item, sub);
+        rl.load(p.cos_t, p.sin_t, p.R, li, rotary_position<D>(p, it));
+        const long long x_off = it.b * p.x_sb + it.t * p.x_st + li * 8, y_off = it.b * p.y_sb + it.t * p.y_st + li * 8;
+        float* rstd_t = NORM ? p.rstd + static_cast<long long>(it.b) * p.H * p.T + it.t : nullptr;
+        for (int h = it.h0; h < it.h1; h += kUnroll) {
+            RnRaw<F32> raw[kUnroll];
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                raw[k].clear();
+                if (it.live && h + k < it.h1) raw[k].load(p.x, x_off + (h + k) * p.x_sh);
+            }
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                if (h + k >= it.h1) break;
+                float v[8], rot[8];
+                raw[k].get(v);
+                rl.template rotate<false>(v, rot);
+                if constexpr (NORM) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) ss += rot[e] * rot[e] + rot[e + 1] * rot[e + 1];
+                    const float rstd = rn_rstd<D>(rn_row_sum<LPR>(ss), p.eps);
+                    float out[8];
+                    rn_scale8(rot, rstd, gm, out);
+                    if (it.live) {
+                        rn_store8<false>(p.y, y_off + (h + k) * p.y_sh, out);
+                        if (li == 0) rstd_t[static_cast<long long>(h + k) * p.T] = rstd;
+                    }
+                } else if (it.live) {
+                    rn_store8<false>(p.y, y_off + (h + k) * p.y_sh, rot);
+                }
+            }
+        }
+    }
+    return item - p.n_items;
+}
+
+template <int D, bool F32, bool HALF, bool NORM>
+__global__ void __launch_bounds__(kRopeNormThreads, kRopeNormFwdBlocks)
+rotary_fwd_kernel(const __grid_constant__ RotaryParams p0, const __grid_constant__ RotaryParams p1) {
+    const unsigned warp = (blockIdx.x * kRopeNormThreads + threadIdx.x) >> 5, n_warps = (gridDim.x * kRopeNormThreads) >> 5;
+    grid_dep_wait();
+    const unsigned next = rotary_fwd_tensor<D, F32, HALF, NORM>(p0, warp, n_warps);
+    rotary_fwd_tensor<D, F32, HALF, NORM>(p1, next, n_warps);
+}
+
+// One tensor's backward; with the norm it leaves this CTA's d_gamma sums in p.partial, which rope_norm_dgamma_kernel adds up.
+template <int D, bool F32, bool HALF, bool NORM>
+__device__ __forceinline__ unsigned rotary_bwd_tensor(const RotaryParams& p, unsigned item, unsigned n_warps, float (*s_part)[D]) {
+    constexpr int LPR = D / 8;
+    constexpr int kUnroll = NORM ? 2 : 4;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = lane / LPR, li = lane % LPR;
+    RotaryLane<D, HALF> rl(p.R, lane, li);
+    float gm[8], dg[8];
+    if constexpr (NORM) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gm[e] = p.gamma[li * 8 + e], dg[e] = 0.f;
+    }
+    for (; item < p.n_items; item += n_warps) {
+        RnItem<D> it(p, item, sub);
+        rl.load(p.cos_t, p.sin_t, p.R, li, rotary_position<D>(p, it));
+        const long long x_off = it.b * p.x_sb + it.t * p.x_st + li * 8, y_off = it.b * p.y_sb + it.t * p.y_st + li * 8;
+        const float* rstd_t = NORM ? p.rstd + static_cast<long long>(it.b) * p.H * p.T + it.t : nullptr;
+        for (int h = it.h0; h < it.h1; h += kUnroll) {
+            RnRaw<F32> raw_x[NORM ? kUnroll : 1];
+            RnRaw<false> raw_dy[kUnroll];
+            float rstd[kUnroll];
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                if constexpr (NORM) raw_x[k].clear();
+                raw_dy[k].clear();
+                rstd[k] = 0.f;
+                if (it.live && h + k < it.h1) {
+                    raw_dy[k].load(p.dy, y_off + (h + k) * p.y_sh);
+                    if constexpr (NORM) {
+                        raw_x[k].load(p.x, x_off + (h + k) * p.x_sh);
+                        rstd[k] = rstd_t[static_cast<long long>(h + k) * p.T];
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                if (h + k >= it.h1) break;
+                float d[8], dx[8];
+                raw_dy[k].get(d);
+                if constexpr (NORM) {
+                    float v[8], rot[8];
+                    raw_x[k].get(v);
+                    rl.template rotate<false>(v, rot);
+                    const float rs = rstd[k];
+                    float s = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float g = d[e] * gm[e];
+                        s += g * rot[e];
+                        dg[e] += d[e] * rot[e] * rs;
+                        d[e] = g;
+                    }
+                    s = rn_row_sum<LPR>(s);
+                    const float coeff = rs * rs * rs * (1.f / float(D)) * s;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) d[e] = rs * d[e] - coeff * rot[e];
+                }
+                rl.template rotate<true>(d, dx);
+                if (it.live) rn_store8<F32>(p.y, x_off + (h + k) * p.x_sh, dx);
+            }
+        }
+    }
+    if constexpr (NORM) {  // as in rope_norm_bwd_tensor: the lanes with the same columns, then the CTA's warps, in a fixed order
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+#pragma unroll
+            for (int o = LPR; o < 32; o <<= 1) dg[e] += __shfl_xor_sync(0xffffffffu, dg[e], o);
+        }
+        if (sub == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s_part[warp][li * 8 + e] = dg[e];
+        }
+        __syncthreads();
+        for (int d = threadIdx.x; d < D; d += kRopeNormThreads) {
+            float acc = 0.f;
+#pragma unroll
+            for (int w = 0; w < kRopeNormThreads / 32; ++w) acc += s_part[w][d];
+            p.partial[static_cast<long long>(blockIdx.x) * D + d] = acc;
+        }
+    }
+    return item - p.n_items;
+}
+
+template <int D, bool F32, bool HALF, bool NORM>
+__global__ void __launch_bounds__(kRopeNormThreads, kRopeNormBwdBlocks)
+rotary_bwd_kernel(const __grid_constant__ RotaryParams p0, const __grid_constant__ RotaryParams p1) {
+    __shared__ float s_part[2][NORM ? kRopeNormThreads / 32 : 1][D];
+    const unsigned warp = (blockIdx.x * kRopeNormThreads + threadIdx.x) >> 5, n_warps = (gridDim.x * kRopeNormThreads) >> 5;
+    grid_dep_wait();
+    const unsigned next = rotary_bwd_tensor<D, F32, HALF, NORM>(p0, warp, n_warps, s_part[0]);
+    rotary_bwd_tensor<D, F32, HALF, NORM>(p1, next, n_warps, s_part[1]);
+}
+
+// The tables: angle = position * frequency of the pair, in 64 bits (in 32 a position of 30000 turns the fastest pair by up to
+// 2^-9 too far), rounded once as cosine and sine.  The frequencies come from base^(-2i/R), see b200attn_rotary_table for `scaling`.
+struct RotaryTableParams {
+    int T, half;
+    double base, divide;                       // frequency base^(-i / half) / divide
+    double trained, factor, fast, slow;        // by parts (trained > 0): frequencies that turn less often lie below
+    float *cos_t, *sin_t;
+};
+__global__ void __launch_bounds__(256) rotary_table_kernel(const RotaryTableParams p) {
+    const long long n = static_cast<long long>(p.T) * p.half;
+    grid_dep_wait();
+    for (long long k = blockIdx.x * 256ll + threadIdx.x; k < n; k += gridDim.x * 256ll) {
+        const int t = int(k / p.half), i = int(k - static_cast<long long>(t) * p.half);
+        double freq = pow(p.base, -double(i) / double(p.half)) / p.divide;
+        if (p.trained > 0.0) {
+            const double turns = p.trained * freq * 0.15915494309189535;  // within the trained length
+            const double keep = fmin(fmax((turns - p.slow) / (p.fast - p.slow), 0.0), 1.0);
+            freq = freq * keep + freq / p.factor * (1.0 - keep);
+        }
+        double sn, cs;
+        sincos(double(t) * freq, &sn, &cs);
+        p.cos_t[k] = float(cs);
+        p.sin_t[k] = float(sn);
+    }
+}
+
+}  // namespace b200attn
