@@ -48,7 +48,8 @@ enum {
     B200ATTN_ERR_DEVICE_WAIT = 7,  /* a kernel gave up on a bounded wait (see b200attn_last_device_status) */
     B200ATTN_ERR_NO_DEVICE = 8,    /* no sm_100 device is current */
     B200ATTN_ERR_TOO_LARGE = 9     /* problem too large: beyond the fixed scratch of b200attn_bwd_static (524288 rows), or
-                                      2^31 or more rows in a RoPE / QK-Norm / KV-append call */
+                                      2^31 or more rows in a RoPE / QK-Norm / KV-append call, or of units
+                                      of work in a call of the long-context operators */
 };
 
 enum { B200ATTN_LAYOUT_BHTD = 0, B200ATTN_LAYOUT_BTHD = 1 };
@@ -312,6 +313,50 @@ int b200attn_kv_append_rotary(const void* xq, const void* xk, const void* xv, in
                               const float* cos_t, const float* sin_t, int n_pos, int R, int pairs, const int* pos,
                               int pos0, const int* rows, int row0, int B, int n_new, int L_cap, int Hq, int Hkv, int D,
                               float eps, void* stream);
+
+/*
+ * Sampling from long contexts (the reference keeps no cache at all, llm/apps/infer_modern_gpt.cu:253-255).
+ *
+ * b200attn_decode_shared: one query token per sequence, for sequences of which B / G each continue one of G prompts (sequence b
+ * continues prompt b / (B / G)).  A prompt's keys and values are read once for all its sequences.
+ *   q, o [B, Hq, D]; lse [B, Hq] or NULL; kprefix, vprefix [G, Hkv, P_cap, D], of which the first prefix_lens[g] rows count
+ *   (device, int32, clamped to 0 .. P; NULL: P); kcache, vcache [B, Hkv, L_cap, D], of which the first lens[b] rows count (clamped
+ *   to 1 .. L; NULL: L).  o = softmax(scale q [Kprefix; K]^T) [Vprefix; V].  Rows that do not count may hold anything.
+ *
+ * b200attn_decode_weights: b200attn_decode_ragged that also adds every key's probability to its weight:
+ *   weights[b, hk, key] += sum over the heads h of the group of exp(scale q_h . k_key - lse_h),  weights [B, Hkv, L_cap] FP32, keys
+ *   0 .. lens[b] - 1 (lens clamped to 1 .. L; NULL: L).  lse may be NULL.  Rows beyond a sequence's length may hold anything.
+ *
+ * b200attn_key_weights: the same sums over a chunk of T new tokens at positions (rows) pos0 .. pos0 + T - 1 of the cache, each of
+ *   which sees the keys up to its own, from the lse [B, Hq, T] that b200attn_fwd_kvcache_at has left; q [.., T, ..] in q_layout.
+ *   Keys 0 .. pos0 + T - 1.  For the sums over the last tokens of a prompt only, pass these tokens' q, lse and position.
+ *
+ * b200attn_kv_evict: of each (batch, KV head)'s first n = lens[b] rows (clamped to 0 .. L; NULL: L) min(n, keep) stay: the rows whose
+ *   position is above newest - recent (the newest being the largest of the n positions, which are distinct; recent <= keep), then those of
+ *   the largest weight (NaN above all numbers), of equal ones the lower row.  Rows that stay and lie below `keep` stay where they are; the j-th
+ *   of the others goes to the j-th free place below `keep`.  K and V [B, Hkv, L_cap, D] change in place (rows behind the first min(n, keep)
+ *   keep their bytes); weights_out and positions_out [B, Hkv, L_cap] are written whole, 0 and -1 behind the rows that stayed, and must not
+ *   overlap weights and positions, which are only read.
+ *
+ * Sums are FP32 and in a fixed order: a call repeats bit for bit.  Workspaces: at least ..._workspace_bytes(...), 256-byte aligned, without
+ * initialisation; calls that may overlap need workspaces of their own.  Nothing is written while the device status word is set.
+ */
+int b200attn_decode_shared(const void* q, const void* kprefix, const void* vprefix, const void* kcache, const void* vcache,
+                           void* o, float* lse, const int* prefix_lens, const int* lens, int B, int G, int P, int P_cap,
+                           int L, int L_cap, int Hq, int Hkv, int D, float softmax_scale, void* workspace,
+                           size_t workspace_bytes, void* stream);
+size_t b200attn_decode_shared_workspace_bytes(int B, int G, int P, int L, int Hq, int Hkv, int D);
+int b200attn_decode_weights(const void* q, const void* kcache, const void* vcache, void* o, float* lse, float* weights,
+                            const int* lens, int B, int L, int L_cap, int Hq, int Hkv, int D, float softmax_scale,
+                            void* workspace, size_t workspace_bytes, void* stream);
+size_t b200attn_decode_weights_workspace_bytes(int B, int L, int Hq, int Hkv, int D);
+int b200attn_key_weights(const void* q, int q_layout, const void* kcache, const float* lse, float* weights, int B, int T,
+                         int pos0, int L_cap, int Hq, int Hkv, int D, float softmax_scale, void* workspace,
+                         size_t workspace_bytes, void* stream);
+size_t b200attn_key_weights_workspace_bytes(int B, int T, int pos0, int Hkv);
+int b200attn_kv_evict(void* kcache, void* vcache, const float* weights, const int* positions, float* weights_out,
+                      int* positions_out, const int* lens, int B, int L, int L_cap, int Hkv, int D, int keep, int recent,
+                      void* stream);
 
 /*
  * Diagnostics for benchmarks (no counterpart in the reference): when three CUDA events are

@@ -13,10 +13,13 @@ from .flash_attn import (  # noqa: F401
     flash_attn_backward,
     flash_attn_backward_gqa,
     flash_attn_decode,
+    flash_attn_decode_shared,
+    flash_attn_decode_weights,
     flash_attn_forward,
     flash_attn_forward_gqa,
+    flash_attn_key_weights,
 )
-from .kv_cache import KVCache  # noqa: F401
+from .kv_cache import KVCache, kv_evict  # noqa: F401
 from .rope_norm import (  # noqa: F401
     make_rope_cache,
     rope_qknorm_backward,
@@ -42,4 +45,8 @@ __all__ = [
     "make_rotary_cache",
     "rotary_forward",
     "rotary_backward",
+    "flash_attn_decode_shared",
+    "flash_attn_decode_weights",
+    "flash_attn_key_weights",
+    "kv_evict",
 ]

@@ -68,6 +68,13 @@ SYMBOLS = (
     "b200attn_rotary_fwd",
     "b200attn_rotary_bwd",
     "b200attn_kv_append_rotary",
+    "b200attn_decode_shared",
+    "b200attn_decode_shared_workspace_bytes",
+    "b200attn_decode_weights",
+    "b200attn_decode_weights_workspace_bytes",
+    "b200attn_key_weights",
+    "b200attn_key_weights_workspace_bytes",
+    "b200attn_kv_evict",
     "b200attn_last_device_status",
     "b200attn_strerror",
     "b200attn_version",
@@ -164,6 +171,20 @@ def load() -> ctypes.CDLL:
     L.b200attn_rotary_bwd.restype = i
     L.b200attn_kv_append_rotary.argtypes = [vp] * 3 + [i] + [vp] * 8 + [i] * 3 + [vp, i, vp, i] + [i] * 6 + [f, vp]
     L.b200attn_kv_append_rotary.restype = i
+    L.b200attn_decode_shared.argtypes = [vp] * 9 + [i] * 9 + [f, vp, sz, vp]
+    L.b200attn_decode_shared.restype = i
+    L.b200attn_decode_shared_workspace_bytes.argtypes = [i] * 7
+    L.b200attn_decode_shared_workspace_bytes.restype = sz
+    L.b200attn_decode_weights.argtypes = [vp] * 7 + [i] * 6 + [f, vp, sz, vp]
+    L.b200attn_decode_weights.restype = i
+    L.b200attn_decode_weights_workspace_bytes.argtypes = [i] * 5
+    L.b200attn_decode_weights_workspace_bytes.restype = sz
+    L.b200attn_key_weights.argtypes = [vp, i, vp, vp, vp] + [i] * 7 + [f, vp, sz, vp]
+    L.b200attn_key_weights.restype = i
+    L.b200attn_key_weights_workspace_bytes.argtypes = [i] * 4
+    L.b200attn_key_weights_workspace_bytes.restype = sz
+    L.b200attn_kv_evict.argtypes = [vp] * 7 + [i] * 7 + [vp]
+    L.b200attn_kv_evict.restype = i
     L.b200attn_last_device_status.argtypes = [vp]
     L.b200attn_last_device_status.restype = i
     L.b200attn_strerror.argtypes = [i]

@@ -21,7 +21,7 @@ NVCC_FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",
     "-Xcompiler", "-fPIC",
 ]
-CUDA_SOURCES = ["b200attn_api.cu", "rotary_api.cu"]
+CUDA_SOURCES = ["b200attn_api.cu", "rotary_api.cu", "context_api.cu"]
 
 
 def sources() -> list[str]:

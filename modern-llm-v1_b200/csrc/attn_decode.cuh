@@ -39,6 +39,23 @@
 
 namespace b200attn {
 
+// What the kernel does besides: nothing; or it leaves the scores for the kernel that adds up the keys' weights (key_weights.cuh); or
+// its softmax goes on over the partial results of a prompt that several sequences share (attn_prefix.cuh).  In the latter two, rows
+// beyond a sequence's length may hold anything, NaN included: their V rows are cleared in shared memory (one tile of a sequence; in
+// the plain kernel, whose caches hold finite values everywhere, that would cost the tile for nothing).
+enum { kDecodePlain = 0, kDecodeScores = 1, kDecodeShared = 2 };
+
+// The partial results of attn_prefix.cuh: per (prompt, KV head, chunk of the group's heads, tile of 128 rows) and split a slot of 128
+// rows, a row being (sequence within the prompt's, head within the chunk).
+struct DecodePrefix {
+    const float* o;    // [slot][D / 4][128 rows][4]  un-normalised
+    const float2* ml;  // [slot][128 rows]  reference of the exponents in raw score units, sum; (-inf, 0): no keys
+    int splits, tiles; // slots per tile of rows, tiles per chunk
+    FastDiv div_n;     // sequences per prompt
+    FastDiv div_heads, div_seqs;  // heads per chunk, sequences per tile
+    int n_chunks, Hkv;
+};
+
 struct DecodeParams {
     int B, L, Hq, Hkv, group;
     int G;         // query heads per unit (a divisor of group, <= 16)
@@ -61,6 +78,8 @@ struct DecodeParams {
                                    // (not where a cluster shares it)
     unsigned long long tag;        // of this launch
     int* status;                   // status word and epoch
+    float* scores;                 // kDecodeScores: [unit][L][G] in raw score units
+    DecodePrefix prefix;           // kDecodeShared
 };
 
 constexpr int kDecodeMaxCtas = 320, kDecodeMaxCluster = 8, kDecodeThreads = 192;
@@ -399,8 +418,52 @@ __device__ __forceinline__ int decode_count(unsigned long long* word, unsigned l
     return int(atomicAdd(word, 1ull) - tag) + 1;
 }
 
+// One pair of output elements (columns d, d + 1 of head j of the group) joined with the prompt's partial results, in the order of the
+// splits; false: a kernel has failed and nothing may be written.  This is the first look at what the kernel in front, which computes
+// them, has written: all else this kernel reads was there before that one began (see grid_dep_launch in attn_prefix.cuh), so its loads
+// run beside it.  (The chain is two round trips through L2 whatever the number of splits up to eight.)
+template <int D>
+__device__ __forceinline__ bool decode_add_prefix(const DecodeParams& p, int b, int hk, int j, int d, float& a0, float& a1, float& m, float& l) {
+    const DecodePrefix& x = p.prefix;
+    grid_dep_wait();
+    const int status = *reinterpret_cast<volatile int*>(p.status);
+    const int prompt = int(fastdiv(b, x.div_n)), seq = b - prompt * int(x.div_n.d);
+    const int chunk = int(fastdiv(j, x.div_heads)), tile = int(fastdiv(seq, x.div_seqs));
+    const int row = (seq - tile * int(x.div_seqs.d)) * int(x.div_heads.d) + j - chunk * int(x.div_heads.d);
+    const size_t slot0 = (size_t((prompt * x.Hkv + hk) * x.n_chunks + chunk) * x.tiles + tile) * x.splits;
+    const float* o = x.o + (slot0 * (D / 4) + d / 4) * 512 + row * 4 + (d & 3);
+    const float2* ml = x.ml + slot0 * 128 + row;
+    constexpr int N = 8;
+    for (int s0 = 0; s0 < x.splits; s0 += N) {
+        float2 pml[N], po[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            pml[k] = make_float2(-INFINITY, 0.f), po[k] = make_float2(0.f, 0.f);
+            if (s0 + k < x.splits) {
+                pml[k] = __ldcg(ml + (s0 + k) * 128);
+                po[k] = __ldcg(reinterpret_cast<const float2*>(o + size_t(s0 + k) * (D * 128)));
+            }
+        }
+        float mn = m;
+#pragma unroll
+        for (int k = 0; k < N; ++k) mn = fmaxf(mn, pml[k].x);
+        const float fa = m == -INFINITY ? 1.f : ex2_approx((m - mn) * p.scale_log2);  // (m = -inf: no score above it, l is 0 or NaN)
+        l *= fa, a0 *= fa, a1 *= fa;
+        m = mn;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (pml[k].x == -INFINITY && pml[k].y == 0.f) continue;  // no keys: nothing else was written
+            const float f = pml[k].x == -INFINITY ? 1.f : ex2_approx((pml[k].x - mn) * p.scale_log2);
+            l += f * pml[k].y;
+            a0 += f * po[k].x;
+            a1 += f * po[k].y;
+        }
+    }
+    return status == 0;
+}
+
 // PF: tiles that a CTA brings into L2 while the kernel in front of this one ends
-template <int D, int NH, int PF>
+template <int D, int NH, int PF, int MODE = kDecodePlain>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
 attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const DecodeParams p) {
@@ -449,7 +512,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         __syncwarp();
         // everything above overlaps the previous kernel's end (the cache append that wrote q and the newest K / V row)
-        grid_dep_wait();
+        if (MODE != kDecodeShared) grid_dep_wait();
         DecodeWalk w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane);
         int j = 0;  // tiles issued so far (ring position)
         bool synced = false, ok = true;
@@ -494,8 +557,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 
     auto write_rows_of = [&](const DecodeWalk& w) {  // final rows of the unit at w
         const int hk = int(fastdiv(w.u, p.div_chunks));
-        const size_t row0 = size_t(w.b) * p.Hq + hk * p.group + (w.u - hk * p.n_chunks) * G;
-        return [&p, row0](int g, int d, float a0, float a1, float m, float l) {
+        const int j0 = (w.u - hk * p.n_chunks) * G, b = w.b;
+        const size_t row0 = size_t(b) * p.Hq + hk * p.group + j0;
+        return [&p, row0, b, hk, j0](int g, int d, float a0, float a1, float m, float l) {
+            if (MODE == kDecodeShared && !decode_add_prefix<D>(p, b, hk, j0 + g, d, a0, a1, m, l)) return;
             const float inv = 1.f / l;
             reinterpret_cast<uint32_t*>(p.o)[(row0 + g) * (D / 2) + d / 2] = pack_bf16x2(a0 * inv, a1 * inv);
             if (p.lse && d == 0) p.lse[row0 + g] = m * p.scale + logf(l);
@@ -519,7 +584,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 __syncwarp();
             });
         }
-        grid_dep_wait();
+        if (MODE != kDecodeShared) grid_dep_wait();
         const DecodeWalk w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane);
         named_bar_sync(kDecodeCountBar, kDecodeThreads);
         if (p.shares || *fail_flag != 0 || w.t >= w.t_end) return;
@@ -549,7 +614,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const int buf = i / ((16 - G) * (D / 8)), r = i % ((16 - G) * (D / 8));
         *reinterpret_cast<uint4*>(sQ + buf * Cfg::kQBytes + (G + r / (D / 8)) * Cfg::kQRow + (r % (D / 8)) * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
-    grid_dep_wait();
+    if (MODE != kDecodeShared) grid_dep_wait();
     // (a launch behind a failure writes nothing; its loads are harmless, but shared memory has to outlive them)
     if (tid == 0) {
         *fail_flag = *reinterpret_cast<volatile int*>(p.status);
@@ -611,6 +676,12 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             // ---- mask keys beyond the cache length (a unit's last tile only)
             const int tile_key = (w.j0 + i) * KEYS;
             if (tile_key + KEYS > w.len) {
+                if (MODE != kDecodePlain) {  // this warp's V rows of them
+                    for (int r = kw; r < kw + KEYS / 4; ++r)
+                        if (tile_key + r >= w.len && lane < D / 8)
+                            *reinterpret_cast<uint4*>(sKV + s * 2 * Cfg::kTileBytes + Cfg::kTileBytes + swz_off(r, lane, Cfg::kBoxBytes)) = make_uint4(0u, 0u, 0u, 0u);
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int kt = 0; kt < KT; ++kt) {
                     const int key = tile_key + kw + kt * 16 + (lane >> 2);
@@ -620,6 +691,23 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         if (key + 8 >= w.len) sc[kt][nh][2] = sc[kt][nh][3] = -INFINITY;
                     }
                 }
+            }
+            if (MODE == kDecodeScores && !failed) {  // 8 keys x G heads of a store lie together
+                float* at = p.scores + (size_t(w.b * p.units_per_seq + w.u) * p.L + tile_key) * G;
+#pragma unroll
+                for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+                    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const int key = kw + kt * 16 + (lane >> 2) + e * 4, g = nh * 8 + (lane & 3) * 2;
+                            if (tile_key + key >= w.len || g >= G) continue;
+                            if (!(G & 1)) *reinterpret_cast<float2*>(at + key * G + g) = make_float2(sc[kt][nh][e], sc[kt][nh][e + 1]);
+                            else {
+                                at[key * G + g] = sc[kt][nh][e];
+                                if (g + 1 < G) at[key * G + g + 1] = sc[kt][nh][e + 1];
+                            }
+                        }
             }
             // ---- online softmax per head over this warp's keys; P^T becomes the B operand of the second product: rows and
             // columns of its 8 x 8 blocks change places (movmatrix)

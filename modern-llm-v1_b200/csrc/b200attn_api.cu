@@ -852,38 +852,6 @@ extern "C" int b200attn_bwd_static(const void* q, const void* k, const void* v, 
                              B200ATTN_BWD_TWO_PASS, scratch, 2 * sizeof(float) * (size_t)B200ATTN_BWD_STATIC_MAX_ROWS, stream);
 }
 
-namespace {
-
-template <int D, int NH, int PF>
-int launch_decode_pf(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p, int n_ctas, cudaStream_t st) {
-    using Cfg = DecodeCfg<D>;
-    static bool set[kMaxDevices] = {false};
-    int rc = set_smem_once(attn_decode_kernel<D, NH, PF>, Cfg::kSmemBytes, set);
-    if (rc) return rc;
-    if (launch_cluster(attn_decode_kernel<D, NH, PF>, dim3(n_ctas), kDecodeThreads, Cfg::kSmemBytes, st, p.cluster, tk, tv, p) != cudaSuccess) {
-        cudaGetLastError();
-        return B200ATTN_ERR_CUDA;
-    }
-    return B200ATTN_OK;
-}
-
-// Where the CTAs fill most of the device the launch is bound by HBM, and the first two tiles of each come into L2 while the kernel
-// in front ends, provided that it lets this one start early, as the append of one token and the decode itself do (us per call over
-// caches larger than L2 in turn, without / with: append + decode B=48 L<=6000 16/4 D=64 35.6 / 34.3, B=64 L<=4096 33.5 / 31.8, B=20 L<=1500
-// D=128 19.3 / 18.0; decode behind decode B=64 L=4096 16/4 D=64 41.9 / 41.3, B=300 L=200 8/8 24.0 / 22.8, B=64 L=1000 6/2 9.0 / 8.5, B=8
-// L=2000 8/8 D=128, 128 CTAs, 14.3 / 14.1).  With a matrix product in front of each append + decode, the product included: 40.6 / 39.9,
-// 38.3 / 37.5, 23.4 / 23.0.  Behind a kernel that does not release this one early the tiles are asked for twice: product and decode
-// 46.1 / 46.0, 29.8 / 29.5, 13.3 / 13.4, 19.1 / 19.3; a first pass on new buffers on an idle device gains nothing (host's time of a call,
-// B=300 41.8 / 42.1, append + decode B=48 67.3 / 67.0).  With three tiles the gain is smaller, with six it is gone.
-// Fewer CTAs are bound by latency, of which this hides nothing: B=6 L<=3000 8/1 D=128 8.5 -> 8.6, B=1 L=1500 16/4 5.26 -> 5.30.
-constexpr int kPrefetchCtas = 128;
-template <int D, int NH>
-int launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p, int n_ctas, cudaStream_t st) {
-    return n_ctas >= kPrefetchCtas ? launch_decode_pf<D, NH, 2>(tk, tv, p, n_ctas, st) : launch_decode_pf<D, NH, 0>(tk, tv, p, n_ctas, st);
-}
-
-}  // namespace
-
 extern "C" int b200attn_decode_default_splits(int B, int L, int Hq, int Hkv, int D) {
     if (B <= 0 || L <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return 0;
     return decode_plan(B, L, Hq, Hkv, D, 0, false).splits;
@@ -924,46 +892,12 @@ extern "C" int b200attn_decode_ragged(const void* q, const void* kcache, const v
     int* status = status_ptr(&rc);
     if (!status) return rc;
     const DecodePlan d = decode_plan(B, L, Hq, Hkv, D, n_splits, lens != nullptr);
-    // the maps end at row L of every (batch, head): rows of the cache beyond it are never read (TMA fills zeros)
-    const Strides sk = strides_for(B200ATTN_LAYOUT_BHTD, Hkv, L_cap, D);
     CUtensorMap tk, tv;
-    if (!make_tmap_bf16_4d(&tk, kcache, D, L, Hkv, B, sk.t, sk.h, sk.b, decode_tile_keys(D)) ||
-        !make_tmap_bf16_4d(&tv, vcache, D, L, Hkv, B, sk.t, sk.h, sk.b, decode_tile_keys(D)))
-        return B200ATTN_ERR_TENSOR_MAP;
     DecodeParams p;
-    p.B = B;
-    p.L = L;
-    p.Hq = Hq;
-    p.Hkv = Hkv;
-    p.group = Hq / Hkv;
-    p.G = d.G;
-    p.n_chunks = d.n_chunks;
-    p.units_per_seq = Hkv * d.n_chunks;
-    p.div_units = fastdiv_make((unsigned)p.units_per_seq);
-    p.div_chunks = fastdiv_make((unsigned)d.n_chunks);
-    p.div_shares = fastdiv_make((unsigned)std::max(d.shares, 1));
-    p.div_tiles = fastdiv_make((unsigned)((L + decode_tile_keys(D) - 1) / decode_tile_keys(D)));
-    p.div_slice = fastdiv_make((unsigned)(d.G * (D / 2) / d.cluster));
-    p.shares = d.shares;
-    p.cluster = d.cluster;
-    p.whole = d.whole;
-    p.slot_mode = d.slot_mode;
-    p.scale = softmax_scale > 0.f ? softmax_scale : 1.f / sqrtf((float)D);
-    p.scale_log2 = p.scale * 1.4426950408889634f;
-    p.lens = lens;
-    p.q = static_cast<const uint16_t*>(q);
-    p.o = static_cast<uint16_t*>(o);
-    p.lse = lse;
-    const size_t rows = (size_t)B * Hq * d.slots;  // slots x heads per slot
-    p.part_o = static_cast<float*>(workspace);
-    p.part_m = p.part_o + rows * D;
-    p.part_l = p.part_m + rows;
-    p.counters = reinterpret_cast<unsigned long long*>(p.part_l + rows);  // (D + 2 is even: 8-byte aligned)
-    p.tag = next_decode_tag();
-    p.status = status;
+    rc = decode_fill(d, p, tk, tv, q, kcache, vcache, o, lse, lens, B, L, L_cap, Hq, Hkv, D, softmax_scale, workspace, status);
+    if (rc) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (D == 64) return d.G <= 8 ? launch_decode<64, 1>(tk, tv, p, d.n_ctas, st) : launch_decode<64, 2>(tk, tv, p, d.n_ctas, st);
-    return d.G <= 8 ? launch_decode<128, 1>(tk, tv, p, d.n_ctas, st) : launch_decode<128, 2>(tk, tv, p, d.n_ctas, st);
+    return launch_decode<kDecodePlain>(D, tk, tv, p, d.n_ctas, st);
 }
 
 namespace {
@@ -1105,7 +1039,7 @@ extern "C" const char* b200attn_strerror(int status) {
         case B200ATTN_ERR_NO_DEVICE: return "no usable CUDA device is current";
         case B200ATTN_ERR_TOO_LARGE:
             return "problem too large: beyond the fixed scratch of b200attn_bwd_static (B*Hq*ceil(T/128)*128 > 524288), or "
-                   "2^31 or more rows in a RoPE / QK-Norm / KV-append call";
+                   "2^31 or more rows in a RoPE / QK-Norm / KV-append call or units of work in a long-context operator's";
         case DEV_WAIT_TIMEOUT_LOAD: return "device: a TMA load barrier never completed";
         case DEV_WAIT_TIMEOUT_MMA: return "device: a tensor-core completion barrier never completed";
         case DEV_WAIT_TIMEOUT_SOFTMAX: return "device: a softmax hand-off barrier never completed";

@@ -1,0 +1,251 @@
+// C ABI of the operators for long-context sampling: decode behind a shared prompt, attention weights of cached keys, eviction
+// (attn_prefix.cuh, key_weights.cuh, kv_evict.cuh; contract in include/b200attn.h).
+#include "attn_prefix.cuh"
+#include "decode_plan.h"
+#include "host_common.h"
+#include "key_weights.cuh"
+#include "kv_evict.cuh"
+#include "tmap.h"
+
+#include <algorithm>
+#include <math.h>
+
+using namespace b200attn;
+
+namespace {
+
+inline size_t round256(size_t n) { return (n + 255) & ~size_t(255); }
+inline float scale_of(float softmax_scale, int D) { return softmax_scale > 0.f ? softmax_scale : 1.f / sqrtf((float)D); }
+inline bool workspace_ok(const void* ws, size_t have, size_t need) { return ws && have >= need && (reinterpret_cast<uintptr_t>(ws) & 255u) == 0; }
+// the largest divisor of n that is at most `most`
+inline int divisor(int n, int most) {
+    int g = std::min(n, most);
+    while (n % g) --g;
+    return g;
+}
+
+// How the prompts' rows and keys are dealt (attn_prefix.cuh)
+struct PrefixPlan {
+    int heads, n_chunks, seqs, tiles, splits;
+    long long units;  // tiles of rows of all prompts, KV heads and chunks
+};
+PrefixPlan prefix_plan(int B, int G, int P, int Hq, int Hkv, int D) {
+    PrefixPlan d;
+    const int group = Hq / Hkv, n = B / G;
+    d.heads = divisor(group, 128);
+    d.n_chunks = group / d.heads;
+    d.seqs = std::min(n, 128 / d.heads);
+    d.tiles = (n + d.seqs - 1) / d.seqs;
+    d.units = (long long)G * Hkv * d.n_chunks * d.tiles;
+    const int keys = D == 64 ? PrefixCfg<64>::kKeys : PrefixCfg<128>::kKeys, all = (P + keys - 1) / keys;
+    d.splits = (int)std::max<long long>(1, std::min<long long>(all, sm_count() / d.units));
+    return d;
+}
+size_t prefix_slots(const PrefixPlan& d) { return (size_t)d.units * d.splits; }
+
+bool shared_sizes_ok(int B, int G, int P, int L, int Hq, int Hkv, int D) {
+    return B > 0 && G > 0 && B % G == 0 && P > 0 && L > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128);
+}
+
+template <int D>
+int launch_prefix(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefixParams& p, unsigned grid, cudaStream_t st) {
+    static bool set[kMaxDevices] = {false};
+    const int rc = set_smem_once(attn_prefix_kernel<D>, PrefixCfg<D>::kSmemBytes, set);
+    if (rc) return rc;
+    if (launch_pdl(attn_prefix_kernel<D>, dim3(grid), kPrefixThreads, PrefixCfg<D>::kSmemBytes, st, tq, tk, tv, p) != cudaSuccess) {
+        cudaGetLastError();
+        return B200ATTN_ERR_CUDA;
+    }
+    return B200ATTN_OK;
+}
+
+// How a chunk's units are made (key_weights.cuh)
+void key_weights_plan(KeyWeightsParams& p, int B, int T, int pos0, int Hq, int Hkv) {
+    p.T = T, p.pos0 = pos0, p.L = pos0 + T, p.Hq = Hq, p.Hkv = Hkv, p.group = Hq / Hkv;
+    p.tokens = std::min(T, 128);
+    p.heads = divisor(p.group, 128 / p.tokens);
+    p.n_qt = (T + p.tokens - 1) / p.tokens;
+    p.n_hc = p.group / p.heads;
+    p.n_kt = (p.L + 127) / 128;
+    // tiles of keys up to full_kt are seen by all tiles of tokens (a chunk of at most 128 tokens is one tile)
+    p.full_kt = p.n_qt == 1 ? p.n_kt : (pos0 + 127) / 128;
+    p.total = (long long)B * Hkv * key_weights_before(p, p.n_kt);
+}
+
+template <int D>
+int launch_key_weights(const CUtensorMap& tq, const CUtensorMap& tk, const KeyWeightsParams& p, int n_ctas, unsigned items, cudaStream_t st) {
+    static bool set[kMaxDevices] = {false};
+    const int rc = set_smem_once(key_weights_kernel<D>, KeyWeightsCfg<D>::kSmemBytes, set);
+    if (rc) return rc;
+    if (launch_pdl(key_weights_kernel<D>, dim3(n_ctas), kKeyWeightsThreads, KeyWeightsCfg<D>::kSmemBytes, st, tq, tk, p) != cudaSuccess ||
+        launch_pdl(key_weights_add_kernel, dim3(items), 128, 0, st, p, n_ctas) != cudaSuccess) {
+        cudaGetLastError();
+        return B200ATTN_ERR_CUDA;
+    }
+    return B200ATTN_OK;
+}
+
+template <int D, bool BIG>
+int launch_evict(const EvictParams& p, unsigned grid, cudaStream_t st) {
+    static bool set[kMaxDevices] = {false};
+    const int rc = set_smem_once(kv_evict_kernel<D, BIG>, kEvictFixedSmem + (BIG ? 0 : kEvictMaxKeys * 4), set);
+    if (rc) return rc;
+    if (launch_pdl(kv_evict_kernel<D, BIG>, dim3(grid), kEvictThreads, kEvictFixedSmem + (BIG ? 0 : (size_t)p.L * 4), st, p) != cudaSuccess) {
+        cudaGetLastError();
+        return B200ATTN_ERR_CUDA;
+    }
+    return B200ATTN_OK;
+}
+
+}  // namespace
+
+extern "C" size_t b200attn_decode_shared_workspace_bytes(int B, int G, int P, int L, int Hq, int Hkv, int D) {
+    if (!shared_sizes_ok(B, G, P, L, Hq, Hkv, D)) return 0;
+    return round256(b200attn_decode_workspace_bytes(B, L, Hq, Hkv, D, 0)) + prefix_slots(prefix_plan(B, G, P, Hq, Hkv, D)) * 128 * (D + 2) * sizeof(float);
+}
+
+extern "C" int b200attn_decode_shared(const void* q, const void* kprefix, const void* vprefix, const void* kcache, const void* vcache, void* o,
+                                      float* lse, const int* prefix_lens, const int* lens, int B, int G, int P, int P_cap, int L, int L_cap,
+                                      int Hq, int Hkv, int D, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_common(B, L, Hq, Hkv, D, B200ATTN_LAYOUT_BHTD);
+    if (rc) return rc;
+    if (!shared_sizes_ok(B, G, P, L, Hq, Hkv, D) || P_cap < P || L_cap < L) return B200ATTN_ERR_INVALID_ARG;
+    if (!q || !kprefix || !vprefix || !kcache || !vcache || !o) return B200ATTN_ERR_INVALID_ARG;
+    for (const void* a : {q, kprefix, vprefix, kcache, vcache, (const void*)o})
+        if (!aligned16(a)) return B200ATTN_ERR_ALIGNMENT;
+    const PrefixPlan x = prefix_plan(B, G, P, Hq, Hkv, D);
+    if (x.units * x.splits >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    if (!workspace_ok(workspace, workspace_bytes, b200attn_decode_shared_workspace_bytes(B, G, P, L, Hq, Hkv, D))) return B200ATTN_ERR_WORKSPACE;
+    int* status = status_ptr(&rc);
+    if (!status) return rc;
+    const int keys = decode_tile_keys(D);
+    const Strides sp = strides_for(B200ATTN_LAYOUT_BHTD, Hkv, P_cap, D);
+    CUtensorMap tq, tkp, tvp, tk, tv;
+    // rows of q as (head, sequence): "tokens" of the map are heads, its "heads" are sequences
+    if (!make_tmap_bf16_4d(&tq, q, D, Hq, B, 1, D, (long long)Hq * D, (long long)B * Hq * D, x.heads, x.seqs) ||
+        !make_tmap_bf16_4d(&tkp, kprefix, D, P, Hkv, G, sp.t, sp.h, sp.b, keys) || !make_tmap_bf16_4d(&tvp, vprefix, D, P, Hkv, G, sp.t, sp.h, sp.b, keys))
+        return B200ATTN_ERR_TENSOR_MAP;
+    const DecodePlan d = decode_plan(B, L, Hq, Hkv, D, 0, lens != nullptr);
+    DecodeParams dp;
+    rc = decode_fill(d, dp, tk, tv, q, kcache, vcache, o, lse, lens, B, L, L_cap, Hq, Hkv, D, softmax_scale, workspace, status);
+    if (rc) return rc;
+    PrefixParams p = {};
+    p.P = P, p.n = B / G, p.heads = x.heads, p.seqs = x.seqs, p.group = Hq / Hkv, p.n_chunks = x.n_chunks, p.Hkv = Hkv;
+    p.splits = x.splits, p.tiles = x.tiles;
+    p.div_splits = fastdiv_make((unsigned)x.splits), p.div_tiles = fastdiv_make((unsigned)x.tiles);
+    p.div_chunks = fastdiv_make((unsigned)x.n_chunks), p.div_hkv = fastdiv_make((unsigned)Hkv);
+    p.lens = prefix_lens;
+    p.scale_log2 = dp.scale_log2;
+    p.o = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(b200attn_decode_workspace_bytes(B, L, Hq, Hkv, D, 0)));
+    p.ml = reinterpret_cast<float2*>(p.o + prefix_slots(x) * 128 * D);
+    p.status = status;
+    DecodePrefix& e = dp.prefix;
+    e.o = p.o, e.ml = p.ml, e.splits = x.splits, e.tiles = x.tiles, e.n_chunks = x.n_chunks, e.Hkv = Hkv;
+    e.div_n = fastdiv_make((unsigned)p.n), e.div_heads = fastdiv_make((unsigned)x.heads), e.div_seqs = fastdiv_make((unsigned)x.seqs);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const unsigned grid = (unsigned)(x.units * x.splits);
+    rc = D == 64 ? launch_prefix<64>(tq, tkp, tvp, p, grid, st) : launch_prefix<128>(tq, tkp, tvp, p, grid, st);
+    return rc ? rc : launch_decode<kDecodeShared>(D, tk, tv, dp, d.n_ctas, st);
+}
+
+extern "C" size_t b200attn_decode_weights_workspace_bytes(int B, int L, int Hq, int Hkv, int D) {
+    if (B <= 0 || L <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128)) return 0;
+    return round256(b200attn_decode_workspace_bytes(B, L, Hq, Hkv, D, 0)) + (size_t)B * Hq * ((size_t)L + 1) * sizeof(float);
+}
+
+extern "C" int b200attn_decode_weights(const void* q, const void* kcache, const void* vcache, void* o, float* lse, float* weights,
+                                       const int* lens, int B, int L, int L_cap, int Hq, int Hkv, int D, float softmax_scale,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_common(B, L, Hq, Hkv, D, B200ATTN_LAYOUT_BHTD);
+    if (rc) return rc;
+    if (L_cap < L || !q || !kcache || !vcache || !o || !weights) return B200ATTN_ERR_INVALID_ARG;
+    for (const void* a : {q, kcache, vcache, (const void*)o})
+        if (!aligned16(a)) return B200ATTN_ERR_ALIGNMENT;
+    if (!workspace_ok(workspace, workspace_bytes, b200attn_decode_weights_workspace_bytes(B, L, Hq, Hkv, D))) return B200ATTN_ERR_WORKSPACE;
+    const int blocks = (L + kDecodeWeightsThreads - 1) / kDecodeWeightsThreads;
+    if ((long long)B * Hkv * blocks >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    int* status = status_ptr(&rc);
+    if (!status) return rc;
+    float* own = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(b200attn_decode_workspace_bytes(B, L, Hq, Hkv, D, 0)));
+    if (!lse) lse = own + (size_t)B * Hq * L;
+    const DecodePlan d = decode_plan(B, L, Hq, Hkv, D, 0, lens != nullptr);
+    CUtensorMap tk, tv;
+    DecodeParams p;
+    rc = decode_fill(d, p, tk, tv, q, kcache, vcache, o, lse, lens, B, L, L_cap, Hq, Hkv, D, softmax_scale, workspace, status);
+    if (rc) return rc;
+    p.scores = own;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    rc = launch_decode<kDecodeScores>(D, tk, tv, p, d.n_ctas, st);
+    if (rc) return rc;
+    DecodeWeightsParams w = {own, lse, weights, lens, status, L, L_cap, Hkv, d.G, d.n_chunks, blocks, p.scale_log2};
+    if (launch_pdl(decode_weights_kernel, dim3((unsigned)(B * Hkv * blocks)), kDecodeWeightsThreads, 0, st, w) != cudaSuccess) {
+        cudaGetLastError();
+        return B200ATTN_ERR_CUDA;
+    }
+    return B200ATTN_OK;
+}
+
+extern "C" size_t b200attn_key_weights_workspace_bytes(int B, int T, int pos0, int Hkv) {
+    if (B <= 0 || T <= 0 || pos0 < 0 || Hkv <= 0 || (long long)pos0 + T > INT_MAX) return 0;
+    return ((size_t)B * Hkv * ((pos0 + (size_t)T + 127) / 128) + sm_count()) * 128 * sizeof(float);
+}
+
+extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kcache, const float* lse, float* weights, int B, int T, int pos0,
+                                    int L_cap, int Hq, int Hkv, int D, float softmax_scale, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+    int rc = check_common(B, T, Hq, Hkv, D, q_layout);
+    if (rc) return rc;
+    if (pos0 < 0 || (long long)pos0 + T > L_cap || !q || !kcache || !lse || !weights) return B200ATTN_ERR_INVALID_ARG;
+    if (!aligned16(q) || !aligned16(kcache)) return B200ATTN_ERR_ALIGNMENT;
+    if (!workspace_ok(workspace, workspace_bytes, b200attn_key_weights_workspace_bytes(B, T, pos0, Hkv))) return B200ATTN_ERR_WORKSPACE;
+    KeyWeightsParams p = {};
+    key_weights_plan(p, B, T, pos0, Hq, Hkv);
+    const long long items = (long long)B * Hkv * p.n_kt;
+    const int n_ctas = (int)std::min<long long>(sm_count(), p.total);
+    if (items >= (1LL << 31) || p.total / n_ctas >= (1LL << 30)) return B200ATTN_ERR_TOO_LARGE;
+    p.status = status_ptr(&rc);
+    if (!p.status) return rc;
+    p.lse = lse, p.w = weights, p.part = static_cast<float*>(workspace), p.L_cap = L_cap;
+    p.scale_log2 = scale_of(softmax_scale, D) * kLog2e;
+    const Strides sq = strides_for(q_layout, Hq, T, D), sk = strides_for(B200ATTN_LAYOUT_BHTD, Hkv, L_cap, D);
+    CUtensorMap tq, tk;
+    // (the map of k ends at the newest token: zeros beyond it, whatever the cache holds there)
+    if (!make_tmap_bf16_4d(&tq, q, D, T, Hq, B, sq.t, sq.h, sq.b, p.tokens, p.heads) ||
+        !make_tmap_bf16_4d(&tk, kcache, D, p.L, Hkv, B, sk.t, sk.h, sk.b, 128))
+        return B200ATTN_ERR_TENSOR_MAP;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return D == 64 ? launch_key_weights<64>(tq, tk, p, n_ctas, (unsigned)items, st) : launch_key_weights<128>(tq, tk, p, n_ctas, (unsigned)items, st);
+}
+
+extern "C" int b200attn_kv_evict(void* kcache, void* vcache, const float* weights, const int* positions, float* weights_out, int* positions_out,
+                                 const int* lens, int B, int L, int L_cap, int Hkv, int D, int keep, int recent, void* stream) {
+    if (B <= 0 || L <= 0 || Hkv <= 0 || L_cap < L || keep <= 0 || recent < 0 || recent > keep) return B200ATTN_ERR_INVALID_ARG;
+    if (D != 64 && D != 128) return B200ATTN_ERR_UNSUPPORTED;
+    if (!kcache || !vcache || !weights || !positions || !weights_out || !positions_out) return B200ATTN_ERR_INVALID_ARG;
+    if (!aligned16(kcache) || !aligned16(vcache)) return B200ATTN_ERR_ALIGNMENT;
+    const long long units = (long long)B * Hkv;
+    if (units >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    // every CTA reads all of the inputs: no output may lie over them
+    const size_t rows = (size_t)units * L_cap;
+    auto apart = [&](const void* a, const void* b) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+        return x + rows * 4 <= y || y + rows * 4 <= x;
+    };
+    if (!apart(weights, weights_out) || !apart(positions, positions_out) || !apart(weights, positions_out) || !apart(positions, weights_out) ||
+        !apart(weights_out, positions_out))
+        return B200ATTN_ERR_INVALID_ARG;
+    int rc = B200ATTN_OK;
+    EvictParams p = {};
+    p.status = status_ptr(&rc);
+    if (!p.status) return rc;
+    p.k = static_cast<uint16_t*>(kcache), p.v = static_cast<uint16_t*>(vcache);
+    p.w = weights, p.pos = positions, p.w_out = weights_out, p.pos_out = positions_out, p.lens = lens;
+    p.L = L, p.L_cap = L_cap, p.Hkv = Hkv, p.keep = keep, p.recent = recent;
+    p.ranks = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, (L + 255) / 256), sm_count() / units));
+    const bool big = L > kEvictMaxKeys;
+    const long long grid = units * p.ranks;
+    if (grid >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (D == 64) return big ? launch_evict<64, true>(p, (unsigned)grid, st) : launch_evict<64, false>(p, (unsigned)grid, st);
+    return big ? launch_evict<128, true>(p, (unsigned)grid, st) : launch_evict<128, false>(p, (unsigned)grid, st);
+}

@@ -2,9 +2,11 @@
 #pragma once
 
 #include <algorithm>
+#include <math.h>
 
 #include "attn_decode.cuh"
 #include "host_common.h"
+#include "tmap.h"
 
 namespace b200attn {
 
@@ -92,6 +94,84 @@ inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits
         d.n_ctas = cap;
     }
     return d;
+}
+
+// A launch's parameters and tensor maps from checked arguments
+inline int decode_fill(const DecodePlan& d, DecodeParams& p, CUtensorMap& tk, CUtensorMap& tv, const void* q, const void* kcache,
+                       const void* vcache, void* o, float* lse, const int* lens, int B, int L, int L_cap, int Hq, int Hkv, int D,
+                       float softmax_scale, void* workspace, int* status) {
+    // the maps end at row L of every (batch, head): rows of the cache beyond it are never read (TMA fills zeros)
+    const Strides sk = strides_for(B200ATTN_LAYOUT_BHTD, Hkv, L_cap, D);
+    if (!make_tmap_bf16_4d(&tk, kcache, D, L, Hkv, B, sk.t, sk.h, sk.b, decode_tile_keys(D)) ||
+        !make_tmap_bf16_4d(&tv, vcache, D, L, Hkv, B, sk.t, sk.h, sk.b, decode_tile_keys(D)))
+        return B200ATTN_ERR_TENSOR_MAP;
+    p = {};
+    p.B = B;
+    p.L = L;
+    p.Hq = Hq;
+    p.Hkv = Hkv;
+    p.group = Hq / Hkv;
+    p.G = d.G;
+    p.n_chunks = d.n_chunks;
+    p.units_per_seq = Hkv * d.n_chunks;
+    p.div_units = fastdiv_make((unsigned)p.units_per_seq);
+    p.div_chunks = fastdiv_make((unsigned)d.n_chunks);
+    p.div_shares = fastdiv_make((unsigned)std::max(d.shares, 1));
+    p.div_tiles = fastdiv_make((unsigned)((L + decode_tile_keys(D) - 1) / decode_tile_keys(D)));
+    p.div_slice = fastdiv_make((unsigned)(d.G * (D / 2) / d.cluster));
+    p.shares = d.shares;
+    p.cluster = d.cluster;
+    p.whole = d.whole;
+    p.slot_mode = d.slot_mode;
+    p.scale = softmax_scale > 0.f ? softmax_scale : 1.f / sqrtf((float)D);
+    p.scale_log2 = p.scale * 1.4426950408889634f;
+    p.lens = lens;
+    p.q = static_cast<const uint16_t*>(q);
+    p.o = static_cast<uint16_t*>(o);
+    p.lse = lse;
+    const size_t rows = (size_t)B * Hq * d.slots;  // slots x heads per slot
+    p.part_o = static_cast<float*>(workspace);
+    p.part_m = p.part_o + rows * D;
+    p.part_l = p.part_m + rows;
+    p.counters = reinterpret_cast<unsigned long long*>(p.part_l + rows);  // (D + 2 is even: 8-byte aligned)
+    p.tag = next_decode_tag();
+    p.status = status;
+    return B200ATTN_OK;
+}
+
+template <int D, int NH, int PF, int MODE>
+int launch_decode_pf(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p, int n_ctas, cudaStream_t st) {
+    using Cfg = DecodeCfg<D>;
+    static bool set[kMaxDevices] = {false};
+    int rc = set_smem_once(attn_decode_kernel<D, NH, PF, MODE>, Cfg::kSmemBytes, set);
+    if (rc) return rc;
+    if (launch_cluster(attn_decode_kernel<D, NH, PF, MODE>, dim3(n_ctas), kDecodeThreads, Cfg::kSmemBytes, st, p.cluster, tk, tv, p) != cudaSuccess) {
+        cudaGetLastError();
+        return B200ATTN_ERR_CUDA;
+    }
+    return B200ATTN_OK;
+}
+
+// Where the CTAs fill most of the device the launch is bound by HBM, and the first two tiles of each come into L2 while the kernel
+// in front ends, provided that it lets this one start early, as the append of one token and the decode itself do (us per call over
+// caches larger than L2 in turn, without / with: append + decode B=48 L<=6000 16/4 D=64 35.6 / 34.3, B=64 L<=4096 33.5 / 31.8, B=20 L<=1500
+// D=128 19.3 / 18.0; decode behind decode B=64 L=4096 16/4 D=64 41.9 / 41.3, B=300 L=200 8/8 24.0 / 22.8, B=64 L=1000 6/2 9.0 / 8.5, B=8
+// L=2000 8/8 D=128, 128 CTAs, 14.3 / 14.1).  With a matrix product in front of each append + decode, the product included: 40.6 / 39.9,
+// 38.3 / 37.5, 23.4 / 23.0.  Behind a kernel that does not release this one early the tiles are asked for twice: product and decode
+// 46.1 / 46.0, 29.8 / 29.5, 13.3 / 13.4, 19.1 / 19.3; a first pass on new buffers on an idle device gains nothing (host's time of a call,
+// B=300 41.8 / 42.1, append + decode B=48 67.3 / 67.0).  With three tiles the gain is smaller, with six it is gone.
+// Fewer CTAs are bound by latency, of which this hides nothing: B=6 L<=3000 8/1 D=128 8.5 -> 8.6, B=1 L=1500 16/4 5.26 -> 5.30.
+constexpr int kPrefetchCtas = 128;
+// (Behind a shared prompt's kernel the loads themselves begin that early.)
+template <int MODE, int D, int NH>
+int launch_decode_heads(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p, int n_ctas, cudaStream_t st) {
+    if (MODE != kDecodeShared && n_ctas >= kPrefetchCtas) return launch_decode_pf<D, NH, MODE != kDecodeShared ? 2 : 0, MODE>(tk, tv, p, n_ctas, st);
+    return launch_decode_pf<D, NH, 0, MODE>(tk, tv, p, n_ctas, st);
+}
+template <int MODE>
+int launch_decode(int D, const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p, int n_ctas, cudaStream_t st) {
+    if (D == 64) return p.G <= 8 ? launch_decode_heads<MODE, 64, 1>(tk, tv, p, n_ctas, st) : launch_decode_heads<MODE, 64, 2>(tk, tv, p, n_ctas, st);
+    return p.G <= 8 ? launch_decode_heads<MODE, 128, 1>(tk, tv, p, n_ctas, st) : launch_decode_heads<MODE, 128, 2>(tk, tv, p, n_ctas, st);
 }
 
 }  // namespace b200attn

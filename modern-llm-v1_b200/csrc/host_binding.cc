@@ -839,12 +839,170 @@ PyObject* rotary_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
     B200ATTN_CATCH
 }
 
+// ---- long contexts
+bool ints_positive(const char* fn, const int* d, int n) {
+    for (int i = 0; i < n; ++i)
+        if (d[i] <= 0) return value_error("%s: sizes must be positive", fn), false;
+    return true;
+}
+// a capacity: an int, or None for the length itself
+bool cap_of(const char* fn, PyObject* o, int length, int* cap) {
+    *cap = length;
+    if (o != Py_None && !ints(&o, 1, cap)) return false;
+    if (*cap < length) return value_error("%s: the capacity is less than the length", fn), false;
+    return true;
+}
+bool heads_ok(const char* fn, int Hq, int Hkv, int D) {
+    if (Hq % Hkv != 0) return value_error("%s: Hq must be a multiple of Hkv", fn), false;
+    if (D != 64 && D != 128) return value_error("%s: d_h must be 64 or 128", fn), false;
+    return true;
+}
+
+// q, kprefix, vprefix, kcache, vcache, o, lse, B, G, P, L, Hq, Hkv, D, prefix_lens, lens, softmax_scale, P_cap, L_cap
+PyObject* decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "flash_attn_decode_shared";
+    B200ATTN_TRY
+    if (!arg_count(n, 19)) return nullptr;
+    const ScalarType bf = ScalarType::BFloat16;
+    for (int i = 0; i < 6; ++i)
+        if (a[i] == Py_None) return value_error("%s: q, kprefix, vprefix, kcache, vcache and o are needed", fn);
+    Items items;
+    items.add(a[0], "q", bf), items.add(a[1], "kprefix", bf), items.add(a[2], "vprefix", bf), items.add(a[3], "kcache", bf);
+    items.add(a[4], "vcache", bf), items.add(a[5], "o", bf), items.add(a[6], "lse", ScalarType::Float);
+    items.add(a[14], "prefix_lens", ScalarType::Int), items.add(a[15], "lens", ScalarType::Int);
+    int d[7], P_cap, L_cap;
+    if (!items.check(fn) || !ints(a + 7, 7, d) || !ints_positive(fn, d, 7)) return nullptr;
+    const int B = d[0], G = d[1], P = d[2], L = d[3], Hq = d[4], Hkv = d[5], D = d[6];
+    if (!heads_ok(fn, Hq, Hkv, D) || !cap_of(fn, a[17], P, &P_cap) || !cap_of(fn, a[18], L, &L_cap)) return nullptr;
+    if (B % G != 0) return value_error("%s: B must be a multiple of G", fn);
+    if (numel(a[0]) != int64_t(B) * Hq * D || numel(a[5]) != numel(a[0])) return value_error("%s: shape mismatch (q/o)", fn);
+    const int64_t np = int64_t(G) * Hkv * P_cap * D, nc = int64_t(B) * Hkv * L_cap * D;
+    if (numel(a[1]) != np || numel(a[2]) != np) return value_error("%s: shape mismatch (prefix)", fn);
+    if (numel(a[3]) != nc || numel(a[4]) != nc) return value_error("%s: shape mismatch (cache)", fn);
+    if (a[6] != Py_None && numel(a[6]) != int64_t(B) * Hq) return value_error("%s: lse must be [B, Hq]", fn);
+    if (a[14] != Py_None && numel(a[14]) != G) return value_error("%s: prefix_lens must be [G]", fn);
+    if (a[15] != Py_None && numel(a[15]) != B) return value_error("%s: lens must be [B]", fn);
+    float scale;
+    if (!scale_of(a[16], &scale)) return nullptr;
+    const Call c(a[0]);
+    void *q = ptr(a[0]), *kp = ptr(a[1]), *vp = ptr(a[2]), *k = ptr(a[3]), *v = ptr(a[4]), *o = ptr(a[5]), *st = c.st();
+    float* lse = opt_ptr<float>(a[6]);
+    const int *pl = opt_ptr<int>(a[14]), *ll = opt_ptr<int>(a[15]);
+    return finish(with_scratch(c, b200attn_decode_shared_workspace_bytes(B, G, P, L, Hq, Hkv, D), [&](void* wp, size_t wn) {
+        return b200attn_decode_shared(q, kp, vp, k, v, o, lse, pl, ll, B, G, P, P_cap, L, L_cap, Hq, Hkv, D, scale, wp, wn, st);
+    }), fn);
+    B200ATTN_CATCH
+}
+
+// q, kcache, vcache, o, lse, weights, B, L, Hq, Hkv, D, lens, softmax_scale, L_cap
+PyObject* decode_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "flash_attn_decode_weights";
+    B200ATTN_TRY
+    if (!arg_count(n, 14)) return nullptr;
+    const ScalarType bf = ScalarType::BFloat16, f = ScalarType::Float;
+    for (int i : {0, 1, 2, 3, 5})
+        if (a[i] == Py_None) return value_error("%s: q, kcache, vcache, o and weights are needed", fn);
+    Items items;
+    items.add(a[0], "q", bf), items.add(a[1], "kcache", bf), items.add(a[2], "vcache", bf), items.add(a[3], "o", bf);
+    items.add(a[4], "lse", f), items.add(a[5], "weights", f), items.add(a[11], "lens", ScalarType::Int);
+    int d[5], L_cap;
+    if (!items.check(fn) || !ints(a + 6, 5, d) || !ints_positive(fn, d, 5)) return nullptr;
+    const int B = d[0], L = d[1], Hq = d[2], Hkv = d[3], D = d[4];
+    if (!heads_ok(fn, Hq, Hkv, D) || !cap_of(fn, a[13], L, &L_cap)) return nullptr;
+    if (numel(a[0]) != int64_t(B) * Hq * D || numel(a[3]) != numel(a[0])) return value_error("%s: shape mismatch (q/o)", fn);
+    const int64_t nc = int64_t(B) * Hkv * L_cap;
+    if (numel(a[1]) != nc * D || numel(a[2]) != nc * D) return value_error("%s: shape mismatch (cache)", fn);
+    if (numel(a[5]) != nc) return value_error("%s: weights must be [B, Hkv, L_cap]", fn);
+    if (a[4] != Py_None && numel(a[4]) != int64_t(B) * Hq) return value_error("%s: lse must be [B, Hq]", fn);
+    if (a[11] != Py_None && numel(a[11]) != B) return value_error("%s: lens must be [B]", fn);
+    float scale;
+    if (!scale_of(a[12], &scale)) return nullptr;
+    const Call c(a[0]);
+    void *q = ptr(a[0]), *k = ptr(a[1]), *v = ptr(a[2]), *o = ptr(a[3]), *st = c.st();
+    float *lse = opt_ptr<float>(a[4]), *w = opt_ptr<float>(a[5]);
+    const int* ll = opt_ptr<int>(a[11]);
+    return finish(with_scratch(c, b200attn_decode_weights_workspace_bytes(B, L, Hq, Hkv, D), [&](void* wp, size_t wn) {
+        return b200attn_decode_weights(q, k, v, o, lse, w, ll, B, L, L_cap, Hq, Hkv, D, scale, wp, wn, st);
+    }), fn);
+    B200ATTN_CATCH
+}
+
+// q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale, L_cap, q_layout
+PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "flash_attn_key_weights";
+    B200ATTN_TRY
+    if (!arg_count(n, 13)) return nullptr;
+    const ScalarType bf = ScalarType::BFloat16, f = ScalarType::Float;
+    for (int i = 0; i < 4; ++i)
+        if (a[i] == Py_None) return value_error("%s: q, kcache, lse and weights are needed", fn);
+    Items items;
+    items.add(a[0], "q", bf), items.add(a[1], "kcache", bf), items.add(a[2], "lse", f), items.add(a[3], "weights", f);
+    int d[6], L_cap;
+    if (!items.check(fn) || !ints(a + 4, 6, d)) return nullptr;
+    const int B = d[0], T = d[1], pos0 = d[2], Hq = d[3], Hkv = d[4], D = d[5];
+    if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || pos0 < 0) return value_error("%s: sizes must be positive and pos0 not negative", fn);
+    if (int64_t(pos0) + T > INT32_MAX) return value_error("%s: pos0 + T is too large", fn);
+    if (!heads_ok(fn, Hq, Hkv, D) || !cap_of(fn, a[11], pos0 + T, &L_cap)) return nullptr;
+    const int layout = layout_of(a[12]);
+    if (layout < 0) return value_error("%s: q_layout must be BHTD or BTHD", fn);
+    const int64_t rows = int64_t(B) * Hq * T, nc = int64_t(B) * Hkv * L_cap;
+    if (numel(a[0]) != rows * D) return value_error("%s: shape mismatch (q)", fn);
+    if (numel(a[1]) != nc * D) return value_error("%s: shape mismatch (cache)", fn);
+    if (numel(a[2]) != rows) return value_error("%s: lse must be [B, Hq, T]", fn);
+    if (numel(a[3]) != nc) return value_error("%s: weights must be [B, Hkv, L_cap]", fn);
+    float scale;
+    if (!scale_of(a[10], &scale)) return nullptr;
+    const Call c(a[0]);
+    void *q = ptr(a[0]), *k = ptr(a[1]), *st = c.st();
+    float *lse = opt_ptr<float>(a[2]), *w = opt_ptr<float>(a[3]);
+    return finish(with_scratch(c, b200attn_key_weights_workspace_bytes(B, T, pos0, Hkv), [&](void* wp, size_t wn) {
+        return b200attn_key_weights(q, layout, k, lse, w, B, T, pos0, L_cap, Hq, Hkv, D, scale, wp, wn, st);
+    }), fn);
+    B200ATTN_CATCH
+}
+
+// kcache, vcache, weights, positions, weights_out, positions_out, B, L, Hkv, D, keep, recent, lens, L_cap
+PyObject* kv_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "kv_evict";
+    B200ATTN_TRY
+    if (!arg_count(n, 14)) return nullptr;
+    const ScalarType bf = ScalarType::BFloat16, f = ScalarType::Float, i32 = ScalarType::Int;
+    for (int i = 0; i < 6; ++i)
+        if (a[i] == Py_None) return value_error("%s: kcache, vcache, weights, positions and their outputs are needed", fn);
+    Items items;
+    items.add(a[0], "kcache", bf), items.add(a[1], "vcache", bf), items.add(a[2], "weights", f), items.add(a[3], "positions", i32);
+    items.add(a[4], "weights_out", f), items.add(a[5], "positions_out", i32), items.add(a[12], "lens", i32);
+    int d[6], L_cap;
+    if (!items.check(fn) || !ints(a + 6, 6, d) || !ints_positive(fn, d, 5)) return nullptr;
+    const int B = d[0], L = d[1], Hkv = d[2], D = d[3], keep = d[4], recent = d[5];
+    if (!heads_ok(fn, Hkv, Hkv, D) || !cap_of(fn, a[13], L, &L_cap)) return nullptr;
+    if (recent < 0 || recent > keep) return value_error("%s: recent must be between 0 and keep", fn);
+    const int64_t nc = int64_t(B) * Hkv * L_cap;
+    if (numel(a[0]) != nc * D || numel(a[1]) != nc * D) return value_error("%s: shape mismatch (cache)", fn);
+    for (int i = 2; i < 6; ++i)
+        if (numel(a[i]) != nc) return value_error("%s: weights and positions must be [B, Hkv, L_cap]", fn);
+    if (a[12] != Py_None && numel(a[12]) != B) return value_error("%s: lens must be [B]", fn);
+    const Call c(a[0]);
+    void *k = ptr(a[0]), *v = ptr(a[1]), *st = c.st();
+    float *w = opt_ptr<float>(a[2]), *wo = opt_ptr<float>(a[4]);
+    int *p = opt_ptr<int>(a[3]), *po = opt_ptr<int>(a[5]);
+    const int* ll = opt_ptr<int>(a[12]);
+    int rc;
+    {
+        const NoGil no_gil;
+        rc = b200attn_kv_evict(k, v, w, p, wo, po, ll, B, L, L_cap, Hkv, D, keep, recent, st);
+    }
+    return finish(rc, fn);
+    B200ATTN_CATCH
+}
+
 #define B200ATTN_FAST(name) \
     { #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {
     B200ATTN_FAST(fwd),      B200ATTN_FAST(bwd),      B200ATTN_FAST(decode),      B200ATTN_FAST(kv_append),
     B200ATTN_FAST(kv_attend), B200ATTN_FAST(rope_fwd), B200ATTN_FAST(rope_bwd),    B200ATTN_FAST(rope_fwd_qk),
-    B200ATTN_FAST(rope_bwd_qk), B200ATTN_FAST(rotary_fwd), B200ATTN_FAST(rotary_bwd), B200ATTN_FAST(rotary_table), {"release_scratch", release_scratch, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    B200ATTN_FAST(rope_bwd_qk), B200ATTN_FAST(rotary_fwd), B200ATTN_FAST(rotary_bwd), B200ATTN_FAST(rotary_table),
+    B200ATTN_FAST(decode_shared), B200ATTN_FAST(decode_weights), B200ATTN_FAST(key_weights), B200ATTN_FAST(kv_evict), {"release_scratch", release_scratch, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

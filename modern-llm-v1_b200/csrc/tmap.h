@@ -24,15 +24,15 @@ inline EncodeTiledFn get_encode_tiled() {
     return fn;
 }
 
-// BF16 tensor seen as 4-D (d, t, h, b) with element strides; box = (64, box_rows, 1, 1),
+// BF16 tensor seen as 4-D (d, t, h, b) with element strides; box = (64, box_rows, box_h, 1),
 // 128-byte swizzle, zero fill out of bounds.  Returns false on any driver error.
 inline bool make_tmap_bf16_4d(CUtensorMap* out, const void* base, int D, int T, int H, int B, long long stride_t,
-                              long long stride_h, long long stride_b, int box_rows) {
+                              long long stride_h, long long stride_b, int box_rows, int box_h = 1) {
     EncodeTiledFn enc = get_encode_tiled();
     if (!enc) return false;
     cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
     cuuint64_t strides[3] = {(cuuint64_t)stride_t * 2, (cuuint64_t)stride_h * 2, (cuuint64_t)stride_b * 2};
-    cuuint32_t box[4] = {64u, (cuuint32_t)box_rows, 1u, 1u};
+    cuuint32_t box[4] = {64u, (cuuint32_t)box_rows, (cuuint32_t)box_h, 1u};
     cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
     auto encode = [&] {
         return enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,

@@ -79,6 +79,28 @@ def flash_attn_decode(q, kcache, vcache, o, lse, B, L, Hq, Hkv, D, softmax_scale
     _lib.host().decode(q, kcache, vcache, o, lse, B, L, Hq, Hkv, D, softmax_scale, n_splits)
 
 
+def flash_attn_decode_shared(q, kprefix, vprefix, kcache, vcache, o, lse, B, G, P, L, Hq, Hkv, D, prefix_lens=None, lens=None,
+                             softmax_scale=None, P_cap=None, L_cap=None):
+    """flash_attn_decode for sequences that share prompts: sequence b continues prompt b // (B // G), whose keys and values are read
+    once for all of them.  q, o [B, Hq, D] BF16; kprefix, vprefix [G, Hkv, P_cap, D], of which prefix_lens[g] rows (int32 [G] on the
+    device, 0 .. P; None: P) count; kcache, vcache [B, Hkv, L_cap, D], of which lens[b] rows (1 .. L; None: L) count, the newest token
+    among them; lse [B, Hq] FP32 or None.  Rows that do not count may hold anything.  Capacities left out equal P and L."""
+    _lib.host().decode_shared(q, kprefix, vprefix, kcache, vcache, o, lse, B, G, P, L, Hq, Hkv, D, prefix_lens, lens, softmax_scale, P_cap, L_cap)
+
+
+def flash_attn_decode_weights(q, kcache, vcache, o, lse, weights, B, L, Hq, Hkv, D, lens=None, softmax_scale=None, L_cap=None):
+    """flash_attn_decode that also adds, to weights[b, hk, key] (FP32 [B, Hkv, L_cap]), the probabilities that the heads of the group
+    give the key.  lens: int32 [B] on the device, rows of each sequence that count (1 .. L), or None: L; the others may hold anything."""
+    _lib.host().decode_weights(q, kcache, vcache, o, lse, weights, B, L, Hq, Hkv, D, lens, softmax_scale, L_cap)
+
+
+def flash_attn_key_weights(q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale=None, L_cap=None, q_layout="BHTD"):
+    """The same sums over a chunk: weights[b, hk, key] += the probabilities that the T tokens in rows pos0 .. pos0 + T - 1 of the cache
+    give the key, over the heads of the group and the tokens that see it.  q: [.., T, ..] in q_layout; lse [B, Hq, T], as the forward over
+    the cache has left it.  For a prompt's last tokens only, pass their q, lse and row."""
+    _lib.host().key_weights(q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale, L_cap, q_layout)
+
+
 def device_status() -> int:
     """Synchronises the current stream and raises RuntimeError if a kernel gave up on a
     bounded wait since the last check; returns 0 otherwise."""

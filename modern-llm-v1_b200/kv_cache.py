@@ -21,6 +21,15 @@ from . import _lib
 from .rope_norm import make_rope_cache
 
 
+def kv_evict(kcache, vcache, weights, positions, weights_out, positions_out, B, L, Hkv, D, keep, recent, lens=None, L_cap=None):
+    """Cuts the first lens[b] rows (int32 [B] on the device; None: L) of every (batch, KV head) down to at most `keep`: the rows whose
+    position is above newest - recent stay, then those of the largest weight, of equal ones the lower row (csrc/kv_evict.cuh).  kcache,
+    vcache [B, Hkv, L_cap, D] BF16 change in place: rows below `keep` that stay are not moved, the j-th row that stays behind them goes
+    to the j-th free place.  weights (FP32) and positions (int32, distinct within a head) [B, Hkv, L_cap] are read, weights_out and
+    positions_out written whole, with 0 and -1 behind the rows that stayed."""
+    _lib.host().kv_evict(kcache, vcache, weights, positions, weights_out, positions_out, B, L, Hkv, D, keep, recent, lens, L_cap)
+
+
 class KVCache:
     def __init__(self, n_layers: int, B: int, Hq: int, Hkv: int, D: int, L_cap: int, device="cuda",
                  rope_base: float = 10000.0, eps: float = 1e-5):
