@@ -54,6 +54,10 @@ struct DecodePrefix {
     FastDiv div_n;     // sequences per prompt
     FastDiv div_heads, div_seqs;  // heads per chunk, sequences per tile
     int n_chunks, Hkv;
+    // In the deal by ranges a CTA first goes through all its pieces, whose results it leaves here (un-normalised O [B, Hq, D], (m, l)
+    // [B, Hq]), and joins them with the prompts' at its end: waiting for those at the first piece would hold up the others.
+    float* own_o;
+    float2* own_ml;
 };
 
 struct DecodeParams {
@@ -418,12 +422,12 @@ __device__ __forceinline__ int decode_count(unsigned long long* word, unsigned l
     return int(atomicAdd(word, 1ull) - tag) + 1;
 }
 
-// One pair of output elements (columns d, d + 1 of head j of the group) joined with the prompt's partial results, in the order of the
+// W output elements (columns d .. d + W - 1 of head j of the group) joined with the prompt's partial results, in the order of the
 // splits; false: a kernel has failed and nothing may be written.  This is the first look at what the kernel in front, which computes
 // them, has written: all else this kernel reads was there before that one began (see grid_dep_launch in attn_prefix.cuh), so its loads
 // run beside it.  (The chain is two round trips through L2 whatever the number of splits up to eight.)
-template <int D>
-__device__ __forceinline__ bool decode_add_prefix(const DecodeParams& p, int b, int hk, int j, int d, float& a0, float& a1, float& m, float& l) {
+template <int D, int W>
+__device__ __forceinline__ bool decode_add_prefix(const DecodeParams& p, int b, int hk, int j, int d, float (&a)[W], float& m, float& l) {
     const DecodePrefix& x = p.prefix;
     grid_dep_wait();
     const int status = *reinterpret_cast<volatile int*>(p.status);
@@ -435,31 +439,60 @@ __device__ __forceinline__ bool decode_add_prefix(const DecodeParams& p, int b, 
     const float2* ml = x.ml + slot0 * 128 + row;
     constexpr int N = 8;
     for (int s0 = 0; s0 < x.splits; s0 += N) {
-        float2 pml[N], po[N];
+        float2 pml[N];
+        float po[N][W];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            pml[k] = make_float2(-INFINITY, 0.f), po[k] = make_float2(0.f, 0.f);
+            pml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int e = 0; e < W; ++e) po[k][e] = 0.f;
             if (s0 + k < x.splits) {
                 pml[k] = __ldcg(ml + (s0 + k) * 128);
-                po[k] = __ldcg(reinterpret_cast<const float2*>(o + size_t(s0 + k) * (D * 128)));
+                const float* const at = o + size_t(s0 + k) * (D * 128);
+                if constexpr (W == 4) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(at));
+                    po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
+                } else {
+                    const float2 v = __ldcg(reinterpret_cast<const float2*>(at));
+                    po[k][0] = v.x, po[k][1] = v.y;
+                }
             }
         }
         float mn = m;
 #pragma unroll
         for (int k = 0; k < N; ++k) mn = fmaxf(mn, pml[k].x);
         const float fa = m == -INFINITY ? 1.f : ex2_approx((m - mn) * p.scale_log2);  // (m = -inf: no score above it, l is 0 or NaN)
-        l *= fa, a0 *= fa, a1 *= fa;
+        l *= fa;
+#pragma unroll
+        for (int e = 0; e < W; ++e) a[e] *= fa;
         m = mn;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             if (pml[k].x == -INFINITY && pml[k].y == 0.f) continue;  // no keys: nothing else was written
             const float f = pml[k].x == -INFINITY ? 1.f : ex2_approx((pml[k].x - mn) * p.scale_log2);
             l += f * pml[k].y;
-            a0 += f * po[k].x;
-            a1 += f * po[k].y;
+#pragma unroll
+            for (int e = 0; e < W; ++e) a[e] += f * po[k][e];
         }
     }
     return status == 0;
+}
+// The same for all rows of the finished unit at w, whose results lie in own_o: four columns a thread, the heads of a unit side by side as
+// their rows are in the prompt's slots.
+template <int D>
+__device__ __forceinline__ void decode_join_unit(const DecodeParams& p, const DecodeWalk& w, int tid) {
+    const int hk = int(fastdiv(w.u, p.div_chunks)), j0 = (w.u - hk * p.n_chunks) * p.G;
+    const size_t row0 = size_t(w.b) * p.Hq + hk * p.group + j0;
+    for (int i = tid; i < p.G * (D / 4); i += 128) {
+        const int c = i / p.G, g = i - c * p.G;
+        const float4 own = __ldcg(reinterpret_cast<const float4*>(p.prefix.own_o + (row0 + g) * D) + c);
+        float2 ml = __ldcg(p.prefix.own_ml + row0 + g);
+        float a[4] = {own.x, own.y, own.z, own.w};
+        if (!decode_add_prefix<D, 4>(p, w.b, hk, j0 + g, c * 4, a, ml.x, ml.y)) continue;
+        const float inv = 1.f / ml.y;
+        reinterpret_cast<uint2*>(p.o)[(row0 + g) * (D / 4) + c] = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
+        if (p.lse && c == 0) p.lse[row0 + g] = ml.x * p.scale + logf(ml.y);
+    }
 }
 
 // PF: tiles that a CTA brings into L2 while the kernel in front of this one ends
@@ -559,8 +592,17 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const int hk = int(fastdiv(w.u, p.div_chunks));
         const int j0 = (w.u - hk * p.n_chunks) * G, b = w.b;
         const size_t row0 = size_t(b) * p.Hq + hk * p.group + j0;
-        return [&p, row0, b, hk, j0](int g, int d, float a0, float a1, float m, float l) {
-            if (MODE == kDecodeShared && !decode_add_prefix<D>(p, b, hk, j0 + g, d, a0, a1, m, l)) return;
+        return [&p, row0, b, hk, j0, warp](int g, int d, float a0, float a1, float m, float l) {
+            if (MODE == kDecodeShared && p.prefix.own_o && warp != 5) {  // (the counter's piece is the last thing that it does)
+                *reinterpret_cast<float2*>(p.prefix.own_o + (row0 + g) * D + d) = make_float2(a0, a1);
+                if (d == 0) p.prefix.own_ml[row0 + g] = make_float2(m, l);
+                return;
+            }
+            if (MODE == kDecodeShared) {
+                float a[2] = {a0, a1};
+                if (!decode_add_prefix<D, 2>(p, b, hk, j0 + g, d, a, m, l)) return;
+                a0 = a[0], a1 = a[1];
+            }
             const float inv = 1.f / l;
             reinterpret_cast<uint32_t*>(p.o)[(row0 + g) * (D / 2) + d / 2] = pack_bf16x2(a0 * inv, a1 * inv);
             if (p.lse && d == 0) p.lse[row0 + g] = m * p.scale + logf(l);
@@ -625,7 +667,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const bool failed = *fail_flag != 0;
     bool ok = true;
     const int rank = p.cluster > 1 ? int(blockIdx.x) % p.cluster : 0;
-    bool sent = false;
+    bool sent = false, last_mine = false;
     int j = 0;  // tiles before this piece (ring position)
     for (int n = 0; w.t < w.t_end; ++n) {
         const int tiles = decode_piece(w);
@@ -822,6 +864,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (!ends_range) {
                 mbar_arrive(bar_part);
             } else if (*last_flag) {
+                last_mine = true;
                 if (tid == 0) *counter = tag;
             } else {
                 __threadfence();
@@ -833,7 +876,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                     __threadfence();
                 }
                 named_bar_sync(1, 128);
-                if (*last_flag)
+                last_mine = *last_flag != 0;
+                if (last_mine)
                     for (int i = tid; i < G * (D / 2); i += 128)
                         decode_add_pieces<D>(p, w, first, last, unit_start, i / (D / 2), (i % (D / 2)) * 2, -1, 0.f, 0.f, 0.f, 0.f, write_rows);
             }
@@ -843,6 +887,16 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         mbar_arrive(&bar_free[s_last]);
         named_bar_sync(1, 128);  // sMl and the flag are rewritten at the next piece's end
         decode_walk_next<KEYS>(p, w, tiles);
+    }
+    if constexpr (MODE == kDecodeShared) {
+        if (p.prefix.own_o && ok && !failed) {  // the units that this CTA has finished
+            named_bar_sync(1, 128);
+            for (w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane); w.t < w.t_end;) {
+                const int tiles = decode_piece(w);
+                if (tiles == w.n_tiles || (w.t + tiles == w.t_end && last_mine)) decode_join_unit<D>(p, w, tid);
+                decode_walk_next<KEYS>(p, w, tiles);
+            }
+        }
     }
     if (p.cluster <= 1) return;
     // ---- the cluster's partial results: this CTA finishes its slice of the outputs.  A CTA without tiles sends weight zero, one

@@ -24,41 +24,57 @@ inline int divisor(int n, int most) {
     return g;
 }
 
-// How the prompts' rows and keys are dealt (attn_prefix.cuh)
+// How the prompts' rows and keys are dealt (attn_prefix.cuh), and the decode behind
 struct PrefixPlan {
     int heads, n_chunks, seqs, tiles, splits;
+    int blocks;       // CTAs side by side per chunk: pairs of tiles, or the one tile
     long long units;  // tiles of rows of all prompts, KV heads and chunks
+    long long grid;
+    DecodePlan decode;
+    size_t decode_bytes, bytes;  // of the workspace: the decode's own, all
+    size_t slots;
 };
-PrefixPlan prefix_plan(int B, int G, int P, int Hq, int Hkv, int D) {
+// The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others, and both are bound by HBM or, when
+// short, by latency: SMs are shared out by the bytes to be read.
+PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool ragged) {
     PrefixPlan d;
-    const int group = Hq / Hkv, n = B / G;
+    const int group = Hq / Hkv, n = B / G, sms = sm_count();
     d.heads = divisor(group, 128);
     d.n_chunks = group / d.heads;
     d.seqs = std::min(n, 128 / d.heads);
     d.tiles = (n + d.seqs - 1) / d.seqs;
     d.units = (long long)G * Hkv * d.n_chunks * d.tiles;
-    const int keys = D == 64 ? PrefixCfg<64>::kKeys : PrefixCfg<128>::kKeys, all = (P + keys - 1) / keys;
-    d.splits = (int)std::max<long long>(1, std::min<long long>(all, sm_count() / d.units));
+    d.blocks = (d.tiles + 1) / 2;
+    const long long ctas = (long long)G * Hkv * d.n_chunks * d.blocks;
+    const int all = (P + kPrefixKeys - 1) / kPrefixKeys;
+    const double keys = (double)G * P, own = (double)B * L;
+    const int share = std::max(1, (int)(sms * keys / (keys + own)));
+    d.splits = (int)std::max<long long>(1, std::min<long long>(all, share / ctas));
+    d.grid = ctas * d.splits;
+    d.slots = (size_t)d.units * d.splits;
+    const int left = d.grid < sms ? sms - (int)d.grid : sms;
+    d.decode = decode_plan(B, L, Hq, Hkv, D, 0, ragged, std::min(2 * left, kDecodeMaxCtas), true);
+    d.decode_bytes = round256((size_t)B * Hq * d.decode.splits * (size_t)(D + 2) * sizeof(float));
+    d.bytes = d.decode_bytes + (d.slots * 128 + (size_t)B * Hq) * (D + 2) * sizeof(float);
     return d;
 }
-size_t prefix_slots(const PrefixPlan& d) { return (size_t)d.units * d.splits; }
 
 bool shared_sizes_ok(int B, int G, int P, int L, int Hq, int Hkv, int D) {
     return B > 0 && G > 0 && B % G == 0 && P > 0 && L > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128);
 }
 
-template <int D>
+template <int D, bool ROWS2>
 int launch_prefix(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefixParams& p, unsigned grid, cudaStream_t st) {
+    constexpr int smem = PrefixCfg<D, ROWS2>::kSmemBytes;
     static bool set[kMaxDevices] = {false};
-    const int rc = set_smem_once(attn_prefix_kernel<D>, PrefixCfg<D>::kSmemBytes, set);
+    const int rc = set_smem_once(attn_prefix_kernel<D, ROWS2>, smem, set);
     if (rc) return rc;
-    if (launch_pdl(attn_prefix_kernel<D>, dim3(grid), kPrefixThreads, PrefixCfg<D>::kSmemBytes, st, tq, tk, tv, p) != cudaSuccess) {
+    if (launch_pdl(attn_prefix_kernel<D, ROWS2>, dim3(grid), kPrefixThreads, smem, st, tq, tk, tv, p) != cudaSuccess) {
         cudaGetLastError();
         return B200ATTN_ERR_CUDA;
     }
     return B200ATTN_OK;
 }
-
 // How a chunk's units are made (key_weights.cuh)
 void key_weights_plan(KeyWeightsParams& p, int B, int T, int pos0, int Hq, int Hkv) {
     p.T = T, p.pos0 = pos0, p.L = pos0 + T, p.Hq = Hq, p.Hkv = Hkv, p.group = Hq / Hkv;
@@ -66,19 +82,24 @@ void key_weights_plan(KeyWeightsParams& p, int B, int T, int pos0, int Hq, int H
     p.heads = divisor(p.group, 128 / p.tokens);
     p.n_qt = (T + p.tokens - 1) / p.tokens;
     p.n_hc = p.group / p.heads;
+    p.div_hc = fastdiv_make((unsigned)p.n_hc), p.div_tokens = fastdiv_make((unsigned)p.tokens);
     p.n_kt = (p.L + 127) / 128;
     // tiles of keys up to full_kt are seen by all tiles of tokens (a chunk of at most 128 tokens is one tile)
     p.full_kt = p.n_qt == 1 ? p.n_kt : (pos0 + 127) / 128;
-    p.total = (long long)B * Hkv * key_weights_before(p, p.n_kt);
+}
+// units of all items, beyond 32 bits too
+long long key_weights_total(const KeyWeightsParams& p, int B) {
+    const long long m = std::max(0, p.n_kt - p.full_kt);
+    return (long long)B * p.Hkv * (((long long)p.n_kt * p.n_qt - m * (m - 1) / 2) * p.n_hc);
 }
 
 template <int D>
-int launch_key_weights(const CUtensorMap& tq, const CUtensorMap& tk, const KeyWeightsParams& p, int n_ctas, unsigned items, cudaStream_t st) {
+int launch_key_weights(const CUtensorMap& tq, const CUtensorMap& tk, const KeyWeightsParams& p, unsigned items, cudaStream_t st) {
     static bool set[kMaxDevices] = {false};
     const int rc = set_smem_once(key_weights_kernel<D>, KeyWeightsCfg<D>::kSmemBytes, set);
     if (rc) return rc;
-    if (launch_pdl(key_weights_kernel<D>, dim3(n_ctas), kKeyWeightsThreads, KeyWeightsCfg<D>::kSmemBytes, st, tq, tk, p) != cudaSuccess ||
-        launch_pdl(key_weights_add_kernel, dim3(items), 128, 0, st, p, n_ctas) != cudaSuccess) {
+    if (launch_pdl(key_weights_kernel<D>, dim3(p.n_ctas), kKeyWeightsThreads, KeyWeightsCfg<D>::kSmemBytes, st, tq, tk, p) != cudaSuccess ||
+        launch_pdl(key_weights_add_kernel, dim3(items), 128, 0, st, p) != cudaSuccess) {
         cudaGetLastError();
         return B200ATTN_ERR_CUDA;
     }
@@ -101,7 +122,7 @@ int launch_evict(const EvictParams& p, unsigned grid, cudaStream_t st) {
 
 extern "C" size_t b200attn_decode_shared_workspace_bytes(int B, int G, int P, int L, int Hq, int Hkv, int D) {
     if (!shared_sizes_ok(B, G, P, L, Hq, Hkv, D)) return 0;
-    return round256(b200attn_decode_workspace_bytes(B, L, Hq, Hkv, D, 0)) + prefix_slots(prefix_plan(B, G, P, Hq, Hkv, D)) * 128 * (D + 2) * sizeof(float);
+    return std::max(prefix_plan(B, G, P, L, Hq, Hkv, D, false).bytes, prefix_plan(B, G, P, L, Hq, Hkv, D, true).bytes);
 }
 
 extern "C" int b200attn_decode_shared(const void* q, const void* kprefix, const void* vprefix, const void* kcache, const void* vcache, void* o,
@@ -113,39 +134,44 @@ extern "C" int b200attn_decode_shared(const void* q, const void* kprefix, const 
     if (!q || !kprefix || !vprefix || !kcache || !vcache || !o) return B200ATTN_ERR_INVALID_ARG;
     for (const void* a : {q, kprefix, vprefix, kcache, vcache, (const void*)o})
         if (!aligned16(a)) return B200ATTN_ERR_ALIGNMENT;
-    const PrefixPlan x = prefix_plan(B, G, P, Hq, Hkv, D);
-    if (x.units * x.splits >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    const PrefixPlan x = prefix_plan(B, G, P, L, Hq, Hkv, D, lens != nullptr);
+    if (x.units * x.splits >= (1LL << 31) || x.grid >= (1LL << 31) || (long long)B * Hq * D >= (1LL << 37)) return B200ATTN_ERR_TOO_LARGE;
     if (!workspace_ok(workspace, workspace_bytes, b200attn_decode_shared_workspace_bytes(B, G, P, L, Hq, Hkv, D))) return B200ATTN_ERR_WORKSPACE;
     int* status = status_ptr(&rc);
     if (!status) return rc;
-    const int keys = decode_tile_keys(D);
     const Strides sp = strides_for(B200ATTN_LAYOUT_BHTD, Hkv, P_cap, D);
     CUtensorMap tq, tkp, tvp, tk, tv;
     // rows of q as (head, sequence): "tokens" of the map are heads, its "heads" are sequences
     if (!make_tmap_bf16_4d(&tq, q, D, Hq, B, 1, D, (long long)Hq * D, (long long)B * Hq * D, x.heads, x.seqs) ||
-        !make_tmap_bf16_4d(&tkp, kprefix, D, P, Hkv, G, sp.t, sp.h, sp.b, keys) || !make_tmap_bf16_4d(&tvp, vprefix, D, P, Hkv, G, sp.t, sp.h, sp.b, keys))
+        !make_tmap_bf16_4d(&tkp, kprefix, D, P, Hkv, G, sp.t, sp.h, sp.b, kPrefixKeys) || !make_tmap_bf16_4d(&tvp, vprefix, D, P, Hkv, G, sp.t, sp.h, sp.b, kPrefixKeys))
         return B200ATTN_ERR_TENSOR_MAP;
-    const DecodePlan d = decode_plan(B, L, Hq, Hkv, D, 0, lens != nullptr);
+    const DecodePlan& d = x.decode;
     DecodeParams dp;
     rc = decode_fill(d, dp, tk, tv, q, kcache, vcache, o, lse, lens, B, L, L_cap, Hq, Hkv, D, softmax_scale, workspace, status);
     if (rc) return rc;
     PrefixParams p = {};
     p.P = P, p.n = B / G, p.heads = x.heads, p.seqs = x.seqs, p.group = Hq / Hkv, p.n_chunks = x.n_chunks, p.Hkv = Hkv;
     p.splits = x.splits, p.tiles = x.tiles;
-    p.div_splits = fastdiv_make((unsigned)x.splits), p.div_tiles = fastdiv_make((unsigned)x.tiles);
+    p.div_splits = fastdiv_make((unsigned)x.splits), p.div_blocks = fastdiv_make((unsigned)x.blocks);
     p.div_chunks = fastdiv_make((unsigned)x.n_chunks), p.div_hkv = fastdiv_make((unsigned)Hkv);
     p.lens = prefix_lens;
     p.scale_log2 = dp.scale_log2;
-    p.o = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(b200attn_decode_workspace_bytes(B, L, Hq, Hkv, D, 0)));
-    p.ml = reinterpret_cast<float2*>(p.o + prefix_slots(x) * 128 * D);
+    p.o = reinterpret_cast<float*>(static_cast<char*>(workspace) + x.decode_bytes);
+    p.ml = reinterpret_cast<float2*>(p.o + x.slots * 128 * D);
     p.status = status;
     DecodePrefix& e = dp.prefix;
     e.o = p.o, e.ml = p.ml, e.splits = x.splits, e.tiles = x.tiles, e.n_chunks = x.n_chunks, e.Hkv = Hkv;
     e.div_n = fastdiv_make((unsigned)p.n), e.div_heads = fastdiv_make((unsigned)x.heads), e.div_seqs = fastdiv_make((unsigned)x.seqs);
+    if (d.shares == 0) {
+        e.own_o = reinterpret_cast<float*>(p.ml + x.slots * 128);
+        e.own_ml = reinterpret_cast<float2*>(e.own_o + (size_t)B * Hq * D);
+    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const unsigned grid = (unsigned)(x.units * x.splits);
-    rc = D == 64 ? launch_prefix<64>(tq, tkp, tvp, p, grid, st) : launch_prefix<128>(tq, tkp, tvp, p, grid, st);
-    return rc ? rc : launch_decode<kDecodeShared>(D, tk, tv, dp, d.n_ctas, st);
+    const unsigned grid = (unsigned)x.grid;
+    if (D == 64) rc = x.tiles > 1 ? launch_prefix<64, true>(tq, tkp, tvp, p, grid, st) : launch_prefix<64, false>(tq, tkp, tvp, p, grid, st);
+    else rc = x.tiles > 1 ? launch_prefix<128, true>(tq, tkp, tvp, p, grid, st) : launch_prefix<128, false>(tq, tkp, tvp, p, grid, st);
+    if (!rc) rc = launch_decode<kDecodeShared>(D, tk, tv, dp, d.n_ctas, st);
+    return rc;
 }
 
 extern "C" size_t b200attn_decode_weights_workspace_bytes(int B, int L, int Hq, int Hkv, int D) {
@@ -162,7 +188,7 @@ extern "C" int b200attn_decode_weights(const void* q, const void* kcache, const 
     for (const void* a : {q, kcache, vcache, (const void*)o})
         if (!aligned16(a)) return B200ATTN_ERR_ALIGNMENT;
     if (!workspace_ok(workspace, workspace_bytes, b200attn_decode_weights_workspace_bytes(B, L, Hq, Hkv, D))) return B200ATTN_ERR_WORKSPACE;
-    const int blocks = (L + kDecodeWeightsThreads - 1) / kDecodeWeightsThreads;
+    const int blocks = (L + kDecodeWeightsThreads * kDecodeWeightsKeys - 1) / (kDecodeWeightsThreads * kDecodeWeightsKeys);
     if ((long long)B * Hkv * blocks >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
     int* status = status_ptr(&rc);
     if (!status) return rc;
@@ -187,7 +213,7 @@ extern "C" int b200attn_decode_weights(const void* q, const void* kcache, const 
 
 extern "C" size_t b200attn_key_weights_workspace_bytes(int B, int T, int pos0, int Hkv) {
     if (B <= 0 || T <= 0 || pos0 < 0 || Hkv <= 0 || (long long)pos0 + T > INT_MAX) return 0;
-    return ((size_t)B * Hkv * ((pos0 + (size_t)T + 127) / 128) + sm_count()) * 128 * sizeof(float);
+    return ((size_t)B * Hkv * ((pos0 + (size_t)T + 127) / 128) + sm_count()) * kKeyWeightsGroups * 128 * sizeof(float);
 }
 
 extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kcache, const float* lse, float* weights, int B, int T, int pos0,
@@ -201,8 +227,11 @@ extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kca
     KeyWeightsParams p = {};
     key_weights_plan(p, B, T, pos0, Hq, Hkv);
     const long long items = (long long)B * Hkv * p.n_kt;
-    const int n_ctas = (int)std::min<long long>(sm_count(), p.total);
-    if (items >= (1LL << 31) || p.total / n_ctas >= (1LL << 30)) return B200ATTN_ERR_TOO_LARGE;
+    const long long total = key_weights_total(p, B);
+    if (items >= (1LL << 31) || total >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    p.total = (int)total;
+    p.n_ctas = std::min(sm_count(), p.total);
+    p.per_cta = p.total / p.n_ctas, p.more = p.total % p.n_ctas;
     p.status = status_ptr(&rc);
     if (!p.status) return rc;
     p.lse = lse, p.w = weights, p.part = static_cast<float*>(workspace), p.L_cap = L_cap;
@@ -214,7 +243,7 @@ extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kca
         !make_tmap_bf16_4d(&tk, kcache, D, p.L, Hkv, B, sk.t, sk.h, sk.b, 128))
         return B200ATTN_ERR_TENSOR_MAP;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return D == 64 ? launch_key_weights<64>(tq, tk, p, n_ctas, (unsigned)items, st) : launch_key_weights<128>(tq, tk, p, n_ctas, (unsigned)items, st);
+    return D == 64 ? launch_key_weights<64>(tq, tk, p, (unsigned)items, st) : launch_key_weights<128>(tq, tk, p, (unsigned)items, st);
 }
 
 extern "C" int b200attn_kv_evict(void* kcache, void* vcache, const float* weights, const int* positions, float* weights_out, int* positions_out,
@@ -241,7 +270,7 @@ extern "C" int b200attn_kv_evict(void* kcache, void* vcache, const float* weight
     p.k = static_cast<uint16_t*>(kcache), p.v = static_cast<uint16_t*>(vcache);
     p.w = weights, p.pos = positions, p.w_out = weights_out, p.pos_out = positions_out, p.lens = lens;
     p.L = L, p.L_cap = L_cap, p.Hkv = Hkv, p.keep = keep, p.recent = recent;
-    p.ranks = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, (L + 255) / 256), sm_count() / units));
+    p.ranks = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, (L + 255) / 256), 4 * sm_count() / units));
     const bool big = L > kEvictMaxKeys;
     const long long grid = units * p.ranks;
     if (grid >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;

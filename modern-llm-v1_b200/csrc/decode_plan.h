@@ -46,9 +46,12 @@ struct DecodePlan {
 constexpr long long kRangesBytes = 16ll << 20;
 constexpr int kSaturatingCtas = 60;
 
-inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits, bool ragged) {
+// cap: CTAs that may run at once, or 0: as many as fit the device.  A decode behind a shared prompt (`shared`) is never dealt more CTAs than
+// that: they wait for the prompts' kernel at their ends.
+inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits, bool ragged, int cap = 0, bool shared = false) {
     DecodePlan d;
-    const int group = Hq / Hkv, cap = decode_max_ctas();
+    const int group = Hq / Hkv;
+    if (cap <= 0) cap = decode_max_ctas();
     d.G = decode_heads_per_cta(group);
     d.n_chunks = group / d.G;
     const long long units = (long long)B * Hkv * d.n_chunks;
@@ -70,11 +73,11 @@ inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits
     } else {
         d.slots = (int)std::min<long long>(n_all, (2 * cap + units - 1) / units);
         if (n_all > 1) counters = std::min<long long>(tiles, cap);  // (a single tile is never shared)
-        while (d.cluster < kDecodeMaxCluster && units * d.cluster * 2 <= sm_count() && n_all > 2 * d.cluster) d.cluster *= 2;
+        while (d.cluster < kDecodeMaxCluster && units * d.cluster * 2 <= (shared ? cap / 2 : sm_count()) && n_all > 2 * d.cluster) d.cluster *= 2;
         d.shares = d.cluster;
         const long long ctas = units * d.cluster, last = ctas % cap ? ctas % cap : cap;
         const long long idle = last < kSaturatingCtas ? unit_bytes / d.cluster * (kSaturatingCtas - last) : 0;
-        if (tiles > d.cluster * units && (idle > kRangesBytes || (ragged && units * unit_bytes > kRangesBytes))) {
+        if ((tiles > d.cluster * units && (idle > kRangesBytes || (ragged && units * unit_bytes > kRangesBytes))) || (shared && ragged && units > cap)) {
             d.shares = 0;
             d.cluster = 1;
             d.slot_mode = d.slots == n_all ? kDecodeSlotTile : kDecodeSlotTwo;

@@ -29,82 +29,107 @@ struct DecodeWeightsParams {
     int blocks;           // of keys per (batch, KV head)
     float scale_log2;
 };
-constexpr int kDecodeWeightsThreads = 256;
+constexpr int kDecodeWeightsThreads = 256, kDecodeWeightsKeys = 4;  // keys per thread: their loads are all issued before the first is used
 
-// a block: keys of one (batch, KV head); thread = key
+// a block: 1024 keys of one (batch, KV head)
 __global__ void __launch_bounds__(kDecodeWeightsThreads) decode_weights_kernel(const DecodeWeightsParams p) {
-    __shared__ float s_lse[128];
-    const int u = int(blockIdx.x) / p.blocks, key0 = (int(blockIdx.x) - u * p.blocks) * kDecodeWeightsThreads, b = u / p.Hkv, key = key0 + int(threadIdx.x);
+    constexpr int K = kDecodeWeightsKeys, STEP = kDecodeWeightsThreads;
+    __shared__ float s_lse[16];
+    const int u = int(blockIdx.x) / p.blocks, key0 = (int(blockIdx.x) - u * p.blocks) * K * STEP, b = u / p.Hkv;
     const int group = p.G * p.n_chunks;
     grid_dep_wait();
     const int len = p.lens ? max(1, min(__ldg(p.lens + b), p.L)) : p.L;
     if (key0 >= len || *reinterpret_cast<const volatile int*>(p.status) != 0) return;
-    float acc = 0.f;
-    float* const w = p.w + size_t(u) * p.L_cap + key;
-    const float old = key < len ? *w : 0.f;
-    for (int g0 = 0; g0 < group; g0 += 128) {  // (a group of more than 128 heads goes by parts)
-        if (g0) __syncthreads();
-        for (int g = threadIdx.x; g < min(128, group - g0); g += kDecodeWeightsThreads)
-            s_lse[g] = __ldcg(p.lse + size_t(u) * group + g0 + g) * kLog2e;
-        __syncthreads();
-        if (key >= len) continue;
-        for (int g = g0; g < min(group, g0 + 128); ++g) {
-            const int chunk = g / p.G;
-            const float s = __ldcg(p.scores + ((size_t(u) * p.n_chunks + chunk) * p.L + key) * p.G + g - chunk * p.G);
-            acc += ex2_approx(fmaf(s, p.scale_log2, -s_lse[g - g0]));
+    float* const w = p.w + size_t(u) * p.L_cap + key0 + threadIdx.x;
+    const int left = len - key0 - int(threadIdx.x);  // key k of this thread counts where k * STEP < left
+    float old[K], acc[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) old[k] = k * STEP < left ? w[k * STEP] : 0.f, acc[k] = 0.f;
+    for (int c = 0; c < p.n_chunks; ++c) {  // (a chunk: at most 16 heads)
+        const float* const s = p.scores + ((size_t(u) * p.n_chunks + c) * p.L + key0 + threadIdx.x) * p.G;
+        const float lse = int(threadIdx.x) < p.G ? __ldcg(p.lse + size_t(u) * group + c * p.G + threadIdx.x) * kLog2e : 0.f;
+        if (c) __syncthreads();
+        for (int g0 = 0; g0 < p.G; g0 += 4) {
+            float v[K][4];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (k * STEP >= left) continue;
+                if (!(p.G & 3)) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4*>(s + size_t(k * STEP) * p.G + g0));
+                    v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[k][e] = g0 + e < p.G ? __ldcg(s + size_t(k * STEP) * p.G + g0 + e) : 0.f;
+                }
+            }
+            if (g0 == 0) {
+                if (int(threadIdx.x) < p.G) s_lse[threadIdx.x] = lse;
+                __syncthreads();
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k * STEP < left && g0 + e < p.G) acc[k] += ex2_approx(fmaf(v[k][e], p.scale_log2, -s_lse[g0 + e]));
         }
     }
-    if (key < len) *w = old + acc;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+        if (k * STEP < left) w[k * STEP] = old[k] + acc[k];
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
 // A chunk of T new tokens behind pos0: row t sees the keys 0 .. pos0 + t.
 //
 // An item is 128 keys of a (batch, KV head); its units are the tiles of query rows that see any of them, each of one head and 128
-// tokens or, for a chunk of fewer tokens, of several heads and all of them.  The units of all items are numbered through and CTA c of n
-// takes the units [c total / n, (c + 1) total / n): equal work whatever the diagonal does.  A piece that is not a whole item is left
-// in the workspace and key_weights_add_kernel adds the pieces up in their order, so a call repeats bit for bit.
+// tokens or, for a chunk of fewer tokens, of several heads and all of them.  The units of all items are numbered through and the CTAs
+// take ranges of them of the same length (to one): equal work whatever the diagonal does.  What a CTA's groups of warps have added up of an
+// item they leave in the workspace, each for itself (joined within the CTA the groups waited for each other at every item's end), and
+// key_weights_add_kernel adds these up in their order, so a call repeats bit for bit.
 //
-// Roles (320 threads): warps 0-7 exponentials and sums, two groups of four that take units in turn, thread = key; warp 8 loads (K of
-// an item, a ring of Q tiles); warp 9 issues the products.  TMEM: four score buffers of 128 columns, two per group.
+// Roles (608 threads): warps 0-15 exponentials and sums, four groups of four that take units in turn, thread = key; warp 16 loads (K
+// of an item, a ring of Q tiles); warp 17 issues the products; warp 18 brings the columns' lse.  TMEM: four score buffers of 128 columns,
+// one per group.
 // What bounds it: 128 x 128 exponentials a unit at 16 a clock, 1024 clocks, where the product takes 256 (D = 128).
 struct KeyWeightsParams {
     const float* lse;   // [B, Hq, T]
     float* w;           // [B, Hkv, L_cap]
-    float* part;        // [item + CTA][128]
+    float* part;        // [item + CTA][group of warps][128]
     int* status;
     int T, pos0, L, L_cap, Hq, Hkv, group;
     int tokens, heads;  // of a unit: tokens * heads <= 128
     int n_qt, n_hc;     // tiles of tokens, chunks of heads
     int n_kt, full_kt;  // tiles of keys; those up to this one are seen by every tile of tokens
-    long long total;    // units
+    FastDiv div_hc, div_tokens;
+    int total;          // units
+    int n_ctas, per_cta, more;  // CTAs, units of each, the first `more` of which have one more
     float scale_log2;
 };
 
+constexpr int kKeyWeightsGroups = 4;
 template <int D>
 struct KeyWeightsCfg {
     static constexpr int kTileBytes = 128 * D * 2, kBoxBytes = 128 * 128, kBoxes = D / 64;
     static constexpr int kStages = 3;
-    static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 4 * 512 + 2 * 1024 + 512 + 256;
+    static constexpr int kSmemBytes = (2 + kStages) * kTileBytes + 2 * kKeyWeightsGroups * 512 + 512 + 256;
 };
-constexpr int kKeyWeightsThreads = 320;
+constexpr int kKeyWeightsThreads = (kKeyWeightsGroups * 4 + 3) * 32;
 
-// Units of a (batch, KV head) in front of key tile kt, per chunk of heads: tile i is seen by n_qt - max(0, i - full_kt) tiles of tokens
-__host__ __device__ __forceinline__ long long key_weights_before(const KeyWeightsParams& p, int kt) {
-    const long long m = kt > p.full_kt ? kt - p.full_kt : 0;
-    return ((long long)kt * p.n_qt - m * (m - 1) / 2) * p.n_hc;
+// Units of a (batch, KV head) in front of key tile kt: tile i is seen by n_qt - max(0, i - full_kt) tiles of tokens
+__host__ __device__ __forceinline__ int key_weights_before(const KeyWeightsParams& p, int kt) {
+    const int m = kt > p.full_kt ? kt - p.full_kt : 0;
+    return (kt * p.n_qt - m * (m - 1) / 2) * p.n_hc;
 }
 struct KeyWeightsItem {
-    int bh, kt;         // batch * Hkv + KV head, tile of keys
-    long long start;    // its first unit, and how many it has
-    int units;
+    int bh, kt;        // batch * Hkv + KV head, tile of keys
+    int start, units;  // its first unit, and how many it has
 };
 // The item that unit u (< total) belongs to
-__host__ __device__ __forceinline__ KeyWeightsItem key_weights_item(const KeyWeightsParams& p, long long u) {
-    const long long per = key_weights_before(p, p.n_kt);
+__host__ __device__ __forceinline__ KeyWeightsItem key_weights_item(const KeyWeightsParams& p, int u) {
+    const int per = key_weights_before(p, p.n_kt);
     KeyWeightsItem it;
-    it.bh = int(u / per);
-    const long long r = u - it.bh * per;
+    it.bh = u / per;
+    const int r = u - it.bh * per;
     int lo = 0, hi = p.n_kt - 1;  // the last tile that begins at or before r
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -113,40 +138,67 @@ __host__ __device__ __forceinline__ KeyWeightsItem key_weights_item(const KeyWei
     }
     it.kt = lo;
     it.start = it.bh * per + key_weights_before(p, lo);
-    it.units = int(key_weights_before(p, lo + 1) - key_weights_before(p, lo));
+    it.units = key_weights_before(p, lo + 1) - key_weights_before(p, lo);
     return it;
 }
 __host__ __device__ __forceinline__ void key_weights_next(const KeyWeightsParams& p, KeyWeightsItem& it) {
     it.start += it.units;
     if (++it.kt == p.n_kt) it.kt = 0, ++it.bh;
-    it.units = int(key_weights_before(p, it.kt + 1) - key_weights_before(p, it.kt));
+    it.units = key_weights_before(p, it.kt + 1) - key_weights_before(p, it.kt);
 }
-__host__ __device__ __forceinline__ long long key_weights_range(const KeyWeightsParams& p, int c, int n) { return p.total / n * c + p.total % n * c / n; }
+// First unit of CTA c's range, and the CTA whose range holds unit u
+__host__ __device__ __forceinline__ int key_weights_range(const KeyWeightsParams& p, int c) { return c * p.per_cta + (c < p.more ? c : p.more); }
+__host__ __device__ __forceinline__ int key_weights_cta(const KeyWeightsParams& p, int u) {
+    const int longer = p.more * (p.per_cta + 1);
+    return u < longer ? u / (p.per_cta + 1) : p.more + (u - longer) / p.per_cta;
+}
+
+// Two exponentials 2^x on the FMA pipes, for the share of a unit's that the special-function units are spared: x = n + f with n the
+// nearest whole number (the addition of 1.5 * 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by a polynomial of degree 5 whose
+// coefficients minimise the largest relative error (7.5e-8; 2.1e-7 with the FP32 arithmetic), times 2^n made of its exponent bits.
+// Clamped to -127 .. 128, whose exponent bits are those of 0 and infinity; NaN stays NaN.
+__device__ __forceinline__ uint64_t exp2_fma_f32x2(uint64_t x2) {
+    float x0, x1;
+    unpack_f32x2(x2, x0, x1);
+    asm("min.NaN.f32 %0, %0, 0f43000000;\n\tmax.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x0));
+    asm("min.NaN.f32 %0, %0, 0f43000000;\n\tmax.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x1));
+    const uint64_t x = pack_f32x2(x0, x1), magic = pack_f32x2(12582912.f, 12582912.f), unmagic = pack_f32x2(-12582912.f, -12582912.f);
+    const uint64_t t = add_f32x2(x, magic);
+    const uint64_t f = fma_f32x2(add_f32x2(t, unmagic), pack_f32x2(-1.f, -1.f), x);
+    uint64_t r = fma_f32x2(f, pack_f32x2(0.001327647129073739f, 0.001327647129073739f), pack_f32x2(0.009675541892647743f, 0.009675541892647743f));
+    r = fma_f32x2(r, f, pack_f32x2(0.05550713464617729f, 0.05550713464617729f));
+    r = fma_f32x2(r, f, pack_f32x2(0.24022120237350464f, 0.24022120237350464f));
+    r = fma_f32x2(r, f, pack_f32x2(0.6931469440460205f, 0.6931469440460205f));
+    r = fma_f32x2(r, f, pack_f32x2(1.0000001192092896f, 1.0000001192092896f));
+    float t0, t1;
+    unpack_f32x2(t, t0, t1);
+    const uint64_t s = pack_f32x2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
+    return mul_f32x2(r, s);
+}
 
 template <int D>
 __global__ void __launch_bounds__(kKeyWeightsThreads, 1)
 key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const KeyWeightsParams p) {
     using Cfg = KeyWeightsCfg<D>;
-    constexpr int NST = Cfg::kStages;
+    constexpr int NST = Cfg::kStages, NG = kKeyWeightsGroups;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sK = smem;                              // [2]
     uint8_t* sQ = sK + 2 * Cfg::kTileBytes;          // [NST]
-    float* sLse = reinterpret_cast<float*>(sQ + NST * Cfg::kTileBytes);  // [group of warps][2][128]
-    float* sW = sLse + 4 * 128;                      // [2][2][128]
-    int* sTok = reinterpret_cast<int*>(sW + 4 * 128);  // [128] token within the unit
+    float* sLse = reinterpret_cast<float*>(sQ + NST * Cfg::kTileBytes);  // [group of warps][2][128], negative
+    int* sTok = reinterpret_cast<int*>(sLse + 2 * NG * 128);  // [128] token within the unit
     uint64_t* bars = reinterpret_cast<uint64_t*>(sTok + 128);
     uint64_t* bar_k_full = bars;           // [2] (phase: piece / 2)
     uint64_t* bar_k_free = bars + 2;       // [2]
     uint64_t* bar_q_full = bars + 4;       // [NST] (phase: unit / NST)
     uint64_t* bar_q_free = bars + 4 + NST; // [NST]
-    uint64_t* bar_s_full = bars + 4 + 2 * NST;   // [4] buffer unit % 4 (phase: unit / 4)
-    uint64_t* bar_s_free = bars + 8 + 2 * NST;   // [4]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12 + 2 * NST);
+    uint64_t* bar_s_full = bars + 4 + 2 * NST;   // [NG] buffer unit % NG (phase: unit / NG)
+    uint64_t* bar_s_free = bars + 4 + NG + 2 * NST;  // [NG]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 4 + 2 * NG + 2 * NST);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cols = p.tokens * p.heads;
-    if (warp == 8 && lane == 0) {
+    if (warp == 4 * NG && lane == 0) {
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
         for (int i = 0; i < 2; ++i) {
@@ -157,19 +209,19 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             mbar_init(&bar_q_full[i], 1);
             mbar_init(&bar_q_free[i], 1);
         }
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&bar_s_full[i], 1);
+        for (int i = 0; i < NG; ++i) {
+            mbar_init(&bar_s_full[i], 2);  // the products and the lse
             mbar_init(&bar_s_free[i], 128);
         }
         fence_mbar_init();
         *abort_flag = 0;
     }
-    if (warp == 9) {
+    if (warp == 4 * NG + 1) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    if (cols < 128 && tid < 256) {  // rows that no load writes: columns that count for nothing, but NaN times nothing is NaN
-        for (int i = tid; i < NST * Cfg::kTileBytes / 16; i += 256) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (cols < 128 && tid < NG * 128) {  // rows that no load writes: columns that count for nothing, but NaN times nothing is NaN
+        for (int i = tid; i < NST * Cfg::kTileBytes / 16; i += NG * 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
     }
     if (tid < 128) sTok[tid] = tid % p.tokens;
@@ -178,23 +230,27 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int failed = *reinterpret_cast<volatile int*>(p.status);
         if (failed != 0) *abort_flag = failed;
     }
-    const long long u0 = key_weights_range(p, int(blockIdx.x), int(gridDim.x)), u1 = key_weights_range(p, int(blockIdx.x) + 1, int(gridDim.x));
-    const int n = int(u1 - u0);
+    grid_dep_launch();  // (the kernel behind takes next to nothing of an SM)
+    const int u0 = key_weights_range(p, int(blockIdx.x)), n = key_weights_range(p, int(blockIdx.x) + 1) - u0;
     KeyWeightsItem it = key_weights_item(p, u0);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
     // unit `u` of item `it`: its tile of tokens (the last ones are seen by most) and its chunk of heads
-    auto unit_qt = [&](const KeyWeightsItem& it, int in_item) { return p.n_qt - 1 - in_item / p.n_hc; };
+    auto unit_qt = [&](int in_item, int* hc) {
+        const int q = int(fastdiv(in_item, p.div_hc));
+        *hc = in_item - q * p.n_hc;
+        return p.n_qt - 1 - q;
+    };
 
     if (*abort_flag != 0) {
         // an earlier kernel has failed
-    } else if (warp == 8) {
+    } else if (warp == 4 * NG) {
         // ------------------------------------------------------------------ producer
         bool ok = true;
         for (int i = 0, piece = 0; ok && i < n; ++piece) {
-            const int first = int(u0 + i - it.start), m = min(it.units - first, n - i);
+            const int first = u0 + i - it.start, m = min(it.units - first, n - i);
             const int b = it.bh / p.Hkv, hk = it.bh - b * p.Hkv;
             if (piece >= 2) ok = mbar_wait_warp(&bar_k_free[piece & 1], uint32_t(piece / 2 - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_FREE);
             if (!ok) break;
@@ -206,7 +262,8 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             __syncwarp();
             for (int e = 0; e < m; ++e, ++i) {
-                const int s = i % NST, qt = unit_qt(it, first + e), hc = (first + e) % p.n_hc;
+                int hc;
+                const int s = i % NST, qt = unit_qt(first + e, &hc);
                 if (i >= NST) ok = mbar_wait_warp(&bar_q_free[s], uint32_t(i / NST - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_FREE);
                 if (!ok) break;
                 if (elect_one()) {
@@ -219,18 +276,18 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             key_weights_next(p, it);
         }
-    } else if (warp == 9) {
+    } else if (warp == 4 * NG + 1) {
         // ------------------------------------------------------------------ products
         constexpr uint32_t idesc = make_idesc_bf16(128, 128, 0, 0);
         bool ok = true;
         for (int i = 0, piece = 0; ok && i < n; ++piece) {
-            const int first = int(u0 + i - it.start), m = min(it.units - first, n - i);
+            const int first = u0 + i - it.start, m = min(it.units - first, n - i);
             ok = mbar_wait_warp(&bar_k_full[piece & 1], uint32_t(piece / 2) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
             const uint64_t k_desc = make_sdesc_sw128(smem_u32(sK + (piece & 1) * Cfg::kTileBytes), 16, 1024);
             for (int e = 0; ok && e < m; ++e, ++i) {
-                const int s = i % NST, buf = i & 3;
+                const int s = i % NST, buf = i % NG;
                 ok = mbar_wait_warp(&bar_q_full[s], uint32_t(i / NST) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
-                if (ok && i >= 4) ok = mbar_wait_warp(&bar_s_free[buf], uint32_t(i / 4 - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_SOFTMAX);
+                if (ok && i >= NG) ok = mbar_wait_warp(&bar_s_free[buf], uint32_t(i / NG - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_SOFTMAX);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint64_t q_desc = make_sdesc_sw128(smem_u32(sQ + s * Cfg::kTileBytes), 16, 1024);
@@ -247,116 +304,161 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             key_weights_next(p, it);
         }
         // nothing may be in flight when tensor memory is freed: the last unit's products
-        if (ok && n > 0) mbar_wait_warp(&bar_s_full[(n - 1) & 3], uint32_t((n - 1) / 4) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
+        if (ok && n > 0) mbar_wait_warp(&bar_s_full[(n - 1) % NG], uint32_t((n - 1) / NG) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
+    } else if (warp == 4 * NG + 2) {
+        // ------------------------------------------------------------------ lse of the units' columns, negative and in powers of two
+        // lane's columns: lane + 32 k
+        int h_col[4], t_col[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) h_col[c] = int(fastdiv(lane + 32 * c, p.div_tokens)), t_col[c] = lane + 32 * c - h_col[c] * p.tokens;
+        auto rows_of = [&](int bh) {
+            const int b = bh / p.Hkv;
+            return p.lse + (size_t(b) * p.Hq + (bh - b * p.Hkv) * p.group) * p.T;
+        };
+        const float* rows = rows_of(it.bh);
+        int in_item = u0 - it.start;
+        float v[2][4];
+        auto load = [&](float (&v)[4]) {  // of the unit at `in_item` of `it`, and on to the next
+            int hc;
+            const int qt = unit_qt(in_item, &hc);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int t = qt * p.tokens + t_col[c];
+                // 2^(x - inf) = 0
+                v[c] = lane + 32 * c < cols && t < p.T ? __ldg(rows + size_t(hc * p.heads + h_col[c]) * p.T + t) * -kLog2e : -INFINITY;
+            }
+            if (++in_item == it.units) {
+                const int bh = it.bh;
+                key_weights_next(p, it);
+                if (it.bh != bh) rows = rows_of(it.bh);
+                in_item = 0;
+            }
+        };
+        bool ok = true;
+        if (n > 0) load(v[0]);
+        auto put = [&](int i, float (&now)[4], float (&then)[4]) {
+            if (i + 1 < n) load(then);
+            // (the group's scores of the unit before are in registers, so it is through with the lse of the one before that, whose buffer this is)
+            if (i >= NG) ok = mbar_wait_warp(&bar_s_free[i % NG], uint32_t(i / NG - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_SOFTMAX);
+            if (!ok) return;
+            float* lse = sLse + ((i % NG) * 2 + (i / NG & 1)) * 128 + lane;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) lse[32 * c] = now[c];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_s_full[i % NG]);
+        };
+        for (int i = 0; ok && i < n; i += 2) {
+            put(i, v[0], v[1]);
+            if (ok && i + 1 < n) put(i + 1, v[1], v[0]);
+        }
     } else {
         // ------------------------------------------------------------------ exponentials and sums
         const int wg = warp >> 2, key = tid & 127;
-        const uint32_t t_lane = tmem + (uint32_t((warp & 3) * 32) << 16);
-        // The lse of this thread's column in the unit that lies `i` units into the CTA's range
-        auto load_lse = [&](const KeyWeightsItem& it, int in_item) -> float {
-            const int qt = unit_qt(it, in_item), hc = in_item % p.n_hc;
-            const int t = qt * p.tokens + sTok[key], h = hc * p.heads + key / p.tokens;
-            const int b = it.bh / p.Hkv, hk = it.bh - b * p.Hkv;
-            if (key >= cols || t >= p.T || h >= p.group) return INFINITY;  // 2^(x - inf) = 0
-            return __ldg(p.lse + (size_t(b) * p.Hq + hk * p.group + h) * p.T + t) * kLog2e;
-        };
+        const uint32_t t_s = tmem + (uint32_t((warp & 3) * 32) << 16) + wg * 128;
+        const int n_c = (cols + 15) / 16;
+        const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
         bool ok = true;
-        float next = 0.f;
-        KeyWeightsItem ahead = it;  // the item of this group's next unit
-        auto fetch = [&](int i) {
-            if (i >= n) return;
-            while (u0 + i >= ahead.start + ahead.units) key_weights_next(p, ahead);
-            next = load_lse(ahead, int(u0 + i - ahead.start));
-        };
-        fetch(wg);
-        for (int i = 0, piece = 0; i < n; ++piece) {
-            const int first = int(u0 + i - it.start), m = min(it.units - first, n - i);
+        for (int i = 0; ok && i < n;) {
+            const int first = u0 + i - it.start, m = min(it.units - first, n - i);
             float acc = 0.f;
-            for (int e = (i & 1) == wg ? 0 : 1; e < m; e += 2) {
-                const int k = i + e, buf = k & 3, qt = unit_qt(it, first + e);
-                float* lse = sLse + (wg * 2 + ((k >> 1) & 1)) * 128;
-                lse[key] = next;
-                fetch(k + 2);
-                named_bar_sync(1 + wg, 128);  // (the buffer's last readers were two units of this group ago: one such barrier between)
-                if (ok) ok = mbar_wait_warp(&bar_s_full[buf], uint32_t(k / 4) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
-                if (!ok) continue;  // (a warp that has given up still meets the others at the named barriers)
+            const int k_lim = it.kt * 128 + key - p.pos0;  // tokens below it do not see the key
+            for (int e = (wg - i % NG + NG) % NG; e < m; e += NG) {
+                int hc;
+                const int k = i + e, lim = k_lim - unit_qt(first + e, &hc) * p.tokens;
+                const bool diagonal = lim + 127 - key > 0;  // whether any key of the tile is unseen by the unit's first token
+                const float* lse = sLse + (wg * 2 + (k / NG & 1)) * 128;
+                ok = mbar_wait_warp(&bar_s_full[wg], uint32_t(k / NG) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
+                if (!ok) break;
                 tc_fence_after_sync();
-                const int k_pos = it.kt * 128 + key, t_first = qt * p.tokens;  // this thread's key, the unit's first token
-                const bool diagonal = it.kt * 128 + 127 > p.pos0 + t_first;
-                const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
                 uint64_t sum2[2] = {0ull, 0ull};
-                const uint32_t t_s = t_lane + buf * 128;
-                const int n_c = (cols + 31) / 32;
-                for (int c = 0; c < n_c; ++c) {
-                    uint32_t v[32];
-                    tmem_ld_x32(t_s + c * 32, v);
-                    tmem_wait_ld();
+                uint32_t v[2][16];
+                auto chunk = [&](int c, uint32_t (&v)[16]) {
                     if (diagonal) {
+                        if (p.heads == 1) {  // (column = token)
+                            if (lim > c * 16) {
 #pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (k_pos > p.pos0 + t_first + sTok[c * 32 + x]) v[x] = 0xff800000u;  // -inf
+                                for (int x = 0; x < 16; ++x)
+                                    if (c * 16 + x < lim) v[x] = 0xff800000u;  // -inf
+                            }
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                if (sTok[c * 16 + x] < lim) v[x] = 0xff800000u;
+                        }
                     }
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4) {
-                        const float4 ls = *reinterpret_cast<const float4*>(lse + c * 32 + x);
-                        float a0, a1, a2, a3;
-                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])), scale2, pack_f32x2(-ls.x, -ls.y)), a0, a1);
-                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[x + 2]), __uint_as_float(v[x + 3])), scale2, pack_f32x2(-ls.z, -ls.w)), a2, a3);
-                        sum2[0] = add_f32x2(sum2[0], pack_f32x2(ex2_approx(a0), ex2_approx(a1)));
-                        sum2[1] = add_f32x2(sum2[1], pack_f32x2(ex2_approx(a2), ex2_approx(a3)));
+                    for (int x = 0; x < 16; x += 8) {
+                        const float4 la = *reinterpret_cast<const float4*>(lse + c * 16 + x), lb = *reinterpret_cast<const float4*>(lse + c * 16 + x + 4);
+                        const float l8[8] = {la.x, la.y, la.z, la.w, lb.x, lb.y, lb.z, lb.w};
+#pragma unroll
+                        for (int e2 = 0; e2 < 4; ++e2) {
+                            const uint64_t a = fma_f32x2(pack_f32x2(__uint_as_float(v[x + 2 * e2]), __uint_as_float(v[x + 2 * e2 + 1])), scale2,
+                                                         pack_f32x2(l8[2 * e2], l8[2 * e2 + 1]));
+                            if (e2 == 3) {  // a quarter of them on the FMA pipes
+                                sum2[1] = add_f32x2(sum2[1], exp2_fma_f32x2(a));
+                            } else {
+                                float a0, a1;
+                                unpack_f32x2(a, a0, a1);
+                                sum2[e2 & 1] = add_f32x2(sum2[e2 & 1], pack_f32x2(ex2_approx(a0), ex2_approx(a1)));
+                            }
+                        }
+                    }
+                };
+                // The next 16 columns are on their way while 16 are worked on; the buffer goes back once all are in registers.  (Two chunks
+                // of code, not eight: the instruction cache.)
+                tmem_ld_x16(t_s, v[0]);
+#pragma unroll 1
+                for (int c = 0; c < n_c; c += 2) {
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        if (c + d >= n_c) break;
+                        tmem_wait_ld();
+                        if (c + d + 1 < n_c) {
+                            tmem_ld_x16(t_s + (c + d + 1) * 16, v[d ^ 1]);
+                        } else {
+                            tc_fence_before_sync();
+                            mbar_arrive(&bar_s_free[wg]);
+                        }
+                        chunk(c + d, v[d]);
                     }
                 }
-                tc_fence_before_sync();
-                mbar_arrive(&bar_s_free[buf]);
                 float s0, s1;
                 unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
                 acc += s0 + s1;
             }
             i += m;
-            // the two groups' sums of the piece
-            float* w2 = sW + (piece & 1) * 256;
-            if (wg == 1) w2[key] = acc;
-            named_bar_sync(3, 256);
-            if (wg == 0 && ok && *abort_flag == 0) {
-                acc += w2[key];
-                if (m == it.units) {
-                    if (it.kt * 128 + key < p.L) p.w[size_t(it.bh) * p.L_cap + it.kt * 128 + key] += acc;
-                } else {
-                    p.part[(size_t(it.bh) * p.n_kt + it.kt + blockIdx.x) * 128 + key] = acc;
-                }
-            }
+            if (ok) p.part[((size_t(it.bh) * p.n_kt + it.kt + blockIdx.x) * NG + wg) * 128 + key] = acc;
             key_weights_next(p, it);
         }
     }
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 4 * NG + 1) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
 }
 
-// Items that several CTAs share: their pieces added up in their order.  grid: items; thread = key.
-__global__ void __launch_bounds__(128) key_weights_add_kernel(const KeyWeightsParams p, const int n_ctas) {
-    const int bh = blockIdx.x / p.n_kt, kt = blockIdx.x - bh * p.n_kt, key = kt * 128 + threadIdx.x;
-    const long long per = key_weights_before(p, p.n_kt), start = bh * per + key_weights_before(p, kt), end = bh * per + key_weights_before(p, kt + 1);
-    // the CTA whose range holds unit u: the last one that begins at or before it
-    auto cta_of = [&](long long u) {
-        int lo = 0, hi = n_ctas - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) / 2;
-            if (key_weights_range(p, mid, n_ctas) <= u) lo = mid;
-            else hi = mid - 1;
-        }
-        return lo;
-    };
-    const int first = cta_of(start), last = cta_of(end - 1);
+// The items' pieces added up in their order.  grid: items; thread = key.
+__global__ void __launch_bounds__(128) key_weights_add_kernel(const KeyWeightsParams p) {
+    const int bh = int(blockIdx.x) / p.n_kt, kt = int(blockIdx.x) - bh * p.n_kt, key = kt * 128 + threadIdx.x;
+    const int per = key_weights_before(p, p.n_kt), start = bh * per + key_weights_before(p, kt), end = bh * per + key_weights_before(p, kt + 1);
+    const int first = key_weights_cta(p, start), last = key_weights_cta(p, end - 1);
+    constexpr int NG = kKeyWeightsGroups;
     grid_dep_wait();
-    if (first == last || key >= p.L || *reinterpret_cast<volatile int*>(p.status) != 0) return;
+    if (key >= p.L || *reinterpret_cast<volatile int*>(p.status) != 0) return;
     float* const w = p.w + size_t(bh) * p.L_cap + key;
+    const float old = *w;
     float acc = 0.f;
-    for (int c = first; c <= last; ++c) acc += __ldcg(p.part + (size_t(blockIdx.x) + c) * 128 + threadIdx.x);
-    *w += acc;
+    for (int c = first; c <= last; ++c) {
+        const float* const part = p.part + (size_t(blockIdx.x) + c) * NG * 128 + threadIdx.x;
+        float v[NG];
+#pragma unroll
+        for (int g = 0; g < NG; ++g) v[g] = __ldcg(part + g * 128);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) acc += v[g];
+    }
+    *w = old + acc;
 }
 
 }  // namespace b200attn

@@ -29,7 +29,7 @@ static int key_weights(std::mt19937& rng) {
     while (p.heads * 2 * p.tokens <= 128 && p.group % (p.heads * 2) == 0) p.heads *= 2;
     p.n_qt = (T + p.tokens - 1) / p.tokens, p.n_hc = p.group / p.heads, p.n_kt = (p.L + 127) / 128;
     p.full_kt = p.n_qt == 1 ? p.n_kt : (pos0 + 127) / 128;
-    p.total = (long long)B * p.Hkv * key_weights_before(p, p.n_kt);
+    p.total = B * p.Hkv * key_weights_before(p, p.n_kt);
     // the units of a key tile are the tiles of tokens that see any of its keys
     for (int kt = 0; kt < p.n_kt; ++kt) {
         int seen = 0;
@@ -43,21 +43,23 @@ static int key_weights(std::mt19937& rng) {
         }
         CHECK(seen * p.n_hc == key_weights_before(p, kt + 1) - key_weights_before(p, kt));
     }
-    const int n = int(std::min<long long>(upto(1, 148), p.total));
+    const int n = p.n_ctas = std::min(upto(1, 148), p.total);
+    p.per_cta = p.total / n, p.more = p.total % n;
     std::vector<int> taken(p.total);
     std::set<long long> slots;
     for (int c = 0; c < n; ++c) {
-        const long long u0 = key_weights_range(p, c, n), u1 = key_weights_range(p, c + 1, n);
+        const int u0 = key_weights_range(p, c), u1 = key_weights_range(p, c + 1);
         CHECK(u1 > u0 && u1 - u0 <= p.total / n + 1);
         KeyWeightsItem it = key_weights_item(p, u0);
-        for (long long u = u0; u < u1;) {
+        for (int u = u0; u < u1;) {
             CHECK(it.start <= u && u < it.start + it.units && it.bh < B * p.Hkv && it.kt < p.n_kt);
-            const long long end = std::min<long long>(u1, it.start + it.units);
-            if (!(u == it.start && end == it.start + it.units)) {
-                const long long slot = (long long)it.bh * p.n_kt + it.kt + c;
-                CHECK(slot < (long long)B * p.Hkv * p.n_kt + n && slots.insert(slot).second);
+            const int end = std::min(u1, it.start + it.units);
+            const long long slot = (long long)it.bh * p.n_kt + it.kt + c;
+            CHECK(slot < (long long)B * p.Hkv * p.n_kt + n && slots.insert(slot).second);
+            for (; u < end; ++u) {
+                CHECK(key_weights_cta(p, u) == c);
+                ++taken[u];
             }
-            for (; u < end; ++u) ++taken[u];
             key_weights_next(p, it);
         }
     }
@@ -66,20 +68,21 @@ static int key_weights(std::mt19937& rng) {
 }
 
 static int prefix() {
-    for (int n = 1; n < 40; ++n) {
-        int i = 0;  // the products: S of tile 0, then S of tile j + 1 and P V of tile j
-        auto next = [&](bool k, int j) {
-            int lj;
-            const bool lk = prefix_load_at(i, n, &lj);
-            return lk == k && lj == j && i++ == (k ? prefix_k_at(j) : prefix_v_at(j, n));
-        };
-        CHECK(next(true, 0));
-        for (int j = 0; j < n; ++j) {
-            if (j + 1 < n) CHECK(next(true, j + 1));
-            CHECK(next(false, j));
+    for (int ahead = 1; ahead <= 2; ++ahead)
+        for (int n = 1; n < 40; ++n) {
+            int i = 0;  // the products: S of the first tiles, then P V of tile j and S of tile j + ahead
+            auto next = [&](bool k, int j) {
+                int lj;
+                const bool lk = prefix_load_at(i, n, ahead, &lj);
+                return lk == k && lj == j && i++ == (k ? prefix_k_at(j, ahead) : prefix_v_at(j, n, ahead));
+            };
+            for (int j = 0; j < ahead && j < n; ++j) CHECK(next(true, j));
+            for (int j = 0; j < n; ++j) {
+                CHECK(next(false, j));
+                if (j + ahead < n) CHECK(next(true, j + ahead));
+            }
+            CHECK(i == 2 * n);
         }
-        CHECK(i == 2 * n);
-    }
     return 0;
 }
 
