@@ -329,7 +329,8 @@ int b200attn_kv_append_rotary(const void* xq, const void* xk, const void* xv, in
  *
  * b200attn_key_weights: the same sums over a chunk of T new tokens at positions (rows) pos0 .. pos0 + T - 1 of the cache, each of
  *   which sees the keys up to its own, from the lse [B, Hq, T] that b200attn_fwd_kvcache_at has left; q [.., T, ..] in q_layout.
- *   Keys 0 .. pos0 + T - 1.  For the sums over the last tokens of a prompt only, pass these tokens' q, lse and position.
+ *   Keys 0 .. pos0 + T - 1.  new_lens: [B] (device, int32), of the T rows of each sequence those that count (the first ones, of a padded
+ *   batch), or NULL: all.  For the sums over the last tokens of a prompt only, pass these tokens' q, lse and position.
  *
  * b200attn_kv_evict: of each (batch, KV head)'s first n = lens[b] rows (clamped to 0 .. L; NULL: L) min(n, keep) stay: the rows whose
  *   position is above newest - recent (the newest being the largest of the n positions, which are distinct; recent <= keep), then those of
@@ -350,13 +351,14 @@ int b200attn_decode_weights(const void* q, const void* kcache, const void* vcach
                             const int* lens, int B, int L, int L_cap, int Hq, int Hkv, int D, float softmax_scale,
                             void* workspace, size_t workspace_bytes, void* stream);
 size_t b200attn_decode_weights_workspace_bytes(int B, int L, int Hq, int Hkv, int D);
-int b200attn_key_weights(const void* q, int q_layout, const void* kcache, const float* lse, float* weights, int B, int T,
-                         int pos0, int L_cap, int Hq, int Hkv, int D, float softmax_scale, void* workspace,
+int b200attn_key_weights(const void* q, int q_layout, const void* kcache, const float* lse, float* weights,
+                         const int* new_lens, int B, int T, int pos0, int L_cap, int Hq, int Hkv, int D, float softmax_scale, void* workspace,
                          size_t workspace_bytes, void* stream);
 size_t b200attn_key_weights_workspace_bytes(int B, int T, int pos0, int Hkv);
 int b200attn_kv_evict(void* kcache, void* vcache, const float* weights, const int* positions, float* weights_out,
                       int* positions_out, const int* lens, int B, int L, int L_cap, int Hkv, int D, int keep, int recent,
-                      void* stream);
+                      void* workspace, size_t workspace_bytes, void* stream);
+size_t b200attn_kv_evict_workspace_bytes(int B, int L, int Hkv, int keep); /* 0: none is needed */
 
 /*
  * Diagnostics for benchmarks (no counterpart in the reference): when three CUDA events are

@@ -75,6 +75,7 @@ SYMBOLS = (
     "b200attn_key_weights",
     "b200attn_key_weights_workspace_bytes",
     "b200attn_kv_evict",
+    "b200attn_kv_evict_workspace_bytes",
     "b200attn_last_device_status",
     "b200attn_strerror",
     "b200attn_version",
@@ -179,12 +180,14 @@ def load() -> ctypes.CDLL:
     L.b200attn_decode_weights.restype = i
     L.b200attn_decode_weights_workspace_bytes.argtypes = [i] * 5
     L.b200attn_decode_weights_workspace_bytes.restype = sz
-    L.b200attn_key_weights.argtypes = [vp, i, vp, vp, vp] + [i] * 7 + [f, vp, sz, vp]
+    L.b200attn_key_weights.argtypes = [vp, i, vp, vp, vp, vp] + [i] * 7 + [f, vp, sz, vp]
     L.b200attn_key_weights.restype = i
     L.b200attn_key_weights_workspace_bytes.argtypes = [i] * 4
     L.b200attn_key_weights_workspace_bytes.restype = sz
-    L.b200attn_kv_evict.argtypes = [vp] * 7 + [i] * 7 + [vp]
+    L.b200attn_kv_evict.argtypes = [vp] * 7 + [i] * 7 + [vp, sz, vp]
     L.b200attn_kv_evict.restype = i
+    L.b200attn_kv_evict_workspace_bytes.argtypes = [i] * 4
+    L.b200attn_kv_evict_workspace_bytes.restype = sz
     L.b200attn_last_device_status.argtypes = [vp]
     L.b200attn_last_device_status.restype = i
     L.b200attn_strerror.argtypes = [i]

@@ -106,17 +106,39 @@ int launch_key_weights(const CUtensorMap& tq, const CUtensorMap& tk, const KeyWe
     return B200ATTN_OK;
 }
 
-template <int D, bool BIG>
-int launch_evict(const EvictParams& p, unsigned grid, cudaStream_t st) {
+// Eviction by one kernel, whose CTAs select for themselves, or by two: with more units than this an SM would have to select more often than
+// its share of the moves is worth.
+constexpr int kEvictListUnits = 74;
+
+template <int D, bool BIG, bool LIST>
+int launch_evict_kernel(const EvictParams& p, unsigned grid, cudaStream_t st) {
     static bool set[kMaxDevices] = {false};
-    const int rc = set_smem_once(kv_evict_kernel<D, BIG>, kEvictFixedSmem + (BIG ? 0 : kEvictMaxKeys * 4), set);
+    const int rc = set_smem_once(kv_evict_kernel<D, BIG, LIST>, kEvictFixedSmem + (BIG ? 0 : kEvictMaxKeys * 4), set);
     if (rc) return rc;
-    if (launch_pdl(kv_evict_kernel<D, BIG>, dim3(grid), kEvictThreads, kEvictFixedSmem + (BIG ? 0 : (size_t)p.L * 4), st, p) != cudaSuccess) {
+    if (launch_pdl(kv_evict_kernel<D, BIG, LIST>, dim3(grid), kEvictThreads, kEvictFixedSmem + (BIG ? 0 : (size_t)p.L * 4), st, p) != cudaSuccess) {
         cudaGetLastError();
         return B200ATTN_ERR_CUDA;
     }
     return B200ATTN_OK;
 }
+template <int D>
+int launch_evict(const EvictParams& p, long long units, cudaStream_t st) {
+    const bool big = p.L > kEvictMaxKeys;
+    if (!p.moves) {
+        const unsigned grid = (unsigned)(units * p.ranks);
+        return big ? launch_evict_kernel<D, true, false>(p, grid, st) : launch_evict_kernel<D, false, false>(p, grid, st);
+    }
+    const int rc = big ? launch_evict_kernel<D, true, true>(p, (unsigned)units, st) : launch_evict_kernel<D, false, true>(p, (unsigned)units, st);
+    if (rc) return rc;
+    if (launch_pdl(kv_move_kernel<D>, dim3((unsigned)(units * p.blocks)), kMoveThreads, 0, st, p) != cudaSuccess) {
+        cudaGetLastError();
+        return B200ATTN_ERR_CUDA;
+    }
+    return B200ATTN_OK;
+}
+// Most moves of a unit, and whether they are listed for a kernel of their own (see kv_evict.cuh)
+inline int evict_most(int L, int keep) { return std::max(0, std::min(keep, L - keep)); }
+inline bool evict_lists(long long units, int L, int keep) { return units > kEvictListUnits && evict_most(L, keep) > 0; }
 
 }  // namespace
 
@@ -216,8 +238,8 @@ extern "C" size_t b200attn_key_weights_workspace_bytes(int B, int T, int pos0, i
     return ((size_t)B * Hkv * ((pos0 + (size_t)T + 127) / 128) + sm_count()) * kKeyWeightsGroups * 128 * sizeof(float);
 }
 
-extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kcache, const float* lse, float* weights, int B, int T, int pos0,
-                                    int L_cap, int Hq, int Hkv, int D, float softmax_scale, void* workspace, size_t workspace_bytes,
+extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kcache, const float* lse, float* weights, const int* new_lens, int B,
+                                    int T, int pos0, int L_cap, int Hq, int Hkv, int D, float softmax_scale, void* workspace, size_t workspace_bytes,
                                     void* stream) {
     int rc = check_common(B, T, Hq, Hkv, D, q_layout);
     if (rc) return rc;
@@ -234,7 +256,7 @@ extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kca
     p.per_cta = p.total / p.n_ctas, p.more = p.total % p.n_ctas;
     p.status = status_ptr(&rc);
     if (!p.status) return rc;
-    p.lse = lse, p.w = weights, p.part = static_cast<float*>(workspace), p.L_cap = L_cap;
+    p.lse = lse, p.rows = new_lens, p.w = weights, p.part = static_cast<float*>(workspace), p.L_cap = L_cap;
     p.scale_log2 = scale_of(softmax_scale, D) * kLog2e;
     const Strides sq = strides_for(q_layout, Hq, T, D), sk = strides_for(B200ATTN_LAYOUT_BHTD, Hkv, L_cap, D);
     CUtensorMap tq, tk;
@@ -246,8 +268,15 @@ extern "C" int b200attn_key_weights(const void* q, int q_layout, const void* kca
     return D == 64 ? launch_key_weights<64>(tq, tk, p, (unsigned)items, st) : launch_key_weights<128>(tq, tk, p, (unsigned)items, st);
 }
 
+extern "C" size_t b200attn_kv_evict_workspace_bytes(int B, int L, int Hkv, int keep) {
+    if (B <= 0 || L <= 0 || Hkv <= 0 || keep <= 0) return 0;
+    const long long units = (long long)B * Hkv;
+    return evict_lists(units, L, keep) ? (size_t)units * (evict_most(L, keep) * sizeof(int2) + sizeof(int)) : 0;
+}
+
 extern "C" int b200attn_kv_evict(void* kcache, void* vcache, const float* weights, const int* positions, float* weights_out, int* positions_out,
-                                 const int* lens, int B, int L, int L_cap, int Hkv, int D, int keep, int recent, void* stream) {
+                                 const int* lens, int B, int L, int L_cap, int Hkv, int D, int keep, int recent, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
     if (B <= 0 || L <= 0 || Hkv <= 0 || L_cap < L || keep <= 0 || recent < 0 || recent > keep) return B200ATTN_ERR_INVALID_ARG;
     if (D != 64 && D != 128) return B200ATTN_ERR_UNSUPPORTED;
     if (!kcache || !vcache || !weights || !positions || !weights_out || !positions_out) return B200ATTN_ERR_INVALID_ARG;
@@ -263,6 +292,8 @@ extern "C" int b200attn_kv_evict(void* kcache, void* vcache, const float* weight
     if (!apart(weights, weights_out) || !apart(positions, positions_out) || !apart(weights, positions_out) || !apart(positions, weights_out) ||
         !apart(weights_out, positions_out))
         return B200ATTN_ERR_INVALID_ARG;
+    const bool lists = evict_lists(units, L, keep);
+    if (lists && !workspace_ok(workspace, workspace_bytes, b200attn_kv_evict_workspace_bytes(B, L, Hkv, keep))) return B200ATTN_ERR_WORKSPACE;
     int rc = B200ATTN_OK;
     EvictParams p = {};
     p.status = status_ptr(&rc);
@@ -270,11 +301,14 @@ extern "C" int b200attn_kv_evict(void* kcache, void* vcache, const float* weight
     p.k = static_cast<uint16_t*>(kcache), p.v = static_cast<uint16_t*>(vcache);
     p.w = weights, p.pos = positions, p.w_out = weights_out, p.pos_out = positions_out, p.lens = lens;
     p.L = L, p.L_cap = L_cap, p.Hkv = Hkv, p.keep = keep, p.recent = recent;
-    p.ranks = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, (L + 255) / 256), 4 * sm_count() / units));
-    const bool big = L > kEvictMaxKeys;
-    const long long grid = units * p.ranks;
-    if (grid >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    p.ranks = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(8, (L + 255) / 256), sm_count() / units));
+    if (lists) {
+        p.most = evict_most(L, keep);
+        p.blocks = (p.most + kMoveRows - 1) / kMoveRows;
+        p.moves = static_cast<int2*>(workspace);
+        p.n_moves = reinterpret_cast<int*>(p.moves + (size_t)units * p.most);
+    }
+    if (units * std::max(p.ranks, p.blocks) >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (D == 64) return big ? launch_evict<64, true>(p, (unsigned)grid, st) : launch_evict<64, false>(p, (unsigned)grid, st);
-    return big ? launch_evict<128, true>(p, (unsigned)grid, st) : launch_evict<128, false>(p, (unsigned)grid, st);
+    return D == 64 ? launch_evict<64>(p, units, st) : launch_evict<128>(p, units, st);
 }

@@ -858,6 +858,57 @@ bool heads_ok(const char* fn, int Hq, int Hkv, int D) {
     return true;
 }
 
+// xq, xk, xv, gamma_q, gamma_k, q_out, kcache, vcache, positions, cos, sin, rotary_dim, pairs (a number), pos, pos0, rows, row0, B, L_cap,
+// Hq, Hkv, D, eps
+PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    const char* fn = "KVCache.append";
+    B200ATTN_TRY
+    if (!arg_count(n, 23)) return nullptr;
+    ScalarType xt;
+    int xd;
+    if (!x_dtype(fn, a[0], &xt, &xd)) return nullptr;
+    const ScalarType bf = ScalarType::BFloat16, f = ScalarType::Float, i32 = ScalarType::Int;
+    for (int i : {1, 2, 5, 6, 7, 9, 10})
+        if (a[i] == Py_None) return value_error("%s: xk, xv and q_out are needed", fn);
+    if ((a[3] == Py_None) != (a[4] == Py_None)) return value_error("%s: gamma_q and gamma_k belong together", fn);
+    Items items;
+    items.add(a[6], "K cache", bf), items.add(a[7], "V cache", bf), items.add(a[0], "xq", xt), items.add(a[1], "xk", xt), items.add(a[2], "xv", xt);
+    items.add(a[5], "q_out", bf), items.add(a[3], "gamma_q", f), items.add(a[4], "gamma_k", f), items.add(a[8], "positions", i32);
+    items.add(a[9], "cos", f), items.add(a[10], "sin", f), items.add(a[13], "pos", i32), items.add(a[15], "rows", i32);
+    int rp[2], pos0, row0, d[5];
+    if (!items.check(fn) || !ints(a + 11, 2, rp) || !ints(a + 14, 1, &pos0) || !ints(a + 16, 1, &row0) || !ints(a + 17, 5, d)) return nullptr;
+    const int B = d[0], L_cap = d[1], Hq = d[2], Hkv = d[3], D = d[4];
+    const at::Tensor& tq = unpack(a[0]);
+    if (tq.dim() != 4 || tq.size(0) != B || tq.size(2) != Hq || tq.size(3) != D) return value_error("%s: xq must be [B, n_new, Hq, D]", fn);
+    const int64_t n_new = tq.size(1);
+    if (n_new <= 0) return value_error("%s: no tokens", fn);
+    for (int i : {1, 2}) {
+        const at::Tensor& t = unpack(a[i]);
+        if (t.dim() != 4 || t.size(0) != B || t.size(1) != n_new || t.size(2) != Hkv || t.size(3) != D)
+            return value_error("%s: xk and xv must be [B, n_new, Hkv, D]", fn);
+    }
+    if (numel(a[5]) != tq.numel()) return value_error("%s: q_out numel mismatch", fn);
+    if (a[3] != Py_None && (numel(a[3]) != D || numel(a[4]) != D)) return value_error("%s: gamma_q and gamma_k must have d_h elements", fn);
+    if (row0 + n_new > L_cap) return value_error("%s: %d + %d tokens exceed the capacity %d", fn, row0, int(n_new), L_cap);
+    const int64_t n_pos = unpack(a[9]).size(0);
+    if (a[13] == Py_None && pos0 + n_new > n_pos)
+        return value_error("%s: %d + %d tokens exceed the %d positions of the tables", fn, pos0, int(n_new), int(n_pos));
+    const double eps = PyFloat_AsDouble(a[22]);
+    if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+    const Call c(a[6]);
+    void *xq = ptr(a[0]), *xk = ptr(a[1]), *xv = ptr(a[2]), *qo = ptr(a[5]), *k = ptr(a[6]), *v = ptr(a[7]), *st = c.st();
+    float *gq = opt_ptr<float>(a[3]), *gk = opt_ptr<float>(a[4]), *cs = opt_ptr<float>(a[9]), *sn = opt_ptr<float>(a[10]);
+    int *ps = opt_ptr<int>(a[8]), *pos = opt_ptr<int>(a[13]), *rows = opt_ptr<int>(a[15]);
+    int rc;
+    {
+        const NoGil no_gil;
+        rc = b200attn_kv_append_rotary(xq, xk, xv, xd, qo, k, v, ps, gq, gk, cs, sn, int(n_pos), rp[0], rp[1], pos, pos0, rows, row0, B, int(n_new),
+                                       L_cap, Hq, Hkv, D, static_cast<float>(eps), st);
+    }
+    return finish(rc, fn);
+    B200ATTN_CATCH
+}
+
 // q, kprefix, vprefix, kcache, vcache, o, lse, B, G, P, L, Hq, Hkv, D, prefix_lens, lens, softmax_scale, P_cap, L_cap
 PyObject* decode_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* fn = "flash_attn_decode_shared";
@@ -927,16 +978,17 @@ PyObject* decode_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
     B200ATTN_CATCH
 }
 
-// q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale, L_cap, q_layout
+// q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale, L_cap, q_layout, new_lens
 PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* fn = "flash_attn_key_weights";
     B200ATTN_TRY
-    if (!arg_count(n, 13)) return nullptr;
+    if (!arg_count(n, 14)) return nullptr;
     const ScalarType bf = ScalarType::BFloat16, f = ScalarType::Float;
     for (int i = 0; i < 4; ++i)
         if (a[i] == Py_None) return value_error("%s: q, kcache, lse and weights are needed", fn);
     Items items;
     items.add(a[0], "q", bf), items.add(a[1], "kcache", bf), items.add(a[2], "lse", f), items.add(a[3], "weights", f);
+    items.add(a[13], "new_lens", ScalarType::Int);
     int d[6], L_cap;
     if (!items.check(fn) || !ints(a + 4, 6, d)) return nullptr;
     const int B = d[0], T = d[1], pos0 = d[2], Hq = d[3], Hkv = d[4], D = d[5];
@@ -950,13 +1002,15 @@ PyObject* key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (numel(a[1]) != nc * D) return value_error("%s: shape mismatch (cache)", fn);
     if (numel(a[2]) != rows) return value_error("%s: lse must be [B, Hq, T]", fn);
     if (numel(a[3]) != nc) return value_error("%s: weights must be [B, Hkv, L_cap]", fn);
+    if (a[13] != Py_None && numel(a[13]) != B) return value_error("%s: new_lens must be [B]", fn);
     float scale;
     if (!scale_of(a[10], &scale)) return nullptr;
     const Call c(a[0]);
     void *q = ptr(a[0]), *k = ptr(a[1]), *st = c.st();
     float *lse = opt_ptr<float>(a[2]), *w = opt_ptr<float>(a[3]);
+    const int* nl = opt_ptr<int>(a[13]);
     return finish(with_scratch(c, b200attn_key_weights_workspace_bytes(B, T, pos0, Hkv), [&](void* wp, size_t wn) {
-        return b200attn_key_weights(q, layout, k, lse, w, B, T, pos0, L_cap, Hq, Hkv, D, scale, wp, wn, st);
+        return b200attn_key_weights(q, layout, k, lse, w, nl, B, T, pos0, L_cap, Hq, Hkv, D, scale, wp, wn, st);
     }), fn);
     B200ATTN_CATCH
 }
@@ -987,11 +1041,9 @@ PyObject* kv_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
     float *w = opt_ptr<float>(a[2]), *wo = opt_ptr<float>(a[4]);
     int *p = opt_ptr<int>(a[3]), *po = opt_ptr<int>(a[5]);
     const int* ll = opt_ptr<int>(a[12]);
-    int rc;
-    {
-        const NoGil no_gil;
-        rc = b200attn_kv_evict(k, v, w, p, wo, po, ll, B, L, L_cap, Hkv, D, keep, recent, st);
-    }
+    const int rc = with_scratch(c, b200attn_kv_evict_workspace_bytes(B, L, Hkv, keep), [&](void* wp, size_t wn) {
+        return b200attn_kv_evict(k, v, w, p, wo, po, ll, B, L, L_cap, Hkv, D, keep, recent, wp, wn, st);
+    });
     return finish(rc, fn);
     B200ATTN_CATCH
 }
@@ -1002,7 +1054,8 @@ PyMethodDef methods[] = {
     B200ATTN_FAST(fwd),      B200ATTN_FAST(bwd),      B200ATTN_FAST(decode),      B200ATTN_FAST(kv_append),
     B200ATTN_FAST(kv_attend), B200ATTN_FAST(rope_fwd), B200ATTN_FAST(rope_bwd),    B200ATTN_FAST(rope_fwd_qk),
     B200ATTN_FAST(rope_bwd_qk), B200ATTN_FAST(rotary_fwd), B200ATTN_FAST(rotary_bwd), B200ATTN_FAST(rotary_table),
-    B200ATTN_FAST(decode_shared), B200ATTN_FAST(decode_weights), B200ATTN_FAST(key_weights), B200ATTN_FAST(kv_evict), {"release_scratch", release_scratch, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    B200ATTN_FAST(decode_shared), B200ATTN_FAST(decode_weights), B200ATTN_FAST(key_weights), B200ATTN_FAST(kv_evict),
+    B200ATTN_FAST(append_rotary), {"release_scratch", release_scratch, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kDecodeWeightsThreads) decode_weights_kernel(c
 // What bounds it: 128 x 128 exponentials a unit at 16 a clock, 1024 clocks, where the product takes 256 (D = 128).
 struct KeyWeightsParams {
     const float* lse;   // [B, Hq, T]
+    const int* rows;    // [B] or nullptr: of the T query rows those that count (a padded batch)
     float* w;           // [B, Hkv, L_cap]
     float* part;        // [item + CTA][group of warps][128]
     int* status;
@@ -315,7 +316,9 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int b = bh / p.Hkv;
             return p.lse + (size_t(b) * p.Hq + (bh - b * p.Hkv) * p.group) * p.T;
         };
+        auto count_of = [&](int bh) { return p.rows ? min(p.T, __ldg(p.rows + bh / p.Hkv)) : p.T; };
         const float* rows = rows_of(it.bh);
+        int T = count_of(it.bh);
         int in_item = u0 - it.start;
         float v[2][4];
         auto load = [&](float (&v)[4]) {  // of the unit at `in_item` of `it`, and on to the next
@@ -325,12 +328,12 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             for (int c = 0; c < 4; ++c) {
                 const int t = qt * p.tokens + t_col[c];
                 // 2^(x - inf) = 0
-                v[c] = lane + 32 * c < cols && t < p.T ? __ldg(rows + size_t(hc * p.heads + h_col[c]) * p.T + t) * -kLog2e : -INFINITY;
+                v[c] = lane + 32 * c < cols && t < T ? __ldg(rows + size_t(hc * p.heads + h_col[c]) * p.T + t) * -kLog2e : -INFINITY;
             }
             if (++in_item == it.units) {
                 const int bh = it.bh;
                 key_weights_next(p, it);
-                if (it.bh != bh) rows = rows_of(it.bh);
+                if (it.bh != bh && it.start < p.total) rows = rows_of(it.bh), T = count_of(it.bh);
                 in_item = 0;
             }
         };

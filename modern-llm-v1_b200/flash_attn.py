@@ -94,11 +94,13 @@ def flash_attn_decode_weights(q, kcache, vcache, o, lse, weights, B, L, Hq, Hkv,
     _lib.host().decode_weights(q, kcache, vcache, o, lse, weights, B, L, Hq, Hkv, D, lens, softmax_scale, L_cap)
 
 
-def flash_attn_key_weights(q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale=None, L_cap=None, q_layout="BHTD"):
+def flash_attn_key_weights(q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale=None, L_cap=None, q_layout="BHTD",
+                           new_lens=None):
     """The same sums over a chunk: weights[b, hk, key] += the probabilities that the T tokens in rows pos0 .. pos0 + T - 1 of the cache
     give the key, over the heads of the group and the tokens that see it.  q: [.., T, ..] in q_layout; lse [B, Hq, T], as the forward over
-    the cache has left it.  For a prompt's last tokens only, pass their q, lse and row."""
-    _lib.host().key_weights(q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale, L_cap, q_layout)
+    the cache has left it; new_lens: int32 [B] on the device, how many of the T rows of each sequence count (a padded batch), or None: all.
+    For a prompt's last tokens only, pass their q, lse and row."""
+    _lib.host().key_weights(q, kcache, lse, weights, B, T, pos0, Hq, Hkv, D, softmax_scale, L_cap, q_layout, new_lens)
 
 
 def device_status() -> int:

@@ -9,7 +9,16 @@ tokens and stores their k and v, `attend` runs attention for them (causal forwar
 or the split-KV decode kernel for one token), `advance` moves the length once every layer is done.
 The B sequences advance in lock step until `set_lengths` gives each its own length (a batch of
 prompts of different lengths); from then on `append` and `attend` take one token per sequence at the
-sequence's own position.  Like the reference's operators, the caller allocates every
+sequence's own position.
+
+For long contexts a cache can also
+  - rotate in other layouts (`pairs`, `rotary_dim`), with scaled frequencies (`scaling`, `factor`, `trained`) and without the
+    QK-norm (gammas None), see rotary.py;
+  - continue prompts that several of its sequences share (`prefix`: a KVCache that holds them; sequence b continues prompt
+    b // (B // prefix.B)): the prompts' keys and values are kept and read once, not once per sequence;
+  - keep the attention weight that each cached key has received and its position (`track_weights`), and cut itself down by it
+    (`evict`): rows and positions then part ways, `next_position` is what counts on.
+Like the reference's operators, the caller allocates every
 input and output; bad arguments raise ValueError, CUDA failures RuntimeError; there is no CPU or
 PyTorch fallback.
 """
@@ -19,6 +28,7 @@ import torch
 
 from . import _lib
 from .rope_norm import make_rope_cache
+from .rotary import make_rotary_cache
 
 
 def kv_evict(kcache, vcache, weights, positions, weights_out, positions_out, B, L, Hkv, D, keep, recent, lens=None, L_cap=None):
@@ -31,8 +41,13 @@ def kv_evict(kcache, vcache, weights, positions, weights_out, positions_out, B, 
 
 
 class KVCache:
+    # the reference's rotation, a cache of its own, no weights
+    _plain, prefix, track_weights = True, None, False
+    _shift, _pos, _evicted = 0, None, False
+
     def __init__(self, n_layers: int, B: int, Hq: int, Hkv: int, D: int, L_cap: int, device="cuda",
-                 rope_base: float = 10000.0, eps: float = 1e-5):
+                 rope_base: float = 10000.0, eps: float = 1e-5, *, rotary_dim=None, pairs="interleaved", scaling="none",
+                 factor: float = 1.0, trained=None, T_max=None, prefix=None, track_weights: bool = False):
         if min(n_layers, B, Hq, Hkv, D, L_cap) <= 0 or Hq % Hkv != 0:
             raise ValueError("KVCache: sizes must be positive and Hq a multiple of Hkv")
         if D not in (64, 128):
@@ -43,16 +58,89 @@ class KVCache:
         self.device = torch.device(device)
         self.k = torch.zeros((n_layers, B, Hkv, L_cap, D), dtype=torch.bfloat16, device=self.device)
         self.v = torch.zeros_like(self.k)
-        self.cos, self.sin = make_rope_cache(L_cap, D, rope_base, device=self.device)
+        self.prefix, self.track_weights = prefix, bool(track_weights)
+        own = (rotary_dim, pairs, scaling) != (None, "interleaved", "none")
+        if prefix is None:
+            self._rotary_setup(rope_base, rotary_dim, pairs, scaling, factor, trained, T_max, own)
+        else:
+            self._prefix_setup(prefix, own, T_max)
+        if self.track_weights:
+            if prefix is not None:
+                raise ValueError("KVCache: a cache that continues shared prompts keeps no weights")
+            shape = (B, Hkv, L_cap)
+            new = lambda: (torch.zeros(shape, device=self.device), torch.full(shape, -1, dtype=torch.int32, device=self.device))  # noqa: E731
+            pairs_ = [new() for _ in range(n_layers + 1)]  # one more than layers: what an eviction writes to
+            self.weights, self.positions = [w for w, _ in pairs_[:-1]], [p for _, p in pairs_[:-1]]
+            self._spare = pairs_[-1]
+        # the layers' own tensors, for the calls that take them
+        self._kl, self._vl = list(self.k.unbind(0)), list(self.v.unbind(0))
+        self._shift = 0  # a token's position minus its row, where all sequences agree
+        self._pos = None  # else: the next token's position per sequence [B] int32 on the device
+        self._evicted = False
         self.length = 0  # tokens held by every layer (the longest sequence's, once lengths differ)
         self.lengths = None  # per-sequence lengths [B] int32 on the device, once set_lengths was called
         self._lens_next = None  # lengths + 1: what the decode kernel reads while the newest token is being attended
         self._lengths_host = None
 
+    def _rotary_setup(self, base, rotary_dim, pairs, scaling, factor, trained, T_max, own):
+        R = self.D if rotary_dim is None else int(rotary_dim)
+        if pairs not in ("interleaved", "half"):
+            raise ValueError("KVCache: pairs must be interleaved or half")
+        if R <= 0 or R > self.D or R % 16 != 0:
+            raise ValueError("KVCache: rotary_dim must be a multiple of 16, at most d_h")
+        T = self.L_cap if T_max is None else int(T_max)
+        if T < self.L_cap:
+            raise ValueError("KVCache: T_max is less than the capacity")
+        self._R, self._pairs, self._scaled, self._base = R, _lib.PAIRS_HALF if pairs == "half" else _lib.PAIRS_INTERLEAVED, (scaling, factor, trained), base
+        self._reference = not own
+        self._plain = not own and not self.track_weights and T_max is None  # the reference's rotation, rows are positions
+        self.cos, self.sin = self._tables(T)
+
+    def _tables(self, T):
+        scaling, factor, trained = self._scaled
+        if self._reference:  # the reference's rotation has its values, of angles in 32 bits
+            return make_rope_cache(T, self.D, self._base, device=self.device)
+        return make_rotary_cache(T, self._R, self._base, scaling, factor, trained, device=self.device)
+
+    def _prefix_setup(self, prefix, own, T_max):
+        if own or T_max is not None:
+            raise ValueError("KVCache: a cache that continues prompts rotates as theirs does")
+        if (prefix.n_layers, prefix.Hq, prefix.Hkv, prefix.D) != (self.n_layers, self.Hq, self.Hkv, self.D) or prefix.prefix is not None:
+            raise ValueError("KVCache: prefix must be a cache of prompts with the same layers and heads")
+        if prefix.track_weights:
+            raise ValueError("KVCache: prefix must not keep weights")
+        if self.B % prefix.B != 0:
+            raise ValueError("KVCache: B must be a multiple of the number of prompts")
+        self._R, self._pairs, self._scaled, self._base, self._reference = prefix._R, prefix._pairs, prefix._scaled, prefix._base, prefix._reference
+        self._plain = False
+        self.cos, self.sin = self._tables(prefix.L_cap + self.L_cap)
+
     def reset(self) -> None:
         """Forgets every token (the buffers keep their bytes; rows >= length are never read)."""
         self.length = 0
         self.lengths = self._lens_next = self._lengths_host = None
+        self._shift, self._pos, self._evicted = 0, None, False
+        if self.track_weights:
+            for w, p in zip(self.weights, self.positions):
+                w.zero_()
+                p.fill_(-1)
+
+    def _place(self):
+        """(first position, positions or None, rows or None) of the next tokens; behind prompts of different lengths they are made when
+        the first token comes"""
+        if self.prefix is not None and self.length == 0 and self._pos is None:
+            if self.prefix.length == 0:
+                raise ValueError("KVCache: the prompts are empty")
+            self._shift = self.prefix.length
+            if self.prefix.lengths is not None:
+                self._pos = self.prefix.lengths.repeat_interleave(self.B // self.prefix.B)
+        return self.length + self._shift, self._pos, self.lengths
+
+    @property
+    def next_position(self):
+        """The position of the next token: an int, or int32 [B] on the device where the sequences differ."""
+        pos0, pos, rows = self._place()
+        return pos if pos is not None else pos0 if rows is None else rows + self._shift
 
     def set_lengths(self, lengths) -> None:
         """Gives every sequence its own length (e.g. after a padded prompt batch went through `append` /
@@ -61,6 +149,8 @@ class KVCache:
         host = [int(x) for x in lengths]
         if len(host) != self.B or min(host) < 0 or max(host) > self.L_cap:
             raise ValueError("KVCache.set_lengths: need B lengths in [0, L_cap]")
+        if self._evicted or self.prefix is not None:
+            raise ValueError("KVCache.set_lengths: not after an eviction, nor behind shared prompts")
         self._lengths_host = host
         self.length = max(host)
         self.lengths = torch.tensor(host, dtype=torch.int32, device=self.device)
@@ -70,15 +160,82 @@ class KVCache:
         """xq [B, n_new, Hq, D], xk / xv [B, n_new, Hkv, D] (the projection outputs, FP32 or BF16, all the
         same type) are the n_new tokens after the `length` cached ones.  Writes q_out [B, Hq, n_new, D] BF16
         (rotated, normalised, times gamma_q) and the tokens' rows of this layer's K (same chain with gamma_k)
-        and V (converted to BF16)."""
-        _lib.host().kv_append(self, layer, xq, xk, xv, gamma_q, gamma_k, q_out)
+        and V (converted to BF16).  Except in a cache with the reference's rotation and nothing else, gamma_q and gamma_k may both be
+        None: no norm."""
+        if self._plain:
+            _lib.host().kv_append(self, layer, xq, xk, xv, gamma_q, gamma_k, q_out)
+            return
+        self._layer_ok("append", layer)
+        pos0, pos, rows = self._place()
+        if rows is not None and pos is None:
+            pos = rows if self._shift == 0 else rows + self._shift
+        if rows is not None and xq.dim() == 4 and xq.shape[1] != 1:
+            raise ValueError("KVCache.append: one token per sequence once the lengths differ")
+        _lib.host().append_rotary(xq, xk, xv, gamma_q, gamma_k, q_out, self._kl[layer], self._vl[layer],
+                                  self.positions[layer] if self.track_weights else None, self.cos, self.sin, self._R, self._pairs, pos, pos0,
+                                  rows, self.length, self.B, self.L_cap, self.Hq, self.Hkv, self.D, self.eps)
 
-    def attend(self, layer: int, q, ctx, lse, n_new: int = 1, softmax_scale=None) -> None:
+    def _layer_ok(self, what, layer):
+        if not 0 <= layer < self.n_layers:
+            raise ValueError(f"KVCache.{what}: layer {layer} out of range")
+
+    def attend(self, layer: int, q, ctx, lse, n_new: int = 1, softmax_scale=None, new_lens=None) -> None:
         """Attention of the n_new appended tokens over the length + n_new cached ones.  q, ctx: [B, Hq, n_new, D]
         BF16; lse: [B, Hq, n_new] FP32 (may be None for n_new == 1).  n_new == 1 is the split-KV decode kernel;
         n_new > 1 is the causal forward of the new tokens over the cache: a whole prompt into an empty cache, or a
-        further chunk of it behind the tokens already cached (chunked prefill; lock-step sequences only)."""
-        _lib.host().kv_attend(self, layer, q, ctx, lse, n_new, softmax_scale)
+        further chunk of it behind the tokens already cached (chunked prefill; lock-step sequences only).
+        Behind shared prompts: one token, over the prompt and the sequence's own tokens.  With track_weights the keys' weights grow by
+        what these tokens give them; new_lens (int32 [B] on the device) says how many of the n_new tokens of each sequence are
+        tokens and not padding, where the prompts of a batch differ in length (`set_lengths` follows)."""
+        if new_lens is not None and (not self.track_weights or n_new == 1):
+            raise ValueError("KVCache.attend: new_lens is for several tokens at once, with track_weights")
+        if self.prefix is None and not self.track_weights:
+            _lib.host().kv_attend(self, layer, q, ctx, lse, n_new, softmax_scale)
+            return
+        self._layer_ok("attend", layer)
+        if n_new <= 0 or self.length + n_new > self.L_cap:
+            raise ValueError("KVCache.attend: n_new out of range")
+        h, k, v, L = _lib.host(), self._kl[layer], self._vl[layer], self.length + n_new
+        if self.prefix is not None:
+            if n_new != 1:
+                raise ValueError("KVCache.attend: one token per sequence behind shared prompts")
+            self._place()
+            p = self.prefix
+            h.decode_shared(q, p._kl[layer], p._vl[layer], k, v, ctx, lse, self.B, p.B, p.length, L, self.Hq, self.Hkv, self.D, p.lengths,
+                            self._lens_next, softmax_scale, p.L_cap, self.L_cap)
+        elif n_new == 1:
+            h.decode_weights(q, k, v, ctx, lse, self.weights[layer], self.B, L, self.Hq, self.Hkv, self.D, self._lens_next, softmax_scale,
+                             self.L_cap)
+        else:
+            h.kv_attend(self, layer, q, ctx, lse, n_new, softmax_scale)
+            h.key_weights(q, k, lse, self.weights[layer], self.B, n_new, self.length, self.Hq, self.Hkv, self.D, softmax_scale, self.L_cap, "BHTD",
+                          new_lens)
+
+    def evict(self, keep: int, recent: int) -> None:
+        """Cuts every layer down to at most `keep` rows per (sequence, KV head): the newest `recent` tokens and those of the largest
+        weight (csrc/kv_evict.cuh).  Between steps, after `advance`.  Later tokens go on at their positions."""
+        if not self.track_weights:
+            raise ValueError("KVCache.evict: the cache keeps no weights (track_weights)")
+        if keep <= 0 or not 0 <= recent <= keep:
+            raise ValueError("KVCache.evict: need 0 <= recent <= keep and keep > 0")
+        if self.length <= keep:
+            return
+        for i in range(self.n_layers):
+            w2, p2 = self._spare
+            _lib.host().kv_evict(self._kl[i], self._vl[i], self.weights[i], self.positions[i], w2, p2, self.B, self.length, self.Hkv, self.D, keep,
+                                 recent, self.lengths, self.L_cap)
+            self._spare = (self.weights[i], self.positions[i])
+            self.weights[i], self.positions[i] = w2, p2
+        self._evicted = True
+        if self.lengths is None:
+            self._shift += self.length - keep
+        else:
+            if self._pos is None:
+                self._pos = self.lengths + self._shift
+            self._lengths_host = [min(x, keep) for x in self._lengths_host]
+            self.lengths = self.lengths.clamp(max=keep)
+            self._lens_next = self.lengths + 1
+        self.length = keep
 
     def advance(self, n_new: int = 1) -> None:
         """Call once per step, after every layer has appended and attended."""
@@ -89,3 +246,5 @@ class KVCache:
             self._lengths_host = [x + n_new for x in self._lengths_host]
             self.lengths += n_new
             self._lens_next += n_new
+        if self._pos is not None:
+            self._pos += n_new

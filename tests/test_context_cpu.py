@@ -26,14 +26,14 @@ def test_c_abi_refuses_before_any_cuda_call(lib):
     assert w(ws=None) == w(n=64) == _lib.ERR_WORKSPACE
 
     c = lambda T=4, pos0=6, L_cap=10, Hkv=2, D=64, layout=0, lse=p, ws=p, n=1 << 30: lib.b200attn_key_weights(  # noqa: E731
-        p, layout, p, lse, p, 2, T, pos0, L_cap, 4, Hkv, D, 0.0, ws, n, None)
+        p, layout, p, lse, p, None, 2, T, pos0, L_cap, 4, Hkv, D, 0.0, ws, n, None)
     assert c(T=0) == c(pos0=-1) == c(pos0=7) == c(Hkv=3) == c(layout=2) == c(lse=None) == _lib.ERR_INVALID_ARG
     assert c(D=256) == _lib.ERR_UNSUPPORTED
     assert c(ws=None) == c(n=64) == _lib.ERR_WORKSPACE
 
     rows = 2 * 2 * 10 * 4  # bytes of an array of weights
     a = [p, p + rows, p + 2 * rows, p + 3 * rows]
-    e = lambda L=10, L_cap=10, D=64, keep=4, recent=2, k=p, a=a: lib.b200attn_kv_evict(k, p, *a, None, 2, L, L_cap, 2, D, keep, recent, None)  # noqa: E731
+    e = lambda L=10, L_cap=10, D=64, keep=4, recent=2, k=p, a=a, B=2: lib.b200attn_kv_evict(k, p, *a, None, B, L, L_cap, 2, D, keep, recent, None, 0, None)  # noqa: E731
     assert e(keep=0) == e(recent=-1) == e(recent=5) == e(L=0) == e(L_cap=9) == e(k=None) == _lib.ERR_INVALID_ARG
     assert e(D=80) == _lib.ERR_UNSUPPORTED
     assert e(k=p + 2) == _lib.ERR_ALIGNMENT
@@ -41,6 +41,10 @@ def test_c_abi_refuses_before_any_cuda_call(lib):
         b = list(a)
         b[j] = b[i] + 4
         assert e(a=b) == _lib.ERR_INVALID_ARG, (i, j)
+    far = [p + (i << 20) for i in range(4)]
+    assert e(a=far, B=100) == _lib.ERR_WORKSPACE  # 200 (batch, head) pairs: their moves are listed
+    assert lib.b200attn_kv_evict_workspace_bytes(100, 10, 2, 4) == 200 * (4 * 8 + 4)
+    assert lib.b200attn_kv_evict_workspace_bytes(2, 10, 2, 4) == lib.b200attn_kv_evict_workspace_bytes(100, 10, 2, 10) == 0
 
 
 def test_python_refuses():
@@ -64,3 +68,32 @@ def test_python_refuses():
         m.kv_evict(k, k, w, p.long(), w, p, 4, 10, 2, 64, 5, 1)
     with pytest.raises(ValueError, match="must be CUDA"):
         m.kv_evict(k, k, w, p, w, p, 4, 10, 2, 64, 5, 1)
+
+
+def test_kvcache_refuses():
+    import modern_llm_v1_b200 as m
+
+    new = lambda *a, **k: m.KVCache(*(a or (1, 4, 4, 2, 64, 16)), device="cpu", **k)  # noqa: E731
+    for kw, what in ((dict(pairs="other"), "pairs must be"), (dict(rotary_dim=24), "multiple of 16"), (dict(rotary_dim=128), "at most d_h"),
+                     (dict(T_max=8), "T_max is less")):
+        with pytest.raises(ValueError, match=what):
+            new(**kw)
+    prompts = new(1, 2, 4, 2, 64, 8)
+    for a, kw, what in (((1, 3, 4, 2, 64, 8), {}, "multiple of the number"), ((2, 2, 4, 2, 64, 8), {}, "same layers"), ((1, 2, 4, 2, 64, 8), dict(T_max=64), "as theirs does"),
+                        ((1, 2, 4, 2, 64, 8), dict(pairs="half"), "as theirs does"), ((1, 2, 4, 2, 64, 8), dict(track_weights=True), "keeps no weights")):
+        with pytest.raises(ValueError, match=what):
+            new(*a, prefix=prompts, **kw)
+    c = new(1, 4, 4, 2, 64, 8, prefix=prompts)
+    with pytest.raises(ValueError, match="prompts must be|same layers"):
+        new(1, 4, 4, 2, 64, 8, prefix=c)
+    with pytest.raises(ValueError, match="keeps no weights"):
+        c.evict(4, 1)
+    with pytest.raises(ValueError, match="nor behind shared"):
+        c.set_lengths([1, 1, 1, 1])
+    w = new(track_weights=True)
+    for keep, recent in ((0, 0), (4, 5), (4, -1)):
+        with pytest.raises(ValueError, match="recent <= keep"):
+            w.evict(keep, recent)
+    w.evict(4, 1)  # nothing to do
+    with pytest.raises(ValueError, match="new_lens"):
+        w.attend(0, None, None, None, 1, new_lens=torch.ones(4))
