@@ -34,6 +34,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ptx.cuh"
 
@@ -422,45 +423,49 @@ __device__ __forceinline__ int decode_count(unsigned long long* word, unsigned l
     return int(atomicAdd(word, 1ull) - tag) + 1;
 }
 
-// W output elements (columns d .. d + W - 1 of head j of the group) joined with the prompt's partial results, in the order of the
-// splits; false: a kernel has failed and nothing may be written.  This is the first look at what the kernel in front, which computes
-// them, has written: all else this kernel reads was there before that one began (see grid_dep_launch in attn_prefix.cuh), so its loads
-// run beside it.  (The chain is two round trips through L2 whatever the number of splits up to eight.)
+// Where the prompt's partial results of head j of the group (of sequence b, KV head hk) lie: its row in the first split's slot
+__device__ __forceinline__ size_t decode_prefix_row(const DecodePrefix& x, int b, int hk, int j, int* row) {
+    const int prompt = int(fastdiv(b, x.div_n)), seq = b - prompt * int(x.div_n.d);
+    const int chunk = int(fastdiv(j, x.div_heads)), tile = int(fastdiv(seq, x.div_seqs));
+    *row = (seq - tile * int(x.div_seqs.d)) * int(x.div_heads.d) + j - chunk * int(x.div_heads.d);
+    return (size_t((prompt * x.Hkv + hk) * x.n_chunks + chunk) * x.tiles + tile) * x.splits;
+}
+// W output elements (columns d .. d + W - 1 of head j of the group) joined with the prompt's partial results, in the order of the splits;
+// false: a kernel has failed and nothing may be written.  Behind grid_dep_wait(): this is the first look at what the kernel in front,
+// which computes them, has written.  All else this kernel reads was there before that one began (see grid_dep_launch in attn_prefix.cuh),
+// so its loads run beside it.  Eight splits' loads are issued together; splits that are not there read the last one's.
 template <int D, int W>
 __device__ __forceinline__ bool decode_add_prefix(const DecodeParams& p, int b, int hk, int j, int d, float (&a)[W], float& m, float& l) {
     const DecodePrefix& x = p.prefix;
-    grid_dep_wait();
     const int status = *reinterpret_cast<volatile int*>(p.status);
-    const int prompt = int(fastdiv(b, x.div_n)), seq = b - prompt * int(x.div_n.d);
-    const int chunk = int(fastdiv(j, x.div_heads)), tile = int(fastdiv(seq, x.div_seqs));
-    const int row = (seq - tile * int(x.div_seqs.d)) * int(x.div_heads.d) + j - chunk * int(x.div_heads.d);
-    const size_t slot0 = (size_t((prompt * x.Hkv + hk) * x.n_chunks + chunk) * x.tiles + tile) * x.splits;
+    int row;
+    const size_t slot0 = decode_prefix_row(x, b, hk, j, &row);
     const float* o = x.o + (slot0 * (D / 4) + d / 4) * 512 + row * 4 + (d & 3);
     const float2* ml = x.ml + slot0 * 128 + row;
     constexpr int N = 8;
+#pragma unroll 1
     for (int s0 = 0; s0 < x.splits; s0 += N) {
         float2 pml[N];
         float po[N][W];
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            pml[k] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-            for (int e = 0; e < W; ++e) po[k][e] = 0.f;
-            if (s0 + k < x.splits) {
-                pml[k] = __ldcg(ml + (s0 + k) * 128);
-                const float* const at = o + size_t(s0 + k) * (D * 128);
-                if constexpr (W == 4) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(at));
-                    po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
-                } else {
-                    const float2 v = __ldcg(reinterpret_cast<const float2*>(at));
-                    po[k][0] = v.x, po[k][1] = v.y;
-                }
+            const int s = min(s0 + k, x.splits - 1);
+            pml[k] = __ldcg(ml + s * 128);
+            const float* const at = o + size_t(s) * (D * 128);
+            if constexpr (W == 4) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(at));
+                po[k][0] = v.x, po[k][1] = v.y, po[k][2] = v.z, po[k][3] = v.w;
+            } else {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(at));
+                po[k][0] = v.x, po[k][1] = v.y;
             }
         }
         float mn = m;
 #pragma unroll
-        for (int k = 0; k < N; ++k) mn = fmaxf(mn, pml[k].x);
+        for (int k = 0; k < N; ++k) {
+            if (s0 + k >= x.splits) pml[k] = make_float2(-INFINITY, 0.f);
+            mn = fmaxf(mn, pml[k].x);
+        }
         const float fa = m == -INFINITY ? 1.f : ex2_approx((m - mn) * p.scale_log2);  // (m = -inf: no score above it, l is 0 or NaN)
         l *= fa;
 #pragma unroll
@@ -468,11 +473,11 @@ __device__ __forceinline__ bool decode_add_prefix(const DecodeParams& p, int b, 
         m = mn;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            if (pml[k].x == -INFINITY && pml[k].y == 0.f) continue;  // no keys: nothing else was written
+            const bool any = !(pml[k].x == -INFINITY && pml[k].y == 0.f);  // no keys: nothing else was written
             const float f = pml[k].x == -INFINITY ? 1.f : ex2_approx((pml[k].x - mn) * p.scale_log2);
             l += f * pml[k].y;
 #pragma unroll
-            for (int e = 0; e < W; ++e) a[e] += f * po[k][e];
+            for (int e = 0; e < W; ++e) a[e] += any ? f * po[k][e] : 0.f;
         }
     }
     return status == 0;
@@ -599,6 +604,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 return;
             }
             if (MODE == kDecodeShared) {
+                grid_dep_wait();
                 float a[2] = {a0, a1};
                 if (!decode_add_prefix<D, 2>(p, b, hk, j0 + g, d, a, m, l)) return;
                 a0 = a[0], a1 = a[1];
@@ -667,6 +673,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     const bool failed = *fail_flag != 0;
     bool ok = true;
     const int rank = p.cluster > 1 ? int(blockIdx.x) % p.cluster : 0;
+    const DecodeWalk w_first = w;  // (kDecodeShared)
     bool sent = false, last_mine = false;
     int j = 0;  // tiles before this piece (ring position)
     for (int n = 0; w.t < w.t_end; ++n) {
@@ -891,7 +898,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if constexpr (MODE == kDecodeShared) {
         if (p.prefix.own_o && ok && !failed) {  // the units that this CTA has finished
             named_bar_sync(1, 128);
-            for (w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane); w.t < w.t_end;) {
+            grid_dep_wait();
+            for (w = w_first; w.t < w.t_end;) {
                 const int tiles = decode_piece(w);
                 if (tiles == w.n_tiles || (w.t + tiles == w.t_end && last_mine)) decode_join_unit<D>(p, w, tid);
                 decode_walk_next<KEYS>(p, w, tiles);

@@ -12,15 +12,18 @@
 // single online softmax cannot do is keep up: product, scores out of tensor memory, maximum, exponentials, P back and the next product
 // are a chain of some 2800 clocks (D = 128), in which an SM's share of HBM brings 64 KB, the tile.  So a CTA runs two of them, each with S
 // and O of its own, and one's chain passes under the other's exponentials (1024 clocks a tile and 128 rows):
-//   ROWS2 = false  one tile of rows, key tiles in turn (the two results are joined through shared memory at the end)
+//   ROWS2 = false  one tile of rows, key tiles in turn (the two results are joined through shared memory at the end).  Up to 64 rows the
+//                  second softmax has them in lanes 64 .. 127, so that each has two of the SM's four schedulers for itself
 //   ROWS2 = true   two tiles of rows, every K and V tile used twice (more than 128 rows; further ones read the prompt through L2)
 // P goes over S's columns once S is in registers, which leaves room for 128 keys and two softmaxes at both head dimensions: with tiles of
 // 64 keys a step of Q K^T, both operands in shared memory, takes the same 64 clocks for half the keys (B=64 P=16384 16/4 D=128, this
 // kernel: 21.5 -> XX us).
 //
-// Roles (320 threads): warps 0-3 and 4-7 softmax, thread = row, as in attn_fwd.cuh (rescaling only where the maximum grew by 2^8); warps
-// that have no row are not waited for and leave.  Warp 8 loads: a ring of K and V tiles in the order in which the products read them.
-// Warp 9 issues the products.  TMEM (512 columns), per softmax: S 128 with P over its first 64, O D.
+// Roles: warps 0 .. 8 H - 1 softmax, the first half of them the one, the second the other; thread = row (ROWS2, H = 1), or row and half of
+// the tile's keys (H = 2: two warps share a row's maximum through shared memory); rescaling only where the maximum grew by 2^8 as in
+// attn_fwd.cuh; warps that have no row are not waited for and leave.  Then a warp that loads, a ring of K and V tiles in the order in
+// which the products read them, and one that issues the products.  TMEM (512 columns), per softmax: S 128 with P over its scores, O D.
+// XX
 #pragma once
 
 #include "ptx.cuh"
@@ -48,13 +51,13 @@ struct PrefixCfg {
     static constexpr int kBoxBytes = kPrefixKeys * 128;  // [keys][64] BF16
     static constexpr int kBoxes = D / 64;
     static constexpr int kStages = D == 64 ? 8 : 4;      // 128 KB
-    static constexpr int kQBoxBytes = 128 * 128, kQTiles = ROWS2 ? 2 : 1;
+    static constexpr int kQBoxBytes = 128 * 128, kQTiles = 2;  // (of the same rows, 64 lanes apart, or of two tiles)
+    static constexpr int kHalves = ROWS2 ? 1 : 2, kThreads = (8 * kHalves + 2) * 32;
     static constexpr int kAhead = ROWS2 ? 1 : 2;       // K tiles loaded ahead of V of tile 0
-    static constexpr int kSmemBytes = kQTiles * kBoxes * kQBoxBytes + kStages * kTileBytes + 1024 + 256;
+    static constexpr int kSmemBytes = kQTiles * kBoxes * kQBoxBytes + kStages * kTileBytes + 6144 + 256;
     static_assert(kStages * kTileBytes >= 128 * D * 4, "one softmax's O goes to the other through the ring");
     static constexpr int kColS = 0, kColO = 128;       // + 256 for the second softmax
 };
-constexpr int kPrefixThreads = 320;
 constexpr float kPrefixRescaleLog2 = 8.0f;  // P <= 2^8: its rounding to BF16 (the second product's operand) is relative
 
 // Place of a load: first `ahead` K tiles, then V of tile j and K of tile j + ahead in turn, the last V tiles at the end
@@ -72,15 +75,17 @@ __host__ __device__ __forceinline__ bool prefix_load_at(int i, int n, int ahead,
 }
 
 template <int D, bool ROWS2>
-__global__ void __launch_bounds__(kPrefixThreads, 1)
+__global__ void __launch_bounds__(PrefixCfg<D, ROWS2>::kThreads, 1)
 attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const PrefixParams p) {
     using Cfg = PrefixCfg<D, ROWS2>;
-    constexpr int KEYS = kPrefixKeys, NST = Cfg::kStages, A = Cfg::kAhead;
+    constexpr int KEYS = kPrefixKeys, NST = Cfg::kStages, A = Cfg::kAhead, H = Cfg::kHalves, PRODUCER = 8 * H, MMA = 8 * H + 1;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;
     uint8_t* sRing = sQ + Cfg::kQTiles * Cfg::kBoxes * Cfg::kQBoxBytes;
-    float2* sMl = reinterpret_cast<float2*>(sRing + NST * Cfg::kTileBytes);  // [128]
+    float* sMax = reinterpret_cast<float*>(sRing + NST * Cfg::kTileBytes);  // [softmax][tile & 1][half][128] maxima of the rows' halves
+    float* sL = sMax + 1024;                                                // [softmax][128] at the end, l of the second halves
+    float2* sMl = reinterpret_cast<float2*>(sL + 256);                      // [128] at the end, the second softmax's (m, l)
     uint64_t* bars = reinterpret_cast<uint64_t*>(sMl + 128);
     uint64_t* bar_full = bars;              // [NST]                                          (phase: load / NST)
     uint64_t* bar_free = bars + NST;        // [NST] the products that read it are done
@@ -102,8 +107,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const int qt0 = ROWS2 ? 2 * block : block;
     const int rows0 = rows_of(qt0), rows1 = ROWS2 ? rows_of(qt0 + 1) : rows0;  // of the two softmaxes
     const bool two = rows1 > 0;
+    const int lane1 = !ROWS2 && rows0 <= 64 ? 64 : 0;  // tensor memory lane of the second softmax's first row
 
-    if (warp == 8 && lane == 0) {
+    if (warp == PRODUCER && lane == 0) {
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
@@ -113,7 +119,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         mbar_init(bar_q, 1);
         for (int x = 0; x < 2; ++x) {
-            const int n = max(32, ((x ? rows1 : rows0) + 31) / 32 * 32);
+            const int n = max(1, ((x ? rows1 : rows0) + 31) / 32) * 32 * H;
             mbar_init(&bar_s_full[x], 1);
             mbar_init(&bar_p_full[x], n);
             mbar_init(&bar_o[x], 1);
@@ -121,7 +127,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         fence_mbar_init();
         *abort_flag = 0;
     }
-    if (warp == 9) {
+    if (warp == MMA) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -144,7 +150,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 
     if (*abort_flag != 0) {
         // an earlier kernel has failed: nothing is loaded, nothing is written
-    } else if (warp == 8) {
+    } else if (warp == PRODUCER) {
         // ------------------------------------------------------------------ producer
         for (int i = 0; i < 2 * n_tiles; ++i) {
             int j;
@@ -152,11 +158,11 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (i >= NST && !mbar_wait_warp(&bar_free[i % NST], uint32_t(i / NST - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_FREE)) break;
             if (elect_one()) {
                 if (i == 0) {
-                    mbar_arrive_expect_tx(bar_q, Cfg::kQTiles * Cfg::kBoxes * p.heads * p.seqs * 128);
-#pragma unroll
-                    for (int e = 0; e < Cfg::kQTiles * Cfg::kBoxes; ++e)
-                        tma_load_4d(sQ + e * Cfg::kQBoxBytes, &tmQ, bar_q, (e % Cfg::kBoxes) * 64, hk * p.group + chunk * p.heads,
-                                    prompt * p.n + (qt0 + e / Cfg::kBoxes) * p.seqs, 0);
+                    const int q_tiles = ROWS2 || lane1 ? 2 : 1;
+                    mbar_arrive_expect_tx(bar_q, q_tiles * Cfg::kBoxes * p.heads * p.seqs * 128);
+                    for (int e = 0; e < q_tiles * Cfg::kBoxes; ++e)
+                        tma_load_4d(sQ + e * Cfg::kQBoxBytes + (e >= Cfg::kBoxes ? lane1 * 128 : 0), &tmQ, bar_q, (e % Cfg::kBoxes) * 64,
+                                    hk * p.group + chunk * p.heads, prompt * p.n + (qt0 + (ROWS2 ? e / Cfg::kBoxes : 0)) * p.seqs, 0);
                 }
                 uint8_t* dst = sRing + (i % NST) * Cfg::kTileBytes;
                 mbar_arrive_expect_tx(&bar_full[i % NST], Cfg::kTileBytes);
@@ -166,7 +172,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             __syncwarp();
         }
-    } else if (warp == 9) {
+    } else if (warp == MMA) {
         // ------------------------------------------------------------------ products
         constexpr uint32_t idesc_s = make_idesc_bf16(128, KEYS, 0, 0), idesc_o = make_idesc_bf16(128, D, 0, 1);
         const uint32_t ring = smem_u32(sRing);
@@ -179,7 +185,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             ok = mbar_wait_warp(&bar_full[at % NST], uint32_t(at / NST) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
             if (!ok) return;
             tc_fence_after_sync();
-            const uint64_t q_desc = make_sdesc_sw128(smem_u32(sQ + (ROWS2 ? x : 0) * Cfg::kBoxes * Cfg::kQBoxBytes), 16, 1024);
+            const uint64_t q_desc = make_sdesc_sw128(smem_u32(sQ + (ROWS2 || lane1 ? x : 0) * Cfg::kBoxes * Cfg::kQBoxBytes), 16, 1024);
             const uint64_t k_desc = make_sdesc_sw128(ring + (at % NST) * Cfg::kTileBytes, 16, 1024);
             if (elect_one()) {
 #pragma unroll
@@ -202,7 +208,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < KEYS / 16; ++ks)
-                    umma_ts(tmem + x * 256 + Cfg::kColO, tmem + x * 256 + Cfg::kColS + ks * 8, v_desc + uint64_t(ks * 128), idesc_o, (i > 1) || (ks > 0));
+                    umma_ts(tmem + x * 256 + Cfg::kColO, tmem + x * 256 + Cfg::kColS + ks * 8 + (H == 2 ? (ks / (KEYS / 32)) * (KEYS / 4) : 0), v_desc + uint64_t(ks * 128), idesc_o, (i > 1) || (ks > 0));
                 if (i + 2 >= n_units) umma_commit(&bar_o[x]);
                 if (last_use(i)) umma_commit(&bar_free[at % NST]);
             }
@@ -213,49 +219,87 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         for (int x = 0; ok && x < 2; ++x)
             if (n_units > x && (two || x == 0)) ok = mbar_wait_warp(&bar_o[x], 0, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
     } else {
-        // ------------------------------------------------------------------ softmax, thread = row
-        const int x = warp >> 2, row = tid & 127, rows = x ? rows1 : rows0, n_warps = (rows + 31) / 32;
-        if ((warp & 3) < n_warps) {
+        // ------------------------------------------------------------------ softmax, thread = row and half of the keys
+        const int x = warp / (4 * H), half = H == 2 ? (warp >> 2) & 1 : 0, row = (tid & 127) - (x ? lane1 : 0), rows = x ? rows1 : rows0, n_warps = (rows + 31) / 32;
+        if (row >= 0 && row < 32 * n_warps) {
+            constexpr int COLS = KEYS / H;
             const uint32_t lanes = (uint32_t((warp & 3) * 32) << 16) + x * 256;
-            const uint32_t t_s = tmem + lanes + Cfg::kColS, t_p = t_s, t_o = tmem + lanes + Cfg::kColO;
+            const uint32_t t_s = tmem + lanes + Cfg::kColS + half * COLS, t_p = t_s,  // (each half's P over its own scores)
+                           t_o = tmem + lanes + Cfg::kColO + half * (D / H);
             const int mine = (n_units - x + 1) / 2;  // units of this softmax
+            const int pair = 1 + x * 4 + (warp & 3);  // named barrier of the two warps that share rows
             bool ok = true;
             float m_ref = -INFINITY, l = 0.f;
             for (int e = 0; e < mine; ++e) {
                 const int j = ROWS2 ? e : 2 * e + x;
-                ok = mbar_wait_warp(&bar_s_full[x], uint32_t(e) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
-                if (!ok) break;
+                if (ok) ok = mbar_wait_warp(&bar_s_full[x], uint32_t(e) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
+                if (H == 1 && !ok) break;
                 tc_fence_after_sync();
-                uint32_t sr[KEYS];
-#pragma unroll
-                for (int c = 0; c < KEYS; c += 32) tmem_ld_x32(t_s + c, &sr[c]);
-                tmem_wait_ld();
-                const int left = len - (j0 + j) * KEYS;  // keys of this tile
-                if (left < KEYS) {
-#pragma unroll
-                    for (int c = 0; c < KEYS; ++c)
-                        if (c >= left) sr[c] = 0xff800000u;  // -inf
-                    if (p.lens) {
-                        // Rows of the prompt's buffer beyond its length may hold anything: 0 * NaN would be NaN.  (With two tiles of rows
-                        // both softmaxes clear them, each in front of its own product.)
-                        const int at = prefix_v_at(j, n_tiles, A);
-                        ok = mbar_wait_warp(&bar_full[at % NST], uint32_t(at / NST) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
-                        if (!ok) break;
-                        uint8_t* v = sRing + (at % NST) * Cfg::kTileBytes;
-                        for (int i = left * 8 * Cfg::kBoxes + row; i < KEYS * 8 * Cfg::kBoxes; i += 32 * n_warps) {
-                            const int r = i / (8 * Cfg::kBoxes), part = i % (8 * Cfg::kBoxes);
-                            *reinterpret_cast<uint4*>(v + (part / 8) * Cfg::kBoxBytes + r * 128 + (part % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        fence_proxy_async_smem();  // (in front of the arrival on bar_p_full, upon which the product reads them)
-                    }
-                }
+                const int left = len - (j0 + j) * KEYS - half * COLS;  // keys of this half tile
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // visit(CH columns, the first of which is c) for the thread's scores.  H = 1: they stay in registers from the first pass to the
+                // second (read twice, 37 us instead of 31: tensor memory is busy with the products); H = 2: there is no room for them, and time
+                constexpr int CH = H == 1 ? 32 : 16;
+                uint32_t v[H == 1 ? COLS / CH : 2][CH];
+                auto mask = [&](int c, uint32_t (&now)[CH]) {
+                    if (left < COLS) {
 #pragma unroll
-                for (int c = 0; c < KEYS; c += 8)
+                        for (int k = 0; k < CH; ++k)
+                            if (c + k >= left) now[k] = 0xff800000u;  // -inf
+                    }
+                };
+                auto columns = [&](bool first, auto visit) {
+                    if constexpr (H == 1) {
+                        if (first) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mx[k] = fmaxf(mx[k], fmaxf(__uint_as_float(sr[c + 2 * k]), __uint_as_float(sr[c + 2 * k + 1])));
-                const float m_new = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m_ref);
+                            for (int c = 0; c < COLS; c += CH) tmem_ld_x32(t_s + c, v[c / CH]);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int c = 0; c < COLS; c += CH) mask(c, v[c / CH]);
+                        }
+#pragma unroll
+                        for (int c = 0; c < COLS; c += CH) visit(c, v[c / CH]);
+                    } else {
+                        tmem_ld_x16(t_s, v[0]);
+#pragma unroll
+                        for (int c = 0; c < COLS; c += CH) {
+                            tmem_wait_ld();
+                            if (c + CH < COLS) tmem_ld_x16(t_s + c + CH, v[(c / CH + 1) & 1]);  // (on its way meanwhile)
+                            mask(c, v[(c / CH) & 1]);
+                            visit(c, v[(c / CH) & 1]);
+                        }
+                    }
+                };
+                if (H == 1 || ok)
+                    columns(true, [&](int, uint32_t (&sr)[CH]) {
+#pragma unroll
+                        for (int k = 0; k < CH; k += 4)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+                                mx[(k / 4 % 2) * 2 + q] = fmaxf(mx[(k / 4 % 2) * 2 + q], fmaxf(__uint_as_float(sr[k + 2 * q]), __uint_as_float(sr[k + 2 * q + 1])));
+                    });
+                // The other half's maximum.  (The place was last read two tiles ago, in front of the barrier of the tile between.)
+                const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                float* const s_max = sMax + (x * 2 + (e & 1)) * 256 + (tid & 127);
+                if (H == 2) {
+                    s_max[half * 128] = m_half;
+                    named_bar_sync(pair, 64);
+                }
+                if (H == 2 && !ok) continue;  // (a warp that has given up still meets the other at the barriers)
+                if (p.lens && len - (j0 + j) * KEYS < KEYS) {
+                    // Rows of the prompt's buffer beyond its length may hold anything: 0 * NaN would be NaN.  (With two tiles of rows
+                    // both softmaxes clear them, each in front of its own product.)
+                    const int at = prefix_v_at(j, n_tiles, A), first = len - (j0 + j) * KEYS;
+                    ok = mbar_wait_warp(&bar_full[at % NST], uint32_t(at / NST) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
+                    if (!ok) continue;
+                    uint8_t* v = sRing + (at % NST) * Cfg::kTileBytes;
+                    for (int i = first * 8 * Cfg::kBoxes + row * H + half; i < KEYS * 8 * Cfg::kBoxes; i += 32 * H * n_warps) {
+                        const int r = i / (8 * Cfg::kBoxes), part = i % (8 * Cfg::kBoxes);
+                        *reinterpret_cast<uint4*>(v + (part / 8) * Cfg::kBoxBytes + r * 128 + (part % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async_smem();  // (in front of the arrival on bar_p_full, upon which the product reads them)
+                }
+                const float m_new = fmaxf(H == 2 ? fmaxf(m_half, s_max[128 - half * 128]) : m_half, m_ref);
                 float alpha = 1.f;
                 if ((m_new - m_ref) * p.scale_log2 > kPrefixRescaleLog2) {  // also true for m_ref == -inf
                     alpha = ex2_approx((m_ref - m_new) * p.scale_log2);
@@ -265,26 +309,33 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), neg2 = pack_f32x2(neg_m, neg_m);
                 uint64_t sum2[2] = {0ull, 0ull};
                 // (P V of the tile before, which adds to O, is complete: it lies in front of this S in the pipe)
+                columns(false, [&](int c, uint32_t (&sr)[CH]) {
+                    uint32_t pk[CH / 2];
 #pragma unroll
-                for (int c = 0; c < KEYS / 32; ++c) {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
+                    for (int i = 0; i < CH / 2; ++i) {
+                        const uint64_t a = fma_f32x2(pack_f32x2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), scale2, neg2);
                         float a0, a1;
-                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[c * 32 + 2 * i]), __uint_as_float(sr[c * 32 + 2 * i + 1])), scale2, neg2), a0, a1);
-                        a0 = ex2_approx(a0);
-                        a1 = ex2_approx(a1);
-                        sum2[i & 1] = add_f32x2(sum2[i & 1], pack_f32x2(a0, a1));
+                        if (H == 2 && i % 4 == 3) {  // a quarter of them on the FMA pipes
+                            const uint64_t e2 = exp2_fma_f32x2(a);
+                            sum2[i & 1] = add_f32x2(sum2[i & 1], e2);
+                            unpack_f32x2(e2, a0, a1);
+                        } else {
+                            unpack_f32x2(a, a0, a1);
+                            a0 = ex2_approx(a0);
+                            a1 = ex2_approx(a1);
+                            sum2[i & 1] = add_f32x2(sum2[i & 1], pack_f32x2(a0, a1));
+                        }
                         pk[i] = pack_bf16x2(a0, a1);
                     }
-                    tmem_st_x16(t_p + c * 16, pk);
-                }
+                    if constexpr (CH == 32) tmem_st_x16(t_p + c / 2, pk);
+                    else tmem_st_x8(t_p + c / 2, pk);
+                });
                 float s0, s1;
                 unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
                 l = l * alpha + (s0 + s1);
                 if (e > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll 1
+                    for (int c = 0; c < D / (32 * H); ++c) {
                         uint32_t orr[32];
                         tmem_ld_x32(t_o + c * 32, orr);
                         tmem_wait_ld();
@@ -299,18 +350,24 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             if (ok && mine > 0) ok = mbar_wait_warp(&bar_o[x], 0, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
             tc_fence_after_sync();
-            // ---- O, m, l out.  Columns 4 c .. 4 c + 3 of all rows lie together: a warp's stores are whole lines.
+            // ---- O, m, l out: the halves' sums first.  Columns 4 c .. 4 c + 3 of all rows lie together: a warp's stores are whole lines.
+            float* const s_l = sL + x * 128 + (tid & 127);
+            if (H == 2) {
+                if (half == 1) *s_l = l;
+                named_bar_sync(pair, 64);
+                if (half == 0) l += *s_l;
+            }
             const int qt = qt0 + (ROWS2 ? x : 0);
             const size_t slot = (size_t(uc) * p.tiles + qt) * p.splits + split;
-            float4* const out = reinterpret_cast<float4*>(p.o) + slot * (D / 4) * 128 + row;
-            float4* const other = reinterpret_cast<float4*>(sRing) + row;  // the second softmax's O, [D / 4][128]
+            const int c0 = half * (D / 4 / H);  // first 16-byte column
+            float4* const out = reinterpret_cast<float4*>(p.o) + (slot * (D / 4) + c0) * 128 + row;
+            float4* const other = reinterpret_cast<float4*>(sRing) + c0 * 128 + row;  // the second softmax's O, [D / 4][128]
             const bool join = !ROWS2 && n_tiles > 1;
+            const int all_threads = 64 * H * n_warps;
             if (join && x == 1) {
-                // (the ring's last tiles have been read: the last P V of both softmaxes is waited for below in front of the reads, here
-                // of this one's, and of the other's by the barrier)
-                named_bar_sync(1, 64 * n_warps);
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
+                named_bar_sync(9, all_threads);  // both softmaxes' last products are done: nothing reads the ring; the maxima are read
+#pragma unroll 1
+                for (int c = 0; c < D / (32 * H); ++c) {
                     uint32_t v[32];
                     tmem_ld_x32(t_o + c * 32, v);
                     tmem_wait_ld();
@@ -319,13 +376,13 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         other[(c * 8 + i) * 128] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]),
                                                                __uint_as_float(v[4 * i + 3]));
                 }
-                sMl[row] = make_float2(m_ref, l);
-                named_bar_sync(1, 64 * n_warps);
+                if (half == 0) sMl[row] = make_float2(m_ref, l);
+                named_bar_sync(9, all_threads);
             } else if (ROWS2 || x == 0) {
                 float f0 = 1.f, f1 = 0.f;
                 if (join) {
-                    named_bar_sync(1, 64 * n_warps);  // both softmaxes' last products are done
-                    named_bar_sync(1, 64 * n_warps);  // the other's results are there
+                    named_bar_sync(9, all_threads);
+                    named_bar_sync(9, all_threads);  // the other's results are there
                     const float2 b = sMl[row];
                     const float m = fmaxf(m_ref, b.x);
                     f0 = m_ref == -INFINITY ? 1.f : ex2_approx((m_ref - m) * p.scale_log2);  // (-inf: l and O are 0, or NaN)
@@ -335,8 +392,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
                 ok = ok && *abort_flag == 0;
                 if (mine > 0) {
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll 1
+                    for (int c = 0; c < D / (32 * H); ++c) {
                         uint32_t v[32];
                         tmem_ld_x32(t_o + c * 32, v);
                         tmem_wait_ld();
@@ -351,7 +408,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         }
                     }
                 }
-                if (ok && row < rows) p.ml[slot * 128 + row] = make_float2(m_ref, l);
+                if (ok && half == 0 && row < rows) p.ml[slot * 128 + row] = make_float2(m_ref, l);
             }
             tc_fence_before_sync();
         }
@@ -359,7 +416,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     // teardown: every role comes here, also after a wait that gave up
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == MMA) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }

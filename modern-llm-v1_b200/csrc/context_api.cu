@@ -34,8 +34,9 @@ struct PrefixPlan {
     size_t decode_bytes, bytes;  // of the workspace: the decode's own, all
     size_t slots;
 };
-// The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others, and both are bound by HBM or, when
-// short, by latency: SMs are shared out by the bytes to be read.
+// The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others: SMs are shared out by the bytes to
+// be read, those of a prompt with more than 128 rows counted half as much again, because the prompts' kernel is then bound by its
+// products and exponentials (B=64 P=16384 L=256 16/4 D=128, prompts on 48 / 72 / 96 SMs: 37.7 / 32.5 / 31.4 us).
 PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool ragged) {
     PrefixPlan d;
     const int group = Hq / Hkv, n = B / G, sms = sm_count();
@@ -47,7 +48,7 @@ PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool 
     d.blocks = (d.tiles + 1) / 2;
     const long long ctas = (long long)G * Hkv * d.n_chunks * d.blocks;
     const int all = (P + kPrefixKeys - 1) / kPrefixKeys;
-    const double keys = (double)G * P, own = (double)B * L;
+    const double keys = (double)G * P * (d.tiles > 1 ? 1.5 : 1.0), own = (double)B * L;
     const int share = std::max(1, (int)(sms * keys / (keys + own)));
     d.splits = (int)std::max<long long>(1, std::min<long long>(all, share / ctas));
     d.grid = ctas * d.splits;
@@ -69,7 +70,7 @@ int launch_prefix(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMa
     static bool set[kMaxDevices] = {false};
     const int rc = set_smem_once(attn_prefix_kernel<D, ROWS2>, smem, set);
     if (rc) return rc;
-    if (launch_pdl(attn_prefix_kernel<D, ROWS2>, dim3(grid), kPrefixThreads, smem, st, tq, tk, tv, p) != cudaSuccess) {
+    if (launch_pdl(attn_prefix_kernel<D, ROWS2>, dim3(grid), PrefixCfg<D, ROWS2>::kThreads, smem, st, tq, tk, tv, p) != cudaSuccess) {
         cudaGetLastError();
         return B200ATTN_ERR_CUDA;
     }

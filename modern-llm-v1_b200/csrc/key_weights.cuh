@@ -154,29 +154,6 @@ __host__ __device__ __forceinline__ int key_weights_cta(const KeyWeightsParams& 
     return u < longer ? u / (p.per_cta + 1) : p.more + (u - longer) / p.per_cta;
 }
 
-// Two exponentials 2^x on the FMA pipes, for the share of a unit's that the special-function units are spared: x = n + f with n the
-// nearest whole number (the addition of 1.5 * 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by a polynomial of degree 5 whose
-// coefficients minimise the largest relative error (7.5e-8; 2.1e-7 with the FP32 arithmetic), times 2^n made of its exponent bits.
-// Clamped to -127 .. 128, whose exponent bits are those of 0 and infinity; NaN stays NaN.
-__device__ __forceinline__ uint64_t exp2_fma_f32x2(uint64_t x2) {
-    float x0, x1;
-    unpack_f32x2(x2, x0, x1);
-    asm("min.NaN.f32 %0, %0, 0f43000000;\n\tmax.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x0));
-    asm("min.NaN.f32 %0, %0, 0f43000000;\n\tmax.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x1));
-    const uint64_t x = pack_f32x2(x0, x1), magic = pack_f32x2(12582912.f, 12582912.f), unmagic = pack_f32x2(-12582912.f, -12582912.f);
-    const uint64_t t = add_f32x2(x, magic);
-    const uint64_t f = fma_f32x2(add_f32x2(t, unmagic), pack_f32x2(-1.f, -1.f), x);
-    uint64_t r = fma_f32x2(f, pack_f32x2(0.001327647129073739f, 0.001327647129073739f), pack_f32x2(0.009675541892647743f, 0.009675541892647743f));
-    r = fma_f32x2(r, f, pack_f32x2(0.05550713464617729f, 0.05550713464617729f));
-    r = fma_f32x2(r, f, pack_f32x2(0.24022120237350464f, 0.24022120237350464f));
-    r = fma_f32x2(r, f, pack_f32x2(0.6931469440460205f, 0.6931469440460205f));
-    r = fma_f32x2(r, f, pack_f32x2(1.0000001192092896f, 1.0000001192092896f));
-    float t0, t1;
-    unpack_f32x2(t, t0, t1);
-    const uint64_t s = pack_f32x2(__uint_as_float((__float_as_uint(t0) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t1) << 23) + 0x3f800000u));
-    return mul_f32x2(r, s);
-}
-
 template <int D>
 __global__ void __launch_bounds__(kKeyWeightsThreads, 1)
 key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const KeyWeightsParams p) {
