@@ -29,7 +29,7 @@ kv_rotary_kernel(const __grid_constant__ KvRotaryParams p) {
     const int lane = threadIdx.x & 31, sub = lane / LPR, li = lane % LPR;
     const unsigned warp0 = (blockIdx.x * kKvAppendThreads + threadIdx.x) >> 5, n_warps = (gridDim.x * kKvAppendThreads) >> 5;
     const unsigned n_rows = p.rows_q + 2u * p.rows_kv;
-    RotaryLane<D, HALF> rl(p.R, lane, li);
+    RotaryLane<D, HALF> rl(p.R, li);
     if (p.n_new == 1) grid_dep_launch();  // (as in kv_append_kernel)
     grid_dep_wait();
 
@@ -59,21 +59,21 @@ kv_rotary_kernel(const __grid_constant__ KvRotaryParams p) {
             else if (pos < 0 || pos + p.n_new > p.n_pos) bad = DEV_ROTARY_POSITION;
             if (bad) pos = row = 0;
             pos += t, row += t;
-            rn_load8<F32>(which == 0 ? p.xq : which == 1 ? p.xk : p.xv, static_cast<long long>(r) * D + li * 8, v);
+            RotaryRaw<F32, HALF> raw;
+            raw.load(which == 0 ? p.xq : which == 1 ? p.xk : p.xv, static_cast<long long>(r) * D, rl.at, rl.more);
+            raw.r.get(v);
             if (NORM && which != 2) {
-                const float* gamma = which == 0 ? p.gamma_q : p.gamma_k;
-                const float4 g0 = *reinterpret_cast<const float4*>(gamma + li * 8), g1 = *reinterpret_cast<const float4*>(gamma + li * 8 + 4);
-                gm[0] = g0.x, gm[1] = g0.y, gm[2] = g0.z, gm[3] = g0.w, gm[4] = g1.x, gm[5] = g1.y, gm[6] = g1.z, gm[7] = g1.w;
+                rotary_gamma(which == 0 ? p.gamma_q : p.gamma_k, rl.at, rl.more, gm);
             }
         }
         // (a position that the tables do not have reads their first rows: t < n_new <= n_pos was checked by the host)
         rl.load(p.cos_t, p.sin_t, p.R, li, pos);
-        rl.template rotate<false>(v, rot);  // every lane takes part in the shuffles
+        rl.template rotate<false>(v, rot);
         float ss = 0.f;
         if constexpr (NORM) {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) ss += rot[e] * rot[e] + rot[e + 1] * rot[e + 1];
-            ss = rn_row_sum<LPR>(ss);
+            ss = rn_row_sum<LPR>(ss);  // every lane takes part in the shuffles
         }
         if (!live) continue;
         if (bad) {
@@ -82,7 +82,7 @@ kv_rotary_kernel(const __grid_constant__ KvRotaryParams p) {
         }
         const long long at = (static_cast<long long>(b) * p.Hkv + h) * p.L_cap + row;  // of k and v rows
         if (which == 2) {
-            rn_store8<false>(p.vcache, at * D + li * 8, v);
+            rotary_store8<false, HALF>(p.vcache, at * D, rl.at, rl.more, v);
             continue;
         }
         if constexpr (NORM) {
@@ -93,9 +93,9 @@ kv_rotary_kernel(const __grid_constant__ KvRotaryParams p) {
             for (int e = 0; e < 8; ++e) rot[e] = out[e];
         }
         if (which == 0) {
-            rn_store8<false>(p.q_out, ((static_cast<long long>(b) * p.Hq + h) * p.n_new + t) * D + li * 8, rot);
+            rotary_store8<false, HALF>(p.q_out, ((static_cast<long long>(b) * p.Hq + h) * p.n_new + t) * D, rl.at, rl.more, rot);
         } else {
-            rn_store8<false>(p.kcache, at * D + li * 8, rot);
+            rotary_store8<false, HALF>(p.kcache, at * D, rl.at, rl.more, rot);
             if (p.positions && li == 0) p.positions[at] = int(pos);
         }
     }

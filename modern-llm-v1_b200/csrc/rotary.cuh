@@ -8,10 +8,10 @@
 //   back, with the norm:  g = dy gamma, s = sum g r, dr = rstd g - rstd^3 / D s r, d_gamma += sum over rows of dy r rstd;
 //   without it dr = dy (x is not read);  dx: (da cos + db sin, -da sin + db cos)
 //
-// Bound by HBM like rope_norm.cuh, whose deal of the work this is: a lane owns 8 consecutive elements, a warp 256 / D tokens and a
-// chunk of heads, so that a token's cosines and sines stay in registers.  Where the halves are paired, an element's partner lies
-// R / 16 lanes further (R is a multiple of 16: never inside a lane) and comes by shuffle; loading it a second time instead would
-// double the requests to L1.
+// Bound by HBM like rope_norm.cuh, whose deal of the work this is: a lane owns 8 elements of a row, a warp 256 / D tokens and a chunk of
+// heads, so that a token's cosines and sines stay in registers.  Where the halves are paired a lane's 8 elements are four pairs, two
+// pieces of four R / 2 apart (R is a multiple of 16); behind R they are two pieces side by side.  (Eight elements in a row, with the
+// partners by shuffle, took twice the registers for the tables and 8 shuffles a row: XX.)
 #pragma once
 
 #include "rope_norm.cuh"
@@ -25,58 +25,78 @@ struct RotaryParams : RopeNormParams {
     int* status;     // set to DEV_ROTARY_POSITION when a position is not a row of the tables (the token's rows are skipped)
 };
 
-// A lane's share of one row of the tables
+// A lane's 8 elements of a row and its share of one row of the tables: four pairs either way, (v[2i], v[2i+1]) of neighbours, (v[i], v[i+4])
+// of halves.
 template <int D, bool HALF>
 struct RotaryLane {
-    float c[HALF ? 8 : 4], s[HALF ? 8 : 4];
-    bool turns;   // the lane's elements are rotated
-    int partner;  // HALF: the lane that has the pairs' other elements
+    float c[4], s[4];
+    bool turns;    // the lane's elements are rotated
+    int at, more;  // the lane's first four elements, and how much further the other four are (4 but for pairs of halves)
     // li: the lane within its row's D / 8
-    __device__ __forceinline__ RotaryLane(int R, int lane, int li) {
+    __device__ __forceinline__ RotaryLane(int R, int li) {
         turns = li * 8 < R;
-        const int half = R / 16;  // lanes
-        partner = !turns ? lane : li < half ? lane + half : lane - half;
+        at = HALF && turns ? li * 4 : li * 8;
+        more = HALF && turns ? R / 2 : 4;
     }
     __device__ __forceinline__ void load(const float* cos_t, const float* sin_t, int R, int li, long long pos) {
         if (!turns) {
 #pragma unroll
-            for (int e = 0; e < (HALF ? 8 : 4); ++e) c[e] = 1.f, s[e] = 0.f;
+            for (int e = 0; e < 4; ++e) c[e] = 1.f, s[e] = 0.f;
             return;
         }
-        const int half = R / 16;
-        const bool first = li < half;
-        const long long at = pos * (R / 2) + (HALF ? (first ? li : li - half) * 8 : li * 4);
-#pragma unroll
-        for (int e = 0; e < (HALF ? 8 : 4); e += 4) {
-            const float4 cv = *reinterpret_cast<const float4*>(cos_t + at + e), sv = *reinterpret_cast<const float4*>(sin_t + at + e);
-            c[e] = cv.x, c[e + 1] = cv.y, c[e + 2] = cv.z, c[e + 3] = cv.w;
-            s[e] = sv.x, s[e + 1] = sv.y, s[e + 2] = sv.z, s[e + 3] = sv.w;
-            if (HALF && first) {  // (the first half of a pair: a cos - b sin)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[e + k] = -s[e + k];
-            }
-        }
+        const long long at_t = pos * (R / 2) + li * 4;
+        const float4 cv = *reinterpret_cast<const float4*>(cos_t + at_t), sv = *reinterpret_cast<const float4*>(sin_t + at_t);
+        c[0] = cv.x, c[1] = cv.y, c[2] = cv.z, c[3] = cv.w;
+        s[0] = sv.x, s[1] = sv.y, s[2] = sv.z, s[3] = sv.w;
     }
-    // BACK: by the opposite angle.  Every lane of the warp takes part.
+    // BACK: by the opposite angle
     template <bool BACK>
     __device__ __forceinline__ void rotate(const float (&v)[8], float (&out)[8]) const {
-        if constexpr (HALF) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float o = __shfl_sync(0xffffffffu, v[e], partner);
-                // (elements that do not turn are copied: times one plus zero times another would make NaN of infinities)
-                out[e] = !turns ? v[e] : BACK ? v[e] * c[e] - o * s[e] : v[e] * c[e] + o * s[e];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = v[2 * i], b = v[2 * i + 1];
-                out[2 * i] = !turns ? a : BACK ? a * c[i] + b * s[i] : a * c[i] - b * s[i];
-                out[2 * i + 1] = !turns ? b : BACK ? b * c[i] - a * s[i] : a * s[i] + b * c[i];
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int x = HALF ? i : 2 * i, y = HALF ? i + 4 : 2 * i + 1;
+            const float a = v[x], b = v[y];
+            // (elements that do not turn are copied: times one plus zero times another would make NaN of infinities)
+            out[x] = !turns ? a : BACK ? a * c[i] + b * s[i] : a * c[i] - b * s[i];
+            out[y] = !turns ? b : BACK ? b * c[i] - a * s[i] : a * s[i] + b * c[i];
         }
     }
 };
+// The lane's 8 elements of the row that begins at element offset `row`, as they lie in memory
+template <bool F32, bool HALF>
+struct RotaryRaw {
+    RnRaw<F32> r;
+    __device__ __forceinline__ void load(const void* base, long long row, int at, int more) {
+        if constexpr (!HALF) {
+            r.load(base, row + at);
+        } else if constexpr (F32) {
+            const float* const ptr = static_cast<const float*>(base) + row + at;
+            r.w[0] = __ldcs(reinterpret_cast<const uint4*>(ptr)), r.w[1] = __ldcs(reinterpret_cast<const uint4*>(ptr + more));
+        } else {
+            const uint16_t* const ptr = static_cast<const uint16_t*>(base) + row + at;
+            const uint2 a = __ldcs(reinterpret_cast<const uint2*>(ptr)), b = __ldcs(reinterpret_cast<const uint2*>(ptr + more));
+            r.w[0] = make_uint4(a.x, a.y, b.x, b.y);
+        }
+    }
+};
+template <bool F32, bool HALF>
+__device__ __forceinline__ void rotary_store8(void* base, long long row, int at, int more, const float (&v)[8]) {
+    if constexpr (!HALF) {
+        rn_store8<F32>(base, row + at, v);
+    } else if constexpr (F32) {
+        float* const ptr = static_cast<float*>(base) + row + at;
+        *reinterpret_cast<float4*>(ptr) = make_float4(v[0], v[1], v[2], v[3]), *reinterpret_cast<float4*>(ptr + more) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint16_t* const ptr = static_cast<uint16_t*>(base) + row + at;
+        *reinterpret_cast<uint2*>(ptr) = make_uint2(rn_pack_bf16x2(v[0], v[1]), rn_pack_bf16x2(v[2], v[3]));
+        *reinterpret_cast<uint2*>(ptr + more) = make_uint2(rn_pack_bf16x2(v[4], v[5]), rn_pack_bf16x2(v[6], v[7]));
+    }
+}
+// gamma of the lane's elements
+__device__ __forceinline__ void rotary_gamma(const float* gamma, int at, int more, float (&g)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(gamma + at), b = *reinterpret_cast<const float4*>(gamma + at + more);
+    g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, g[4] = b.x, g[5] = b.y, g[6] = b.z, g[7] = b.w;
+}
 
 // The position of a lane's token; a token whose position the tables do not have is dropped (live = false).
 template <int D>
@@ -95,29 +115,28 @@ __device__ __forceinline__ unsigned rotary_fwd_tensor(const RotaryParams& p, uns
     constexpr int kUnroll = 4;
     const int lane = threadIdx.x & 31;
     const int sub = lane / LPR, li = lane % LPR;
-    RotaryLane<D, HALF> rl(p.R, lane, li);
+    RotaryLane<D, HALF> rl(p.R, li);
     float gm[8];
     if constexpr (NORM) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gm[e] = p.gamma[li * 8 + e];
+        rotary_gamma(p.gamma, rl.at, rl.more, gm);
     }
     for (; item < p.n_items; item += n_warps) {
         RnItem<D> it(p, item, sub);
         rl.load(p.cos_t, p.sin_t, p.R, li, rotary_position<D>(p, it));
-        const long long x_off = it.b * p.x_sb + it.t * p.x_st + li * 8, y_off = it.b * p.y_sb + it.t * p.y_st + li * 8;
+        const long long x_off = it.b * p.x_sb + it.t * p.x_st, y_off = it.b * p.y_sb + it.t * p.y_st;
         float* rstd_t = NORM ? p.rstd + static_cast<long long>(it.b) * p.H * p.T + it.t : nullptr;
         for (int h = it.h0; h < it.h1; h += kUnroll) {
-            RnRaw<F32> raw[kUnroll];
+            RotaryRaw<F32, HALF> raw[kUnroll];
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) {
-                raw[k].clear();
-                if (it.live && h + k < it.h1) raw[k].load(p.x, x_off + (h + k) * p.x_sh);
+                raw[k].r.clear();
+                if (it.live && h + k < it.h1) raw[k].load(p.x, x_off + (h + k) * p.x_sh, rl.at, rl.more);
             }
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) {
                 if (h + k >= it.h1) break;
                 float v[8], rot[8];
-                raw[k].get(v);
+                raw[k].r.get(v);
                 rl.template rotate<false>(v, rot);
                 if constexpr (NORM) {
                     float ss = 0.f;
@@ -127,11 +146,11 @@ __device__ __forceinline__ unsigned rotary_fwd_tensor(const RotaryParams& p, uns
                     float out[8];
                     rn_scale8(rot, rstd, gm, out);
                     if (it.live) {
-                        rn_store8<false>(p.y, y_off + (h + k) * p.y_sh, out);
+                        rotary_store8<false, HALF>(p.y, y_off + (h + k) * p.y_sh, rl.at, rl.more, out);
                         if (li == 0) rstd_t[static_cast<long long>(h + k) * p.T] = rstd;
                     }
                 } else if (it.live) {
-                    rn_store8<false>(p.y, y_off + (h + k) * p.y_sh, rot);
+                    rotary_store8<false, HALF>(p.y, y_off + (h + k) * p.y_sh, rl.at, rl.more, rot);
                 }
             }
         }
@@ -155,30 +174,31 @@ __device__ __forceinline__ unsigned rotary_bwd_tensor(const RotaryParams& p, uns
     constexpr int kUnroll = NORM ? 2 : 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int sub = lane / LPR, li = lane % LPR;
-    RotaryLane<D, HALF> rl(p.R, lane, li);
+    RotaryLane<D, HALF> rl(p.R, li);
     float gm[8], dg[8];
     if constexpr (NORM) {
+        rotary_gamma(p.gamma, rl.at, rl.more, gm);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) gm[e] = p.gamma[li * 8 + e], dg[e] = 0.f;
+        for (int e = 0; e < 8; ++e) dg[e] = 0.f;
     }
     for (; item < p.n_items; item += n_warps) {
         RnItem<D> it(p, item, sub);
         rl.load(p.cos_t, p.sin_t, p.R, li, rotary_position<D>(p, it));
-        const long long x_off = it.b * p.x_sb + it.t * p.x_st + li * 8, y_off = it.b * p.y_sb + it.t * p.y_st + li * 8;
+        const long long x_off = it.b * p.x_sb + it.t * p.x_st, y_off = it.b * p.y_sb + it.t * p.y_st;
         const float* rstd_t = NORM ? p.rstd + static_cast<long long>(it.b) * p.H * p.T + it.t : nullptr;
         for (int h = it.h0; h < it.h1; h += kUnroll) {
-            RnRaw<F32> raw_x[NORM ? kUnroll : 1];
-            RnRaw<false> raw_dy[kUnroll];
+            RotaryRaw<F32, HALF> raw_x[NORM ? kUnroll : 1];
+            RotaryRaw<false, HALF> raw_dy[kUnroll];
             float rstd[kUnroll];
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) {
-                if constexpr (NORM) raw_x[k].clear();
-                raw_dy[k].clear();
+                if constexpr (NORM) raw_x[k].r.clear();
+                raw_dy[k].r.clear();
                 rstd[k] = 0.f;
                 if (it.live && h + k < it.h1) {
-                    raw_dy[k].load(p.dy, y_off + (h + k) * p.y_sh);
+                    raw_dy[k].load(p.dy, y_off + (h + k) * p.y_sh, rl.at, rl.more);
                     if constexpr (NORM) {
-                        raw_x[k].load(p.x, x_off + (h + k) * p.x_sh);
+                        raw_x[k].load(p.x, x_off + (h + k) * p.x_sh, rl.at, rl.more);
                         rstd[k] = rstd_t[static_cast<long long>(h + k) * p.T];
                     }
                 }
@@ -187,10 +207,10 @@ __device__ __forceinline__ unsigned rotary_bwd_tensor(const RotaryParams& p, uns
             for (int k = 0; k < kUnroll; ++k) {
                 if (h + k >= it.h1) break;
                 float d[8], dx[8];
-                raw_dy[k].get(d);
+                raw_dy[k].r.get(d);
                 if constexpr (NORM) {
                     float v[8], rot[8];
-                    raw_x[k].get(v);
+                    raw_x[k].r.get(v);
                     rl.template rotate<false>(v, rot);
                     const float rs = rstd[k];
                     float s = 0.f;
@@ -207,7 +227,7 @@ __device__ __forceinline__ unsigned rotary_bwd_tensor(const RotaryParams& p, uns
                     for (int e = 0; e < 8; ++e) d[e] = rs * d[e] - coeff * rot[e];
                 }
                 rl.template rotate<true>(d, dx);
-                if (it.live) rn_store8<F32>(p.y, x_off + (h + k) * p.x_sh, dx);
+                if (it.live) rotary_store8<F32, HALF>(p.y, x_off + (h + k) * p.x_sh, rl.at, rl.more, dx);
             }
         }
     }
@@ -219,7 +239,7 @@ __device__ __forceinline__ unsigned rotary_bwd_tensor(const RotaryParams& p, uns
         }
         if (sub == 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s_part[warp][li * 8 + e] = dg[e];
+            for (int e = 0; e < 8; ++e) s_part[warp][rl.at + (e < 4 ? e : rl.more + e - 4)] = dg[e];
         }
         __syncthreads();
         for (int d = threadIdx.x; d < D; d += kRopeNormThreads) {
