@@ -37,11 +37,12 @@ __global__ void __launch_bounds__(kDecodeWeightsThreads) decode_weights_kernel(c
     __shared__ float s_lse[16];
     const int u = int(blockIdx.x) / p.blocks, key0 = (int(blockIdx.x) - u * p.blocks) * K * STEP, b = u / p.Hkv;
     const int group = p.G * p.n_chunks;
+    grid_dep_launch();  // (the next step's first kernel waits for the end of this one, but not with its set-up)
     grid_dep_wait();
-    const int len = p.lens ? max(1, min(__ldg(p.lens + b), p.L)) : p.L;
-    if (key0 >= len || *reinterpret_cast<const volatile int*>(p.status) != 0) return;
+    // What the length and the status word say is looked at behind the loads, which go as far as L: one round trip
+    const int status = *reinterpret_cast<const volatile int*>(p.status), len = p.lens ? max(1, min(__ldg(p.lens + b), p.L)) : p.L;
     float* const w = p.w + size_t(u) * p.L_cap + key0 + threadIdx.x;
-    const int left = len - key0 - int(threadIdx.x);  // key k of this thread counts where k * STEP < left
+    const int left = p.L - key0 - int(threadIdx.x), count = len - key0 - int(threadIdx.x);  // key k of this thread: k * STEP < left, < count
     float old[K], acc[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) old[k] = k * STEP < left ? w[k * STEP] : 0.f, acc[k] = 0.f;
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(kDecodeWeightsThreads) decode_weights_kernel(c
     }
 #pragma unroll
     for (int k = 0; k < K; ++k)
-        if (k * STEP < left) w[k * STEP] = old[k] + acc[k];
+        if (k * STEP < count && status == 0) w[k * STEP] = old[k] + acc[k];
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------
