@@ -7,23 +7,27 @@
 // The decode kernel behind (attn_decode.cuh, kDecodeShared) goes on with the sequences' own rows and joins the two: the softmax of a
 // union is the partial results' sum with weights 2^((m_i - max m) scale_log2).
 //
-// A CTA takes a share of the prompt's key tiles (128 keys) and one or two tiles of 128 rows (a row = a lane of tensor memory:
-// S = Q K^T with Q's rows as M); rows that a tile does not have cost their part of the products, which are not what bounds it.  What a
-// single online softmax cannot do is keep up: product, scores out of tensor memory, maximum, exponentials, P back and the next product
-// are a chain of some 2800 clocks (D = 128), in which an SM's share of HBM brings 64 KB, the tile.  So a CTA runs two of them, each with S
-// and O of its own, and one's chain passes under the other's exponentials (1024 clocks a tile and 128 rows):
-//   ROWS2 = false  one tile of rows, key tiles in turn (the two results are joined through shared memory at the end).  Up to 64 rows the
-//                  second softmax has them in lanes 64 .. 127, so that each has two of the SM's four schedulers for itself
-//   ROWS2 = true   two tiles of rows, every K and V tile used twice (more than 128 rows; further ones read the prompt through L2)
-// P goes over S's columns once S is in registers, which leaves room for 128 keys and two softmaxes at both head dimensions: with tiles of
-// 64 keys a step of Q K^T, both operands in shared memory, takes the same 64 clocks for half the keys (B=64 P=16384 16/4 D=128, this
-// kernel: 21.5 -> XX us).
+// A CTA takes a tile of 128 rows (a row = a lane of tensor memory: S = Q K^T with Q's rows as M) and a share of the prompt's key tiles
+// (128 keys); rows that the tile does not have cost their part of the products, which are not what bounds it, and further tiles of rows
+// read the prompt through L2.  What a single online softmax cannot do is keep up: product, scores out of tensor memory, maximum,
+// exponentials, P back and the next product are a chain of 3300 clocks, in which an SM's share of HBM brings 64 KB, a tile at D = 128.  So
+// a CTA runs two of them, taking its tiles in turn, each with S and O of its own; the two results are joined through shared memory at
+// the end.  Up to 64 rows the second softmax has them in lanes 64 .. 127, so that each has two of the SM's four schedulers for itself.
+// P goes over S's columns, which leaves room for 128 keys and two softmaxes at both head dimensions.
 //
-// Roles: warps 0 .. 8 H - 1 softmax, the first half of them the one, the second the other; thread = row (ROWS2, H = 1), or row and half of
-// the tile's keys (H = 2: two warps share a row's maximum through shared memory); rescaling only where the maximum grew by 2^8 as in
-// attn_fwd.cuh; warps that have no row are not waited for and leave.  Then a warp that loads, a ring of K and V tiles in the order in
-// which the products read them, and one that issues the products.  TMEM (512 columns), per softmax: S 128 with P over its scores, O D.
-// XX
+// Roles (576 threads): warps 0-7 the one softmax, 8-15 the other; thread = row and half of the tile's keys (two warps share a row's maximum
+// through shared memory), rescaling only where the maximum grew by 2^8 as in attn_fwd.cuh; warps that have no row are not waited for
+// and leave.  Warp 16 loads, a ring of K and V tiles in the order in which the products read them; warp 17 issues the products.  TMEM
+// (512 columns), per softmax: S 128 with P over each half's scores, O D.
+//
+// Measured on B200, us per call, this kernel and the decode behind (G prompts, n sequences each, 16/4 heads):
+//   G=8 n=16 P<=2000 L<=300 D=64: one softmax 28.3, two, thread = row 27.0, thread = row and half 25.3
+//   G=1 n=64 P=16384 L=256 D=128: one softmax 31.5, two, thread = row and half 27.4 (67 MB: 2.4 TB/s)
+//   G=1 n=8 P=500 L=12 6/2 D=64: 6.9, 7.0 and 7.2 (the two launches' latency)
+// Measured and dropped: tiles of 64 keys with P beside S (Q K^T takes 64 clocks a step for half the keys); two tiles of rows in a CTA, every K and
+// V tile used twice, 31.5 where two CTAs that each read them take 27.4 (the partial results of 256 rows are as many bytes as 256 keys, and
+// twice as many shares have to be joined); its results added up over a cluster through distributed shared memory (35: clusters of four
+// crowd into a few GPCs, whose bandwidth they then share); a second warp for the products (38: the two interleave on the tensor pipe).
 #pragma once
 
 #include "ptx.cuh"
@@ -36,7 +40,7 @@ struct PrefixParams {
     int heads, seqs;        // of a tile of rows: heads x seqs <= 128
     int group, n_chunks, Hkv;
     int splits, tiles;      // shares of the keys, tiles of rows per chunk
-    FastDiv div_splits, div_blocks, div_chunks, div_hkv;  // blocks: of tiles, ceil(tiles / 2) or tiles
+    FastDiv div_splits, div_tiles, div_chunks, div_hkv;
     const int* lens;        // [prompts] or nullptr: P
     float scale_log2;
     float* o;               // [slot][D / 4][128][4]
@@ -45,44 +49,40 @@ struct PrefixParams {
 };
 
 constexpr int kPrefixKeys = 128;  // per tile
-template <int D, bool ROWS2>
+constexpr int kPrefixThreads = 576;
+template <int D>
 struct PrefixCfg {
     static constexpr int kTileBytes = kPrefixKeys * D * 2;
     static constexpr int kBoxBytes = kPrefixKeys * 128;  // [keys][64] BF16
     static constexpr int kBoxes = D / 64;
     static constexpr int kStages = D == 64 ? 8 : 4;      // 128 KB
-    static constexpr int kQBoxBytes = 128 * 128, kQTiles = 2;  // (of the same rows, 64 lanes apart, or of two tiles)
-    static constexpr int kHalves = ROWS2 ? 1 : 2, kThreads = (8 * kHalves + 2) * 32;
-    static constexpr int kAhead = ROWS2 ? 1 : 2;       // K tiles loaded ahead of V of tile 0
-    static constexpr int kSmemBytes = kQTiles * kBoxes * kQBoxBytes + kStages * kTileBytes + 6144 + 256;
+    static constexpr int kQBoxBytes = 128 * 128;
+    static constexpr int kQBytes = 2 * kBoxes * kQBoxBytes;  // once, and once more 64 rows further down
+    static constexpr int kSmemBytes = kQBytes + kStages * kTileBytes + 6144 + 256;
     static_assert(kStages * kTileBytes >= 128 * D * 4, "one softmax's O goes to the other through the ring");
-    static constexpr int kColS = 0, kColO = 128;       // + 256 for the second softmax
+    static constexpr int kColS = 0, kColO = 128;         // + 256 for the second softmax
 };
 constexpr float kPrefixRescaleLog2 = 8.0f;  // P <= 2^8: its rounding to BF16 (the second product's operand) is relative
 
-// Place of a load: first `ahead` K tiles, then V of tile j and K of tile j + ahead in turn, the last V tiles at the end
-__host__ __device__ __forceinline__ int prefix_k_at(int j, int ahead) { return j < ahead ? j : 2 * j - ahead + 1; }
-__host__ __device__ __forceinline__ int prefix_v_at(int j, int n, int ahead) { return j + ahead < n ? 2 * j + ahead : n + j; }
+// Place of a load: K of tiles 0 and 1, then V of tile j and K of tile j + 2 in turn, the last two V tiles at the end
+__host__ __device__ __forceinline__ int prefix_k_at(int j) { return j < 2 ? j : 2 * j - 1; }
+__host__ __device__ __forceinline__ int prefix_v_at(int j, int n) { return j + 2 < n ? 2 * j + 2 : n + j; }
 // The i-th load of 2 n: whether it is a K tile, and of which tile
-__host__ __device__ __forceinline__ bool prefix_load_at(int i, int n, int ahead, int* j) {
-    const int pairs = n - ahead;  // loads [ahead, ahead + 2 pairs) come in pairs
-    if (i < ahead && i < n) return *j = i, true;
-    if (pairs > 0 && i < ahead + 2 * pairs) {
-        const int e = i - ahead;
-        return (e & 1) ? (*j = ahead + e / 2, true) : (*j = e / 2, false);
-    }
+__host__ __device__ __forceinline__ bool prefix_load_at(int i, int n, int* j) {
+    if (i < 2 && i < n) return *j = i, true;
+    if (i >= 2 && i < 2 * n - 2) return (i & 1) ? (*j = (i + 1) / 2, true) : (*j = i / 2 - 1, false);
     return *j = i - n, false;
 }
 
-template <int D, bool ROWS2>
-__global__ void __launch_bounds__(PrefixCfg<D, ROWS2>::kThreads, 1)
+template <int D>
+__global__ void __launch_bounds__(kPrefixThreads, 1)
 attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const PrefixParams p) {
-    using Cfg = PrefixCfg<D, ROWS2>;
-    constexpr int KEYS = kPrefixKeys, NST = Cfg::kStages, A = Cfg::kAhead, H = Cfg::kHalves, PRODUCER = 8 * H, MMA = 8 * H + 1;
+    using Cfg = PrefixCfg<D>;
+    constexpr int KEYS = kPrefixKeys, NST = Cfg::kStages;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;
-    uint8_t* sRing = sQ + Cfg::kQTiles * Cfg::kBoxes * Cfg::kQBoxBytes;
+    uint8_t* sRing = sQ + Cfg::kQBytes;
     float* sMax = reinterpret_cast<float*>(sRing + NST * Cfg::kTileBytes);  // [softmax][tile & 1][half][128] maxima of the rows' halves
     float* sL = sMax + 1024;                                                // [softmax][128] at the end, l of the second halves
     float2* sMl = reinterpret_cast<float2*>(sL + 256);                      // [128] at the end, the second softmax's (m, l)
@@ -97,19 +97,16 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // blockIdx.x -> (prompt, KV head, chunk of heads, tiles of rows, split)
+    // blockIdx.x -> (prompt, KV head, chunk of heads, tile of rows, split)
     const int id = int(blockIdx.x);
     const int unit = int(fastdiv(id, p.div_splits)), split = id - unit * p.splits;
-    const int uc = int(fastdiv(unit, p.div_blocks)), block = unit - uc * int(p.div_blocks.d);
+    const int uc = int(fastdiv(unit, p.div_tiles)), qt = unit - uc * p.tiles;
     const int uh = int(fastdiv(uc, p.div_chunks)), chunk = uc - uh * p.n_chunks;
     const int prompt = int(fastdiv(uh, p.div_hkv)), hk = uh - prompt * p.Hkv;
-    auto rows_of = [&](int qt) { return max(0, min(p.seqs, p.n - qt * p.seqs)) * p.heads; };
-    const int qt0 = ROWS2 ? 2 * block : block;
-    const int rows0 = rows_of(qt0), rows1 = ROWS2 ? rows_of(qt0 + 1) : rows0;  // of the two softmaxes
-    const bool two = rows1 > 0;
-    const int lane1 = !ROWS2 && rows0 <= 64 ? 64 : 0;  // tensor memory lane of the second softmax's first row
+    const int rows = min(p.seqs, p.n - qt * p.seqs) * p.heads, n_warps = (rows + 31) / 32;  // warps of 32 rows
+    const int lane1 = p.heads * p.seqs <= 64 ? 64 : 0;  // tensor memory lane of the second softmax's first row (Q's box has that many rows)
 
-    if (warp == PRODUCER && lane == 0) {
+    if (warp == 16 && lane == 0) {
         tma_prefetch_desc(&tmQ);
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
@@ -119,15 +116,14 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         mbar_init(bar_q, 1);
         for (int x = 0; x < 2; ++x) {
-            const int n = max(1, ((x ? rows1 : rows0) + 31) / 32) * 32 * H;
             mbar_init(&bar_s_full[x], 1);
-            mbar_init(&bar_p_full[x], n);
+            mbar_init(&bar_p_full[x], 64 * n_warps);
             mbar_init(&bar_o[x], 1);
         }
         fence_mbar_init();
         *abort_flag = 0;
     }
-    if (warp == MMA) {
+    if (warp == 17) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -145,24 +141,22 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
-    // A unit is a tile's turn in one of the softmaxes: unit i is softmax i & 1's, of tile i / 2 (ROWS2) or i.
-    const int n_units = ROWS2 ? 2 * n_tiles : n_tiles;
 
     if (*abort_flag != 0) {
         // an earlier kernel has failed: nothing is loaded, nothing is written
-    } else if (warp == PRODUCER) {
+    } else if (warp == 16) {
         // ------------------------------------------------------------------ producer
         for (int i = 0; i < 2 * n_tiles; ++i) {
             int j;
-            const bool is_k = prefix_load_at(i, n_tiles, A, &j);
+            const bool is_k = prefix_load_at(i, n_tiles, &j);
             if (i >= NST && !mbar_wait_warp(&bar_free[i % NST], uint32_t(i / NST - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_FREE)) break;
             if (elect_one()) {
                 if (i == 0) {
-                    const int q_tiles = ROWS2 || lane1 ? 2 : 1;
-                    mbar_arrive_expect_tx(bar_q, q_tiles * Cfg::kBoxes * p.heads * p.seqs * 128);
-                    for (int e = 0; e < q_tiles * Cfg::kBoxes; ++e)
+                    const int boxes = (lane1 ? 2 : 1) * Cfg::kBoxes;
+                    mbar_arrive_expect_tx(bar_q, boxes * p.heads * p.seqs * 128);
+                    for (int e = 0; e < boxes; ++e)
                         tma_load_4d(sQ + e * Cfg::kQBoxBytes + (e >= Cfg::kBoxes ? lane1 * 128 : 0), &tmQ, bar_q, (e % Cfg::kBoxes) * 64,
-                                    hk * p.group + chunk * p.heads, prompt * p.n + (qt0 + (ROWS2 ? e / Cfg::kBoxes : 0)) * p.seqs, 0);
+                                    hk * p.group + chunk * p.heads, prompt * p.n + qt * p.seqs, 0);
                 }
                 uint8_t* dst = sRing + (i % NST) * Cfg::kTileBytes;
                 mbar_arrive_expect_tx(&bar_full[i % NST], Cfg::kTileBytes);
@@ -172,106 +166,85 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             __syncwarp();
         }
-    } else if (warp == MMA) {
+    } else if (warp == 17) {
         // ------------------------------------------------------------------ products
         constexpr uint32_t idesc_s = make_idesc_bf16(128, KEYS, 0, 0), idesc_o = make_idesc_bf16(128, D, 0, 1);
         const uint32_t ring = smem_u32(sRing);
         bool ok = n_tiles > 0 && mbar_wait_warp(bar_q, 0, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
-        // the tile's place is free behind its last unit
-        auto last_use = [&](int i) { return !ROWS2 || (i & 1) || !two; };
-        auto issue_s = [&](int i) {  // S = Q K^T of unit i; P of the softmax's unit before, over S, has been read by the products in front
-            const int x = i & 1, j = ROWS2 ? i >> 1 : i, at = prefix_k_at(j, A);
-            if (ROWS2 && x && !two) return;
+        auto issue_s = [&](int j) {  // S = Q K^T of tile j; P of the softmax's tile before, over S, has been read by the products in front
+            const int x = j & 1, at = prefix_k_at(j);
             ok = mbar_wait_warp(&bar_full[at % NST], uint32_t(at / NST) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
             if (!ok) return;
             tc_fence_after_sync();
-            const uint64_t q_desc = make_sdesc_sw128(smem_u32(sQ + (ROWS2 || lane1 ? x : 0) * Cfg::kBoxes * Cfg::kQBoxBytes), 16, 1024);
+            const uint64_t q_desc = make_sdesc_sw128(smem_u32(sQ + (lane1 ? x : 0) * Cfg::kBoxes * Cfg::kQBoxBytes), 16, 1024);
             const uint64_t k_desc = make_sdesc_sw128(ring + (at % NST) * Cfg::kTileBytes, 16, 1024);
             if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
                     umma_ss(tmem + x * 256 + Cfg::kColS, q_desc + kmajor_step(ks, Cfg::kQBoxBytes), k_desc + kmajor_step(ks, Cfg::kBoxBytes), idesc_s, ks > 0);
                 umma_commit(&bar_s_full[x]);
-                if (last_use(i)) umma_commit(&bar_free[at % NST]);
+                umma_commit(&bar_free[at % NST]);
             }
             __syncwarp();
         };
-        for (int i = 0; ok && i < min(2, n_units); ++i) issue_s(i);
-        for (int i = 0; ok && i < n_units; ++i) {
-            const int x = i & 1, j = ROWS2 ? i >> 1 : i, at = prefix_v_at(j, n_tiles, A);
-            if (ROWS2 && x && !two) continue;
+        for (int j = 0; ok && j < min(2, n_tiles); ++j) issue_s(j);
+        for (int j = 0; ok && j < n_tiles; ++j) {
+            const int x = j & 1, at = prefix_v_at(j, n_tiles);
             ok = mbar_wait_warp(&bar_full[at % NST], uint32_t(at / NST) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
-            if (ok) ok = mbar_wait_warp(&bar_p_full[x], uint32_t(i / 2) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_SOFTMAX);
+            if (ok) ok = mbar_wait_warp(&bar_p_full[x], uint32_t(j / 2) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_SOFTMAX);
             if (!ok) break;
             tc_fence_after_sync();
             const uint64_t v_desc = make_sdesc_sw128(ring + (at % NST) * Cfg::kTileBytes, Cfg::kBoxBytes, 1024);
             if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < KEYS / 16; ++ks)
-                    umma_ts(tmem + x * 256 + Cfg::kColO, tmem + x * 256 + Cfg::kColS + ks * 8 + (H == 2 ? (ks / (KEYS / 32)) * (KEYS / 4) : 0), v_desc + uint64_t(ks * 128), idesc_o, (i > 1) || (ks > 0));
-                if (i + 2 >= n_units) umma_commit(&bar_o[x]);
-                if (last_use(i)) umma_commit(&bar_free[at % NST]);
+                for (int ks = 0; ks < KEYS / 16; ++ks)  // P of keys 0-63 in columns 0-31, of keys 64-127 in columns 64-95
+                    umma_ts(tmem + x * 256 + Cfg::kColO, tmem + x * 256 + Cfg::kColS + (ks % 4) * 8 + (ks / 4) * 64, v_desc + uint64_t(ks * 128), idesc_o,
+                            (j > 1) || (ks > 0));
+                if (j + 2 >= n_tiles) umma_commit(&bar_o[x]);
+                umma_commit(&bar_free[at % NST]);
             }
             __syncwarp();
-            if (i + 2 < n_units) issue_s(i + 2);
+            if (j + 2 < n_tiles) issue_s(j + 2);
         }
         // nothing may be in flight when tensor memory is freed
-        for (int x = 0; ok && x < 2; ++x)
-            if (n_units > x && (two || x == 0)) ok = mbar_wait_warp(&bar_o[x], 0, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
+        for (int x = 0; ok && x < min(2, n_tiles); ++x) ok = mbar_wait_warp(&bar_o[x], 0, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
     } else {
         // ------------------------------------------------------------------ softmax, thread = row and half of the keys
-        const int x = warp / (4 * H), half = H == 2 ? (warp >> 2) & 1 : 0, row = (tid & 127) - (x ? lane1 : 0), rows = x ? rows1 : rows0, n_warps = (rows + 31) / 32;
+        const int x = warp >> 3, half = (warp >> 2) & 1, row = (tid & 127) - (x ? lane1 : 0);
         if (row >= 0 && row < 32 * n_warps) {
-            constexpr int COLS = KEYS / H;
+            constexpr int COLS = KEYS / 2, CH = 16;
             const uint32_t lanes = (uint32_t((warp & 3) * 32) << 16) + x * 256;
             const uint32_t t_s = tmem + lanes + Cfg::kColS + half * COLS, t_p = t_s,  // (each half's P over its own scores)
-                           t_o = tmem + lanes + Cfg::kColO + half * (D / H);
-            const int mine = (n_units - x + 1) / 2;  // units of this softmax
+                           t_o = tmem + lanes + Cfg::kColO + half * (D / 2);
+            const int mine = (n_tiles - x + 1) / 2;   // tiles of this softmax
             const int pair = 1 + x * 4 + (warp & 3);  // named barrier of the two warps that share rows
             bool ok = true;
             float m_ref = -INFINITY, l = 0.f;
             for (int e = 0; e < mine; ++e) {
-                const int j = ROWS2 ? e : 2 * e + x;
+                const int j = 2 * e + x;
                 if (ok) ok = mbar_wait_warp(&bar_s_full[x], uint32_t(e) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
-                if (H == 1 && !ok) break;
                 tc_fence_after_sync();
                 const int left = len - (j0 + j) * KEYS - half * COLS;  // keys of this half tile
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                // visit(CH columns, the first of which is c) for the thread's scores.  H = 1: they stay in registers from the first pass to the
-                // second (read twice, 37 us instead of 31: tensor memory is busy with the products); H = 2: there is no room for them, and time
-                constexpr int CH = H == 1 ? 32 : 16;
-                uint32_t v[H == 1 ? COLS / CH : 2][CH];
-                auto mask = [&](int c, uint32_t (&now)[CH]) {
-                    if (left < COLS) {
+                // visit(16 columns, the first of which is c) for the thread's scores, the next of which are on their way meanwhile
+                uint32_t v[2][CH];
+                auto columns = [&](auto visit) {
+                    tmem_ld_x16(t_s, v[0]);
 #pragma unroll
-                        for (int k = 0; k < CH; ++k)
-                            if (c + k >= left) now[k] = 0xff800000u;  // -inf
+                    for (int c = 0; c < COLS; c += CH) {
+                        tmem_wait_ld();
+                        if (c + CH < COLS) tmem_ld_x16(t_s + c + CH, v[(c / CH + 1) & 1]);
+                        uint32_t(&now)[CH] = v[(c / CH) & 1];
+                        if (left < COLS) {
+#pragma unroll
+                            for (int k = 0; k < CH; ++k)
+                                if (c + k >= left) now[k] = 0xff800000u;  // -inf
+                        }
+                        visit(c, now);
                     }
                 };
-                auto columns = [&](bool first, auto visit) {
-                    if constexpr (H == 1) {
-                        if (first) {
-#pragma unroll
-                            for (int c = 0; c < COLS; c += CH) tmem_ld_x32(t_s + c, v[c / CH]);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int c = 0; c < COLS; c += CH) mask(c, v[c / CH]);
-                        }
-#pragma unroll
-                        for (int c = 0; c < COLS; c += CH) visit(c, v[c / CH]);
-                    } else {
-                        tmem_ld_x16(t_s, v[0]);
-#pragma unroll
-                        for (int c = 0; c < COLS; c += CH) {
-                            tmem_wait_ld();
-                            if (c + CH < COLS) tmem_ld_x16(t_s + c + CH, v[(c / CH + 1) & 1]);  // (on its way meanwhile)
-                            mask(c, v[(c / CH) & 1]);
-                            visit(c, v[(c / CH) & 1]);
-                        }
-                    }
-                };
-                if (H == 1 || ok)
-                    columns(true, [&](int, uint32_t (&sr)[CH]) {
+                if (ok)
+                    columns([&](int, uint32_t (&sr)[CH]) {
 #pragma unroll
                         for (int k = 0; k < CH; k += 4)
 #pragma unroll
@@ -281,25 +254,22 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 // The other half's maximum.  (The place was last read two tiles ago, in front of the barrier of the tile between.)
                 const float m_half = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 float* const s_max = sMax + (x * 2 + (e & 1)) * 256 + (tid & 127);
-                if (H == 2) {
-                    s_max[half * 128] = m_half;
-                    named_bar_sync(pair, 64);
-                }
-                if (H == 2 && !ok) continue;  // (a warp that has given up still meets the other at the barriers)
+                s_max[half * 128] = m_half;
+                named_bar_sync(pair, 64);
+                if (!ok) continue;  // (a warp that has given up still meets the other at the barriers)
                 if (p.lens && len - (j0 + j) * KEYS < KEYS) {
-                    // Rows of the prompt's buffer beyond its length may hold anything: 0 * NaN would be NaN.  (With two tiles of rows
-                    // both softmaxes clear them, each in front of its own product.)
-                    const int at = prefix_v_at(j, n_tiles, A), first = len - (j0 + j) * KEYS;
+                    // rows of the prompt's buffer beyond its length may hold anything: 0 * NaN would be NaN
+                    const int at = prefix_v_at(j, n_tiles), first = len - (j0 + j) * KEYS;
                     ok = mbar_wait_warp(&bar_full[at % NST], uint32_t(at / NST) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
                     if (!ok) continue;
                     uint8_t* v = sRing + (at % NST) * Cfg::kTileBytes;
-                    for (int i = first * 8 * Cfg::kBoxes + row * H + half; i < KEYS * 8 * Cfg::kBoxes; i += 32 * H * n_warps) {
+                    for (int i = first * 8 * Cfg::kBoxes + row * 2 + half; i < KEYS * 8 * Cfg::kBoxes; i += 64 * n_warps) {
                         const int r = i / (8 * Cfg::kBoxes), part = i % (8 * Cfg::kBoxes);
                         *reinterpret_cast<uint4*>(v + (part / 8) * Cfg::kBoxBytes + r * 128 + (part % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async_smem();  // (in front of the arrival on bar_p_full, upon which the product reads them)
                 }
-                const float m_new = fmaxf(H == 2 ? fmaxf(m_half, s_max[128 - half * 128]) : m_half, m_ref);
+                const float m_new = fmaxf(fmaxf(m_half, s_max[128 - half * 128]), m_ref);
                 float alpha = 1.f;
                 if ((m_new - m_ref) * p.scale_log2 > kPrefixRescaleLog2) {  // also true for m_ref == -inf
                     alpha = ex2_approx((m_ref - m_new) * p.scale_log2);
@@ -309,13 +279,13 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2), neg2 = pack_f32x2(neg_m, neg_m);
                 uint64_t sum2[2] = {0ull, 0ull};
                 // (P V of the tile before, which adds to O, is complete: it lies in front of this S in the pipe)
-                columns(false, [&](int c, uint32_t (&sr)[CH]) {
+                columns([&](int c, uint32_t (&sr)[CH]) {
                     uint32_t pk[CH / 2];
 #pragma unroll
                     for (int i = 0; i < CH / 2; ++i) {
                         const uint64_t a = fma_f32x2(pack_f32x2(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), scale2, neg2);
                         float a0, a1;
-                        if (H == 2 && i % 4 == 3) {  // a quarter of them on the FMA pipes
+                        if (i % 4 == 3) {  // a quarter of them on the FMA pipes
                             const uint64_t e2 = exp2_fma_f32x2(a);
                             sum2[i & 1] = add_f32x2(sum2[i & 1], e2);
                             unpack_f32x2(e2, a0, a1);
@@ -327,15 +297,14 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         }
                         pk[i] = pack_bf16x2(a0, a1);
                     }
-                    if constexpr (CH == 32) tmem_st_x16(t_p + c / 2, pk);
-                    else tmem_st_x8(t_p + c / 2, pk);
+                    tmem_st_x8(t_p + c / 2, pk);
                 });
                 float s0, s1;
                 unpack_f32x2(add_f32x2(sum2[0], sum2[1]), s0, s1);
                 l = l * alpha + (s0 + s1);
                 if (e > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
-                    for (int c = 0; c < D / (32 * H); ++c) {
+                    for (int c = 0; c < D / 64; ++c) {
                         uint32_t orr[32];
                         tmem_ld_x32(t_o + c * 32, orr);
                         tmem_wait_ld();
@@ -352,22 +321,19 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             tc_fence_after_sync();
             // ---- O, m, l out: the halves' sums first.  Columns 4 c .. 4 c + 3 of all rows lie together: a warp's stores are whole lines.
             float* const s_l = sL + x * 128 + (tid & 127);
-            if (H == 2) {
-                if (half == 1) *s_l = l;
-                named_bar_sync(pair, 64);
-                if (half == 0) l += *s_l;
-            }
-            const int qt = qt0 + (ROWS2 ? x : 0);
+            if (half == 1) *s_l = l;
+            named_bar_sync(pair, 64);
+            if (half == 0) l += *s_l;
             const size_t slot = (size_t(uc) * p.tiles + qt) * p.splits + split;
-            const int c0 = half * (D / 4 / H);  // first 16-byte column
+            const int c0 = half * (D / 8);  // first 16-byte column
             float4* const out = reinterpret_cast<float4*>(p.o) + (slot * (D / 4) + c0) * 128 + row;
             float4* const other = reinterpret_cast<float4*>(sRing) + c0 * 128 + row;  // the second softmax's O, [D / 4][128]
-            const bool join = !ROWS2 && n_tiles > 1;
-            const int all_threads = 64 * H * n_warps;
+            const bool join = n_tiles > 1;
+            const int all_threads = 128 * n_warps;
             if (join && x == 1) {
                 named_bar_sync(9, all_threads);  // both softmaxes' last products are done: nothing reads the ring; the maxima are read
 #pragma unroll 1
-                for (int c = 0; c < D / (32 * H); ++c) {
+                for (int c = 0; c < D / 64; ++c) {
                     uint32_t v[32];
                     tmem_ld_x32(t_o + c * 32, v);
                     tmem_wait_ld();
@@ -378,7 +344,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
                 if (half == 0) sMl[row] = make_float2(m_ref, l);
                 named_bar_sync(9, all_threads);
-            } else if (ROWS2 || x == 0) {
+            } else if (x == 0) {
                 float f0 = 1.f, f1 = 0.f;
                 if (join) {
                     named_bar_sync(9, all_threads);
@@ -393,7 +359,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 ok = ok && *abort_flag == 0;
                 if (mine > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < D / (32 * H); ++c) {
+                    for (int c = 0; c < D / 64; ++c) {
                         uint32_t v[32];
                         tmem_ld_x32(t_o + c * 32, v);
                         tmem_wait_ld();
@@ -416,7 +382,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     // teardown: every role comes here, also after a wait that gave up
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == MMA) {
+    if (warp == 17) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }

@@ -27,16 +27,15 @@ inline int divisor(int n, int most) {
 // How the prompts' rows and keys are dealt (attn_prefix.cuh), and the decode behind
 struct PrefixPlan {
     int heads, n_chunks, seqs, tiles, splits;
-    int blocks;       // CTAs side by side per chunk: pairs of tiles, or the one tile
     long long units;  // tiles of rows of all prompts, KV heads and chunks
     long long grid;
     DecodePlan decode;
     size_t decode_bytes, bytes;  // of the workspace: the decode's own, all
     size_t slots;
 };
-// The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others: SMs are shared out by the bytes to
-// be read, those of a prompt with more than 128 rows counted half as much again, because the prompts' kernel is then bound by its
-// products and exponentials (B=64 P=16384 L=256 16/4 D=128, prompts on 48 / 72 / 96 SMs: 37.7 / 32.5 / 31.4 us).
+// The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others, and both are bound by HBM or, when
+// short, by latency: SMs are shared out by the bytes to be read, those of a prompt with more than 128 rows, which several CTAs read, counted
+// twice (B=64 P=16384 L=256 16/4 D=128, prompts on 48 / 72 / 96 / 104 / 120 SMs: 35.4 / 29.9 / 27.6 / 27.1 / 36.8 us).
 PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool ragged) {
     PrefixPlan d;
     const int group = Hq / Hkv, n = B / G, sms = sm_count();
@@ -45,13 +44,11 @@ PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool 
     d.seqs = std::min(n, 128 / d.heads);
     d.tiles = (n + d.seqs - 1) / d.seqs;
     d.units = (long long)G * Hkv * d.n_chunks * d.tiles;
-    d.blocks = (d.tiles + 1) / 2;
-    const long long ctas = (long long)G * Hkv * d.n_chunks * d.blocks;
     const int all = (P + kPrefixKeys - 1) / kPrefixKeys;
-    const double keys = (double)G * P * (d.tiles > 1 ? 1.5 : 1.0), own = (double)B * L;
+    const double keys = (double)G * P * (d.tiles > 1 ? 2.0 : 1.0), own = (double)B * L;
     const int share = std::max(1, (int)(sms * keys / (keys + own)));
-    d.splits = (int)std::max<long long>(1, std::min<long long>(all, share / ctas));
-    d.grid = ctas * d.splits;
+    d.splits = (int)std::max<long long>(1, std::min<long long>(all, share / d.units));
+    d.grid = d.units * d.splits;
     d.slots = (size_t)d.units * d.splits;
     const int left = d.grid < sms ? sms - (int)d.grid : sms;
     d.decode = decode_plan(B, L, Hq, Hkv, D, 0, ragged, std::min(2 * left, kDecodeMaxCtas), true);
@@ -64,13 +61,13 @@ bool shared_sizes_ok(int B, int G, int P, int L, int Hq, int Hkv, int D) {
     return B > 0 && G > 0 && B % G == 0 && P > 0 && L > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128);
 }
 
-template <int D, bool ROWS2>
+template <int D>
 int launch_prefix(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const PrefixParams& p, unsigned grid, cudaStream_t st) {
-    constexpr int smem = PrefixCfg<D, ROWS2>::kSmemBytes;
+    constexpr int smem = PrefixCfg<D>::kSmemBytes;
     static bool set[kMaxDevices] = {false};
-    const int rc = set_smem_once(attn_prefix_kernel<D, ROWS2>, smem, set);
+    const int rc = set_smem_once(attn_prefix_kernel<D>, smem, set);
     if (rc) return rc;
-    if (launch_pdl(attn_prefix_kernel<D, ROWS2>, dim3(grid), PrefixCfg<D, ROWS2>::kThreads, smem, st, tq, tk, tv, p) != cudaSuccess) {
+    if (launch_pdl(attn_prefix_kernel<D>, dim3(grid), kPrefixThreads, smem, st, tq, tk, tv, p) != cudaSuccess) {
         cudaGetLastError();
         return B200ATTN_ERR_CUDA;
     }
@@ -175,7 +172,7 @@ extern "C" int b200attn_decode_shared(const void* q, const void* kprefix, const 
     PrefixParams p = {};
     p.P = P, p.n = B / G, p.heads = x.heads, p.seqs = x.seqs, p.group = Hq / Hkv, p.n_chunks = x.n_chunks, p.Hkv = Hkv;
     p.splits = x.splits, p.tiles = x.tiles;
-    p.div_splits = fastdiv_make((unsigned)x.splits), p.div_blocks = fastdiv_make((unsigned)x.blocks);
+    p.div_splits = fastdiv_make((unsigned)x.splits), p.div_tiles = fastdiv_make((unsigned)x.tiles);
     p.div_chunks = fastdiv_make((unsigned)x.n_chunks), p.div_hkv = fastdiv_make((unsigned)Hkv);
     p.lens = prefix_lens;
     p.scale_log2 = dp.scale_log2;
@@ -191,8 +188,7 @@ extern "C" int b200attn_decode_shared(const void* q, const void* kprefix, const 
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const unsigned grid = (unsigned)x.grid;
-    if (D == 64) rc = x.tiles > 1 ? launch_prefix<64, true>(tq, tkp, tvp, p, grid, st) : launch_prefix<64, false>(tq, tkp, tvp, p, grid, st);
-    else rc = x.tiles > 1 ? launch_prefix<128, true>(tq, tkp, tvp, p, grid, st) : launch_prefix<128, false>(tq, tkp, tvp, p, grid, st);
+    rc = D == 64 ? launch_prefix<64>(tq, tkp, tvp, p, grid, st) : launch_prefix<128>(tq, tkp, tvp, p, grid, st);
     if (!rc) rc = launch_decode<kDecodeShared>(D, tk, tv, dp, d.n_ctas, st);
     return rc;
 }

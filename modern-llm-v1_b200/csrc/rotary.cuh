@@ -11,7 +11,10 @@
 // Bound by HBM like rope_norm.cuh, whose deal of the work this is: a lane owns 8 elements of a row, a warp 256 / D tokens and a chunk of
 // heads, so that a token's cosines and sines stay in registers.  Where the halves are paired a lane's 8 elements are four pairs, two
 // pieces of four R / 2 apart (R is a multiple of 16); behind R they are two pieces side by side.  (Eight elements in a row, with the
-// partners by shuffle, took twice the registers for the tables and 8 shuffles a row: XX.)
+// partners by shuffle, took twice the registers for the tables and 8 to 16 shuffles a row: backward with the norm, BF16 B=4 T=8192 16/4
+// D=128, 122.8 us instead of 105.8.)  Measured, q and k together: that backward 4.8 TB/s (interleaved 100 us); FP32 forward with the norm,
+// B=16 T=1024 16/4 D=64 R=32, 23.4 us, 5.4 TB/s; one token 4 us, a launch.  More rows in flight (3 or 4 instead of 2), 2 or 4 CTAs per SM
+// instead of 3: all slower (102.6 -> 105 to 130).
 #pragma once
 
 #include "rope_norm.cuh"

@@ -68,21 +68,20 @@ static int key_weights(std::mt19937& rng) {
 }
 
 static int prefix() {
-    for (int ahead = 1; ahead <= 2; ++ahead)
-        for (int n = 1; n < 40; ++n) {
-            int i = 0;  // the products: S of the first tiles, then P V of tile j and S of tile j + ahead
-            auto next = [&](bool k, int j) {
-                int lj;
-                const bool lk = prefix_load_at(i, n, ahead, &lj);
-                return lk == k && lj == j && i++ == (k ? prefix_k_at(j, ahead) : prefix_v_at(j, n, ahead));
-            };
-            for (int j = 0; j < ahead && j < n; ++j) CHECK(next(true, j));
-            for (int j = 0; j < n; ++j) {
-                CHECK(next(false, j));
-                if (j + ahead < n) CHECK(next(true, j + ahead));
-            }
-            CHECK(i == 2 * n);
+    for (int n = 1; n < 40; ++n) {
+        int i = 0;  // the products: S of the first two tiles, then P V of tile j and S of tile j + 2
+        auto next = [&](bool k, int j) {
+            int lj;
+            const bool lk = prefix_load_at(i, n, &lj);
+            return lk == k && lj == j && i++ == (k ? prefix_k_at(j) : prefix_v_at(j, n));
+        };
+        for (int j = 0; j < 2 && j < n; ++j) CHECK(next(true, j));
+        for (int j = 0; j < n; ++j) {
+            CHECK(next(false, j));
+            if (j + 2 < n) CHECK(next(true, j + 2));
         }
+        CHECK(i == 2 * n);
+    }
     return 0;
 }
 
