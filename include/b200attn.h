@@ -325,12 +325,13 @@ int b200attn_kv_append_rotary(const void* xq, const void* xk, const void* xv, in
  *
  * b200attn_decode_weights: b200attn_decode_ragged that also adds every key's probability to its weight:
  *   weights[b, hk, key] += sum over the heads h of the group of exp(scale q_h . k_key - lse_h),  weights [B, Hkv, L_cap] FP32, keys
- *   0 .. lens[b] - 1 (lens clamped to 1 .. L; NULL: L).  lse may be NULL.  Rows beyond a sequence's length may hold anything.
+ *   0 .. lens[b] - 1 (lens clamped to 1 .. L; NULL: L).  lse may be NULL.  Rows beyond a sequence's length may hold anything.  The
+ *   workspace holds the scores, 4 B Hq L bytes.
  *
  * b200attn_key_weights: the same sums over a chunk of T new tokens at positions (rows) pos0 .. pos0 + T - 1 of the cache, each of
  *   which sees the keys up to its own, from the lse [B, Hq, T] that b200attn_fwd_kvcache_at has left; q [.., T, ..] in q_layout.
  *   Keys 0 .. pos0 + T - 1.  new_lens: [B] (device, int32), of the T rows of each sequence those that count (the first ones, of a padded
- *   batch), or NULL: all.  For the sums over the last tokens of a prompt only, pass these tokens' q, lse and position.
+ *   batch; the others may hold anything), or NULL: all.  For the sums over the last tokens of a prompt only, pass these tokens' q, lse and position.
  *
  * b200attn_kv_evict: of each (batch, KV head)'s first n = lens[b] rows (clamped to 0 .. L; NULL: L) min(n, keep) stay: the rows whose
  *   position is above newest - recent (the newest being the largest of the n positions, which are distinct; recent <= keep), then those of

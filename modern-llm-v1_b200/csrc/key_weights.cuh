@@ -13,6 +13,8 @@
 // (columns), so that a key's sum runs inside a thread and needs no exchange.
 #pragma once
 
+#include <limits.h>
+
 #include "attn_decode.cuh"
 #include "ptx.cuh"
 
@@ -349,9 +351,11 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int first = u0 + i - it.start, m = min(it.units - first, n - i);
             float acc = 0.f;
             const int k_lim = it.kt * 128 + key - p.pos0;  // tokens below it do not see the key
+            const int rows = p.rows ? __ldg(p.rows + it.bh / p.Hkv) : INT_MAX;
             for (int e = (wg - i % NG + NG) % NG; e < m; e += NG) {
                 int hc;
-                const int k = i + e, lim = k_lim - unit_qt(first + e, &hc) * p.tokens;
+                const int k = i + e, t_first = unit_qt(first + e, &hc) * p.tokens, lim = k_lim - t_first;
+                const bool padding = t_first + p.tokens > rows;  // some query rows do not count: whatever they hold
                 const bool diagonal = lim + 127 - key > 0;  // whether any key of the tile is unseen by the unit's first token
                 const float* lse = sLse + (wg * 2 + (k / NG & 1)) * 128;
                 ok = mbar_wait_warp(&bar_s_full[wg], uint32_t(k / NG) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
@@ -360,6 +364,11 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 uint64_t sum2[2] = {0ull, 0ull};
                 uint32_t v[2][16];
                 auto chunk = [&](int c, uint32_t (&v)[16]) {
+                    if (padding) {
+#pragma unroll
+                        for (int x = 0; x < 16; ++x)
+                            if (t_first + sTok[c * 16 + x] >= rows) v[x] = 0u;
+                    }
                     if (diagonal) {
                         if (p.heads == 1) {  // (column = token)
                             if (lim > c * 16) {

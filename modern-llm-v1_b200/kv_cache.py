@@ -43,7 +43,7 @@ def kv_evict(kcache, vcache, weights, positions, weights_out, positions_out, B, 
 class KVCache:
     # the reference's rotation, a cache of its own, no weights
     _plain, prefix, track_weights = True, None, False
-    _shift, _pos, _evicted = 0, None, False
+    _shift, _pos, _evicted, _prompts = 0, None, False, None
 
     def __init__(self, n_layers: int, B: int, Hq: int, Hkv: int, D: int, L_cap: int, device="cuda",
                  rope_base: float = 10000.0, eps: float = 1e-5, *, rotary_dim=None, pairs="interleaved", scaling="none",
@@ -119,7 +119,7 @@ class KVCache:
         """Forgets every token (the buffers keep their bytes; rows >= length are never read)."""
         self.length = 0
         self.lengths = self._lens_next = self._lengths_host = None
-        self._shift, self._pos, self._evicted = 0, None, False
+        self._shift, self._pos, self._evicted, self._prompts = 0, None, False, None
         if self.track_weights:
             for w, p in zip(self.weights, self.positions):
                 w.zero_()
@@ -128,12 +128,14 @@ class KVCache:
     def _place(self):
         """(first position, positions or None, rows or None) of the next tokens; behind prompts of different lengths they are made when
         the first token comes"""
-        if self.prefix is not None and self.length == 0 and self._pos is None:
+        if self.prefix is not None and self._prompts is None:
             if self.prefix.length == 0:
                 raise ValueError("KVCache: the prompts are empty")
-            self._shift = self.prefix.length
+            self._shift, self._prompts = self.prefix.length, (self.prefix.length, self.prefix.lengths)
             if self.prefix.lengths is not None:
                 self._pos = self.prefix.lengths.repeat_interleave(self.B // self.prefix.B)
+        elif self.prefix is not None and (self.prefix.length != self._prompts[0] or self.prefix.lengths is not self._prompts[1]):
+            raise ValueError("KVCache: the prompts have changed since their first continuation (reset this cache)")
         return self.length + self._shift, self._pos, self.lengths
 
     @property
@@ -169,7 +171,7 @@ class KVCache:
         pos0, pos, rows = self._place()
         if rows is not None and pos is None:
             pos = rows if self._shift == 0 else rows + self._shift
-        if rows is not None and xq.dim() == 4 and xq.shape[1] != 1:
+        if rows is not None and isinstance(xq, torch.Tensor) and xq.dim() == 4 and xq.shape[1] != 1:
             raise ValueError("KVCache.append: one token per sequence once the lengths differ")
         _lib.host().append_rotary(xq, xk, xv, gamma_q, gamma_k, q_out, self._kl[layer], self._vl[layer],
                                   self.positions[layer] if self.track_weights else None, self.cos, self.sin, self._R, self._pairs, pos, pos0,

@@ -198,6 +198,27 @@ def test_key_weights(B, T, pos0, Hq, Hkv, D, layout):
     assert torch.equal(w, first)  # a call repeats bit for bit
 
 
+def test_key_weights_of_a_padded_batch():
+    """rows of padding, NaN in q and lse, count for nothing: every sequence's weights are those that it gets alone"""
+    B, T, pos0, Hq, Hkv, D = 4, 300, 40, 4, 2, 64
+    g = torch.Generator().manual_seed(7)
+    q, k = randn(g, B, Hq, T, D), randn(g, B, Hkv, pos0 + T, D)
+    lens = [300, 1, 130, 0]
+    lse = torch.rand((B, Hq, T), generator=g) + 6
+    for b, n in enumerate(lens):
+        q[b, :, n:], lse[b, :, n:] = NAN, NAN
+    w = torch.zeros((B, Hkv, pos0 + T), device="cuda")
+    m.flash_attn_key_weights(q.cuda(), k.cuda(), lse.cuda(), w, B, T, pos0, Hq, Hkv, D, new_lens=torch.tensor(lens, dtype=I32, device="cuda"))
+    for b, n in enumerate(lens):
+        one = torch.zeros((1, Hkv, pos0 + T), device="cuda")
+        if n:
+            m.flash_attn_key_weights(q[b:b + 1, :, :n].contiguous().cuda(), k[b:b + 1].cuda(), lse[b:b + 1, :, :n].contiguous().cuda(), one, 1, n, pos0, Hq, Hkv, D,
+                                     L_cap=pos0 + T)
+        # the same terms in other groups: at most 32 + 2 * 300 / 32 + 150 additions each way
+        assert ((w[b] - one[0]).abs() <= 2 * 201 * 2.0**-24 * one[0]).all()
+    m.device_status()
+
+
 def test_the_weights_of_a_prompt_are_those_of_its_tokens():
     """a prompt at once and token by token; each token hands out one unit of weight per head of the group"""
     B, T, Hq, Hkv, D = 2, 70, 6, 2, 64

@@ -101,8 +101,14 @@ def test_sequences_that_share_prompts_are_those_that_hold_them(lens, own):
     m.device_status()
     with pytest.raises(ValueError, match="exceed the capacity"):
         step(samples, 0, tokens(g, G * n, 1, Hq, Hkv, D), gammas)
+    prompts.reset()
+    with pytest.raises(ValueError, match="prompts have changed"):
+        samples.next_position
+    for i in range(layers):
+        step(prompts, i, tokens(g, G, T, Hq, Hkv, D), gammas)
+    prompts.advance(T)
     samples.reset()
-    assert samples.length == 0
+    assert samples.length == 0 and samples.next_position == T
     with pytest.raises(ValueError, match="one token per sequence"):
         step(samples, 0, tokens(g, G * n, 2, Hq, Hkv, D), gammas)
 
