@@ -6,7 +6,7 @@
 // Large caches are bound by HBM (every K and V byte is read exactly once), small ones by latency.  A unit is one
 // (batch, KV head, chunk of at most 16 query heads of the group): all its query heads are served from the same K/V tile,
 // which is the bandwidth win of GQA.  One launch does everything; it deals the units' tiles in one of two ways
-// (decode_plan in b200attn_api.cu chooses):
+// (decode_plan in decode_plan.h chooses), or, behind shared prompts, whole units as CTAs come to them (decode_next_unit):
 //  * shares: a unit's tiles are split evenly over 1, 2, 4 or 8 CTAs, a cluster, which exchange their partial results
 //    through distributed shared memory, each CTA finishing a slice of the outputs.  (A caller may ask for any other number of
 //    shares; their partial results go through the workspace as in the next deal.)
@@ -44,7 +44,8 @@ namespace b200attn {
 // its softmax goes on over the partial results of a prompt that several sequences share (attn_prefix.cuh).  In the latter two, rows
 // beyond a sequence's length may hold anything, NaN included: their V rows are cleared in shared memory (one tile of a sequence; in
 // the plain kernel, whose caches hold finite values everywhere, that would cost the tile for nothing).
-enum { kDecodePlain = 0, kDecodeScores = 1, kDecodeShared = 2 };
+// kDecodeSharedTurn: kDecodeShared in a deal of its own, see DecodeParams::turn.
+enum { kDecodePlain = 0, kDecodeScores = 1, kDecodeShared = 2, kDecodeSharedTurn = 3 };
 
 // The partial results of attn_prefix.cuh: per (prompt, KV head, chunk of the group's heads, tile of 128 rows) and split a slot of 128
 // rows, a row being (sequence within the prompt's, head within the chunk).
@@ -55,7 +56,7 @@ struct DecodePrefix {
     FastDiv div_n;     // sequences per prompt
     FastDiv div_heads, div_seqs;  // heads per chunk, sequences per tile
     int n_chunks, Hkv;
-    // In the deal by ranges a CTA first goes through all its pieces, whose results it leaves here (un-normalised O [B, Hq, D], (m, l)
+    // A CTA with several pieces goes through all of them first, whose results it leaves here (un-normalised O [B, Hq, D], (m, l)
     // [B, Hq]), and joins them with the prompts' at its end: waiting for those at the first piece would hold up the others.
     float* own_o;
     float2* own_ml;
@@ -71,6 +72,7 @@ struct DecodeParams {
     int cluster;        // CTAs per cluster: shares where they exchange through distributed shared memory, else 1
     int whole;          // ranges: they begin and end at unit boundaries (all sequences have length L)
     int slot_mode;      // where a shared unit's pieces lie in the workspace, see decode_slot
+    int turn, units;    // kDecodeSharedTurn: CTAs that begin with the unit of their number; units
     float scale, scale_log2;
     const int* lens;    // [B] cache length per sequence (1 <= lens[b]; clamped to L), or nullptr: every sequence has L
     const uint16_t* q;  // [B, Hq, D]
@@ -80,7 +82,7 @@ struct DecodeParams {
     float* part_m;      // [slot][G]     row maximum, raw score units
     float* part_l;      // [slot][G]     sum of exp2((s - m) * scale_log2)
     unsigned long long* counters;  // one per CTA, see decode_count: pieces finished of the shared unit that begins in that CTA
-                                   // (not where a cluster shares it)
+                                   // (not where a cluster shares it); kDecodeSharedTurn: one, see decode_next_unit
     unsigned long long tag;        // of this launch
     int* status;                   // status word and epoch
     float* scores;                 // kDecodeScores: [unit][L][G] in raw score units
@@ -88,6 +90,7 @@ struct DecodeParams {
 };
 
 constexpr int kDecodeMaxCtas = 320, kDecodeMaxCluster = 8, kDecodeThreads = 192;
+constexpr int kDecodeTurnList = kDecodeMaxCluster * 32;  // units that a CTA finishes before it joins them with the prompts' results
 // Workspace slot of CTA c's piece of a shared unit: one per tile when there are as many slots (mode 0), one per CTA in the deal
 // by shares (mode 1), else two per CTA (mode 2: a range may end one shared unit and begin another).
 enum { kDecodeSlotTile = 0, kDecodeSlotCta = 1, kDecodeSlotTwo = 2 };
@@ -156,6 +159,17 @@ __host__ __device__ __forceinline__ int decode_len(const DecodeParams& p, int b)
 #else
     return p.lens ? std::max(1, std::min(p.lens[b], p.L)) : p.L;
 #endif
+}
+// A whole unit
+template <int KEYS>
+__device__ __forceinline__ void decode_walk_unit(const DecodeParams& p, DecodeWalk& w, int unit) {
+    w.b = int(fastdiv(unit, p.div_units));
+    w.u = unit - w.b * p.units_per_seq;
+    w.len = decode_len(p, w.b);
+    w.n_tiles = (w.len + KEYS - 1) / KEYS;
+    w.t = w.j0 = w.cta0 = 0;
+    w.t_end = w.total = w.n_tiles;
+    w.n_ctas = 1;
 }
 // First tile of CTA c's range, and the CTA whose range holds tile t.
 __host__ __device__ __forceinline__ int decode_range(const DecodeWalk& w, int c) {
@@ -423,6 +437,24 @@ __device__ __forceinline__ int decode_count(unsigned long long* word, unsigned l
     return int(atomicAdd(word, 1ull) - tag) + 1;
 }
 
+// kDecodeSharedTurn: the number of the next unit, counted in a word of the same kind, but for a longer count and a shorter tag.  Every CTA
+// asks until it is told one beyond the last; whoever is the last to be told so puts the count back to zero.  A unit's result does not depend
+// on who takes it.
+constexpr int kDecodeTurnBits = 24;
+constexpr int kDecodeTurnUnits = (1 << kDecodeTurnBits) - kDecodeMaxCtas;
+__device__ __forceinline__ int decode_next_unit(const DecodeParams& p, unsigned epoch, bool first, int n_ctas) {
+    const unsigned long long tag = ((p.tag >> kDecodeCountBits) + epoch) << kDecodeTurnBits;
+    int n = -1;
+    if (first) {
+        const unsigned long long seen = decode_ld_acquire(p.counters);
+        if ((seen >> kDecodeTurnBits) != (tag >> kDecodeTurnBits) && atomicCAS(p.counters, seen, tag + 1) == seen) n = 0;
+    }
+    if (n < 0) n = int(atomicAdd(p.counters, 1ull) - tag);
+    n += p.turn;
+    if (n == p.units + n_ctas - 1) *p.counters = tag;
+    return n < p.units ? n : -1;
+}
+
 // Where the prompt's partial results of head j of the group (of sequence b, KV head hk) lie: its row in the first split's slot
 __device__ __forceinline__ size_t decode_prefix_row(const DecodePrefix& x, int b, int hk, int j, int* row) {
     const int prompt = int(fastdiv(b, x.div_n)), seq = b - prompt * int(x.div_n.d);
@@ -500,12 +532,74 @@ __device__ __forceinline__ void decode_join_unit(const DecodeParams& p, const De
     }
 }
 
+// The same for the n units of a list, in kDecodeSharedTurn.  Of prompts in one or two splits, four elements' loads are issued together.
+template <int D, int KEYS>
+__device__ __forceinline__ void decode_join_units(const DecodeParams& p, const int* list, int n, int tid) {
+    const DecodePrefix& x = p.prefix;
+    const int per = p.G * (D / 4), total = n * per;
+    DecodeWalk w;
+    if (x.splits > 2) {
+        for (int k = 0; k < n; ++k) {
+            decode_walk_unit<KEYS>(p, w, list[k]);
+            decode_join_unit<D>(p, w, tid);
+        }
+        return;
+    }
+    const int status = *reinterpret_cast<volatile int*>(p.status);
+    constexpr int E = 4;
+    for (int i0 = tid; i0 < total; i0 += 128 * E) {
+        float4 own[E], po[E][2];
+        float2 ml[E], pml[E][2];
+        size_t at[E];
+        int col[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = min(i0 + e * 128, total - 1), k = i / per, r = i - k * per, c = r / p.G, g = r - c * p.G;
+            const int unit = list[k], b = int(fastdiv(unit, p.div_units)), u = unit - b * p.units_per_seq;
+            const int hk = int(fastdiv(u, p.div_chunks)), j = (u - hk * p.n_chunks) * p.G + g;
+            at[e] = size_t(b) * p.Hq + hk * p.group + j, col[e] = c;
+            own[e] = __ldcg(reinterpret_cast<const float4*>(x.own_o + at[e] * D) + c);
+            ml[e] = __ldcg(x.own_ml + at[e]);
+            int row;
+            const size_t slot0 = decode_prefix_row(x, b, hk, j, &row);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const size_t slot = slot0 + min(s, x.splits - 1);
+                pml[e][s] = __ldcg(x.ml + slot * 128 + row);
+                po[e][s] = __ldcg(reinterpret_cast<const float4*>(x.o + (slot * (D / 4) + c) * 512 + row * 4));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (i0 + e * 128 >= total || status != 0) break;
+            if (x.splits < 2) pml[e][1] = make_float2(-INFINITY, 0.f);
+            const float m = fmaxf(ml[e].x, fmaxf(pml[e][0].x, pml[e][1].x));
+            const float f = ml[e].x == -INFINITY ? 1.f : ex2_approx((ml[e].x - m) * p.scale_log2);
+            float l = ml[e].y * f, a[4] = {own[e].x * f, own[e].y * f, own[e].z * f, own[e].w * f};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const bool any = !(pml[e][s].x == -INFINITY && pml[e][s].y == 0.f);
+                const float fs = pml[e][s].x == -INFINITY ? 1.f : ex2_approx((pml[e][s].x - m) * p.scale_log2);
+                l += fs * pml[e][s].y;
+                a[0] += any ? fs * po[e][s].x : 0.f;
+                a[1] += any ? fs * po[e][s].y : 0.f;
+                a[2] += any ? fs * po[e][s].z : 0.f;
+                a[3] += any ? fs * po[e][s].w : 0.f;
+            }
+            const float inv = 1.f / l;
+            reinterpret_cast<uint2*>(p.o)[at[e] * (D / 4) + col[e]] = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
+            if (p.lse && col[e] == 0) p.lse[at[e]] = m * p.scale + logf(l);
+        }
+    }
+}
+
 // PF: tiles that a CTA brings into L2 while the kernel in front of this one ends
 template <int D, int NH, int PF, int MODE = kDecodePlain>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
 attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const DecodeParams p) {
     using Cfg = DecodeCfg<D>;
+    constexpr bool TURN = MODE == kDecodeSharedTurn, SHARED = TURN || MODE == kDecodeShared;
     constexpr int KEYS = Cfg::kKeys;
     constexpr int NST = Cfg::kStages;
     constexpr int KS = D / 16;     // k-steps of Q K^T
@@ -528,6 +622,8 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     volatile int* last_flag = abort_flag + 1;
     volatile int* fail_flag = abort_flag + 2;
     volatile int* epoch = abort_flag + 3;
+    volatile int* turn_unit = abort_flag + 4;                            // [2] kDecodeSharedTurn: the unit whose q rows lie in buffer 0 / 1, or -1: no more
+    int* turn_list = reinterpret_cast<int*>(sXMl);                       // (there are no clusters then)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = p.G;
@@ -550,11 +646,24 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         __syncwarp();
         // everything above overlaps the previous kernel's end (the cache append that wrote q and the newest K / V row)
-        if (MODE != kDecodeShared) grid_dep_wait();
-        DecodeWalk w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane);
+        if (!SHARED) grid_dep_wait();
+        DecodeWalk w;
         int j = 0;  // tiles issued so far (ring position)
         bool synced = false, ok = true;
-        for (int n = 0; w.t < w.t_end && ok; ++n) {
+        int unit = -1, next = -1, n = 0;
+        unsigned turn_epoch = 0;
+        if constexpr (TURN) {
+            turn_epoch = *reinterpret_cast<volatile unsigned*>(p.status + 1);
+            const bool first = int(blockIdx.x) < p.turn;
+            if (lane == 0) unit = first ? int(blockIdx.x) : decode_next_unit(p, turn_epoch, true, int(gridDim.x));
+            unit = __shfl_sync(0xffffffffu, unit, 0);
+            if (lane == 0 && unit >= 0) next = decode_next_unit(p, turn_epoch, first, int(gridDim.x));
+            w.t = 0, w.t_end = unit >= 0;
+            if (unit >= 0) decode_walk_unit<KEYS>(p, w, unit);
+        } else {
+            w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane);
+        }
+        for (; w.t < w.t_end && ok; ++n) {
             const int tiles = decode_piece(w);
             const int hk = int(fastdiv(w.u, p.div_chunks)), h0 = hk * p.group + (w.u - hk * p.n_chunks) * G;
             for (int i = 0; i < tiles; ++i, ++j) {
@@ -581,29 +690,48 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         if (!ok) break;
                     }
                     if (elect_one()) {
+                        if (TURN) turn_unit[n & 1] = unit;
                         mbar_arrive_expect_tx(&bar_q[n & 1], G * D * 2);
                         bulk_load_1d(sQ + (n & 1) * Cfg::kQBytes, p.q + (size_t(w.b) * p.Hq + h0) * D, G * D * 2, &bar_q[n & 1]);
                     }
                     __syncwarp();
                 }
             }
-            decode_walk_next<KEYS>(p, w, tiles);
+            if constexpr (TURN) {  // the next one, which was asked for a unit ago, and another
+                unit = __shfl_sync(0xffffffffu, next, 0);
+                w.t = 0, w.t_end = unit >= 0;
+                if (unit >= 0) {
+                    decode_walk_unit<KEYS>(p, w, unit);
+                    if (lane == 0 && ok) next = decode_next_unit(p, turn_epoch, false, int(gridDim.x));
+                }
+            } else {
+                decode_walk_next<KEYS>(p, w, tiles);
+            }
         }
         if (!synced) decode_started();
+        if (TURN && ok) {
+            if (n >= 2) ok = mbar_wait_warp(&bar_q_free[n & 1], ((n >> 1) - 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_FREE);
+            if (ok && elect_one()) {
+                turn_unit[n & 1] = -1;
+                mbar_arrive(&bar_q[n & 1]);
+            }
+        }
         return;
     }
 
+    // whether results are left for the CTA's end (the counter's piece is the last thing that it does)
+    bool defer = SHARED && p.prefix.own_o && warp != 5;
     auto write_rows_of = [&](const DecodeWalk& w) {  // final rows of the unit at w
         const int hk = int(fastdiv(w.u, p.div_chunks));
         const int j0 = (w.u - hk * p.n_chunks) * G, b = w.b;
         const size_t row0 = size_t(b) * p.Hq + hk * p.group + j0;
-        return [&p, row0, b, hk, j0, warp](int g, int d, float a0, float a1, float m, float l) {
-            if (MODE == kDecodeShared && p.prefix.own_o && warp != 5) {  // (the counter's piece is the last thing that it does)
+        return [&p, row0, b, hk, j0, defer](int g, int d, float a0, float a1, float m, float l) {
+            if (SHARED && defer) {
                 *reinterpret_cast<float2*>(p.prefix.own_o + (row0 + g) * D + d) = make_float2(a0, a1);
                 if (d == 0) p.prefix.own_ml[row0 + g] = make_float2(m, l);
                 return;
             }
-            if (MODE == kDecodeShared) {
+            if (SHARED) {
                 grid_dep_wait();
                 float a[2] = {a0, a1};
                 if (!decode_add_prefix<D, 2>(p, b, hk, j0 + g, d, a, m, l)) return;
@@ -632,7 +760,11 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 __syncwarp();
             });
         }
-        if (MODE != kDecodeShared) grid_dep_wait();
+        if (!SHARED) grid_dep_wait();
+        if (TURN) {
+            named_bar_sync(kDecodeCountBar, kDecodeThreads);
+            return;
+        }
         const DecodeWalk w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane);
         named_bar_sync(kDecodeCountBar, kDecodeThreads);
         if (p.shares || *fail_flag != 0 || w.t >= w.t_end) return;
@@ -662,26 +794,36 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const int buf = i / ((16 - G) * (D / 8)), r = i % ((16 - G) * (D / 8));
         *reinterpret_cast<uint4*>(sQ + buf * Cfg::kQBytes + (G + r / (D / 8)) * Cfg::kQRow + (r % (D / 8)) * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
-    if (MODE != kDecodeShared) grid_dep_wait();
+    if (!SHARED) grid_dep_wait();
     // (a launch behind a failure writes nothing; its loads are harmless, but shared memory has to outlive them)
     if (tid == 0) {
         *fail_flag = *reinterpret_cast<volatile int*>(p.status);
         *epoch = *reinterpret_cast<volatile int*>(p.status + 1);
     }
-    DecodeWalk w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane);
+    DecodeWalk w = {};
+    if constexpr (!TURN) w = decode_walk_start<KEYS>(p, int(blockIdx.x), int(gridDim.x), lane);
     decode_started();
     const bool failed = *fail_flag != 0;
     bool ok = true;
     const int rank = p.cluster > 1 ? int(blockIdx.x) % p.cluster : 0;
     const DecodeWalk w_first = w;  // (kDecodeShared)
+    int listed = 0;                // (kDecodeSharedTurn)
     bool sent = false, last_mine = false;
     int j = 0;  // tiles before this piece (ring position)
-    for (int n = 0; w.t < w.t_end; ++n) {
+    for (int n = 0; TURN || w.t < w.t_end; ++n) {
+        if (ok) ok = mbar_wait_warp(&bar_q[n & 1], (n >> 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
+        if constexpr (TURN) {
+            ok = decode_bar_ok(ok);
+            if (!ok) break;
+            const int unit = turn_unit[n & 1];
+            if (unit < 0) break;
+            decode_walk_unit<KEYS>(p, w, unit);
+            if (tid == 0 && defer) turn_list[listed] = unit;
+        }
         const int tiles = decode_piece(w);
         DecodeState<D, NH> st;
         st.clear();
         uint32_t bq[KS][NH][2];  // B fragments of Q^T (columns = heads)
-        if (ok) ok = mbar_wait_warp(&bar_q[n & 1], (n >> 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
         {
             const uint32_t q_base = smem_u32(sQ + (n & 1) * Cfg::kQBytes);
 #pragma unroll
@@ -825,7 +967,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             if (p.cluster > 1) break;  // (one piece)
             fence_proxy_async_smem();
             mbar_arrive(&bar_free[s_last]);
-            decode_walk_next<KEYS>(p, w, tiles);
+            if constexpr (!TURN) decode_walk_next<KEYS>(p, w, tiles);
             continue;
         }
         float* sO = reinterpret_cast<float*>(sKV + s_last * 2 * Cfg::kTileBytes);
@@ -842,7 +984,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             });
             sent = true;
             break;
-        } else if (tiles == w.n_tiles) {
+        } else if (TURN || tiles == w.n_tiles) {
             decode_merge<D, NH>(st, sO, sMl, warp, lane, tid, G, p.scale_log2, write_rows);
         } else {
             const int cta = int(blockIdx.x) - w.cta0;
@@ -893,9 +1035,23 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         fence_proxy_async_smem();
         mbar_arrive(&bar_free[s_last]);
         named_bar_sync(1, 128);  // sMl and the flag are rewritten at the next piece's end
-        decode_walk_next<KEYS>(p, w, tiles);
+        if constexpr (TURN) {
+            if (defer && ++listed == kDecodeTurnList) {  // (from here on the prompts' results are there)
+                grid_dep_wait();
+                decode_join_units<D, KEYS>(p, turn_list, listed, tid);
+                listed = 0;
+                defer = false;
+            }
+        } else {
+            decode_walk_next<KEYS>(p, w, tiles);
+        }
     }
-    if constexpr (MODE == kDecodeShared) {
+    if constexpr (TURN) {
+        if (ok && listed > 0) {  // the units that this CTA has finished; none behind a failure
+            grid_dep_wait();
+            decode_join_units<D, KEYS>(p, turn_list, listed, tid);
+        }
+    } else if constexpr (MODE == kDecodeShared) {
         if (p.prefix.own_o && ok && !failed) {  // the units that this CTA has finished
             named_bar_sync(1, 128);
             grid_dep_wait();

@@ -34,8 +34,11 @@ struct PrefixPlan {
     size_t slots;
 };
 // The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others, and both are bound by HBM or, when
-// short, by latency: SMs are shared out by the bytes to be read, those of a prompt with more than 128 rows, which several CTAs read, counted
-// twice (B=64 P=16384 L=256 16/4 D=128, prompts on 48 / 72 / 96 / 104 / 120 SMs: 35.4 / 29.9 / 27.6 / 27.1 / 36.8 us).
+// short, by latency: SMs are shared out by the keys to be gone through, once for every tile of a prompt's rows, and kUnitKeys more for each
+// unit of the decode's, its beginning and end.  (1 prompt x 64 samples, P=16384 L=256 16/4 D=128, all lengths the same, us with 0 / 128 / 192 /
+// 256 of them: 27.5 / 28.5 / 27.7 / 29.7; L=64: 39.4 / 27.8 / 26.9 / 27.9; 1 x 16 16000 100 32/8 128: 42.8 / 25.3 / 23.3 / 23.2; 8 x 16 2000 1
+// 16/4 64, the first token behind the prompts: 67.9 / 21.6 / 21.6 / 21.6.)
+constexpr int kUnitKeys = 192;
 PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool ragged) {
     PrefixPlan d;
     const int group = Hq / Hkv, n = B / G, sms = sm_count();
@@ -45,13 +48,13 @@ PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool 
     d.tiles = (n + d.seqs - 1) / d.seqs;
     d.units = (long long)G * Hkv * d.n_chunks * d.tiles;
     const int all = (P + kPrefixKeys - 1) / kPrefixKeys;
-    const double keys = (double)G * P * (d.tiles > 1 ? 2.0 : 1.0), own = (double)B * L;
-    const int share = std::max(1, (int)(sms * keys / (keys + own)));
-    d.splits = (int)std::max<long long>(1, std::min<long long>(all, share / d.units));
+    const double keys = (double)G * P * d.tiles, own = (double)B * (L + kUnitKeys);
+    d.splits = std::max(1, std::min(all, (int)(sms * keys / (keys + own) / d.units + 0.5)));
     d.grid = d.units * d.splits;
     d.slots = (size_t)d.units * d.splits;
     const int left = d.grid < sms ? sms - (int)d.grid : sms;
     d.decode = decode_plan(B, L, Hq, Hkv, D, 0, ragged, std::min(2 * left, kDecodeMaxCtas), true);
+    if (d.grid >= sms) d.decode.turn = d.decode.n_ctas;  // all of them start as the prompts' CTAs end
     d.decode_bytes = round256((size_t)B * Hq * d.decode.splits * (size_t)(D + 2) * sizeof(float));
     d.bytes = d.decode_bytes + (d.slots * 128 + (size_t)B * Hq) * (D + 2) * sizeof(float);
     return d;
@@ -189,7 +192,7 @@ extern "C" int b200attn_decode_shared(const void* q, const void* kprefix, const 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const unsigned grid = (unsigned)x.grid;
     rc = D == 64 ? launch_prefix<64>(tq, tkp, tvp, p, grid, st) : launch_prefix<128>(tq, tkp, tvp, p, grid, st);
-    if (!rc) rc = launch_decode<kDecodeShared>(D, tk, tv, dp, d.n_ctas, st);
+    if (!rc) rc = d.in_turn ? launch_decode<kDecodeSharedTurn>(D, tk, tv, dp, d.n_ctas, st) : launch_decode<kDecodeShared>(D, tk, tv, dp, d.n_ctas, st);
     return rc;
 }
 

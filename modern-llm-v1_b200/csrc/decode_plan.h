@@ -29,6 +29,8 @@ struct DecodePlan {
     int cluster;  // CTAs per cluster
     bool whole;   // ranges of whole units
     int n_ctas, slot_mode;
+    bool in_turn; // kDecodeSharedTurn
+    int turn;     // and DecodeParams::turn
 };
 
 // The deal (see attn_decode.cuh).
@@ -45,9 +47,17 @@ struct DecodePlan {
 // n_splits > 0 asks for that many shares per unit (at most 64, none empty): a cluster where it can have that size.
 constexpr long long kRangesBytes = 16ll << 20;
 constexpr int kSaturatingCtas = 60;
+constexpr long long kTurnBytes = 3ll << 18;
 
-// cap: CTAs that may run at once, or 0: as many as fit the device.  A decode behind a shared prompt (`shared`) is never dealt more CTAs than
-// that: they wait for the prompts' kernel at their ends.
+// cap: CTAs that may run at once, or 0: as many as fit the device.
+//
+// Behind shared prompts (`shared`, cap: CTAs on the SMs that the prompts' kernel leaves) the CTAs wait for the prompts' kernel at their ends.
+// More units than those CTAs, of at most kTurnBytes: each takes a whole unit, then the next that nobody has taken, and so do the CTAs that
+// start on the SMs which the prompts' kernel frees.  Longer units are dealt in ranges among cap CTAs, which come out more even.  (us, units of
+// different lengths up to L, ranges / in turn; G prompts x n samples, P, L, heads, D: 8 x 16 2000 300 16/4 64 25.7 / 21.7; 16 x 16 500 300 8/4
+// 64 45.0 / 28.3; 2 x 128 3000 250 32/8 128 97.0 / 61.1; 16 x 4 4000 256 16/8 64 75.1 / 41.6; 8 x 8 1000 100 16/16 64 114.7 / 31.3; units of
+// 512 KB 4 x 40 1000 2000 16/4 64 54.1 / 50.5; of 1 MB 2 x 20 2000 2000 32/8 128 57.9 / 58.7, 1 x 300 1000 4000 8/1 64 52.9 / 57.2; equal
+// lengths, whole units dealt beforehand / in turn: 4 x 64 8192 256 16/4 128 57.3 / 51.6, 1 x 64 16384 256 16/4 128 27.7 / 27.8.)
 inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits, bool ragged, int cap = 0, bool shared = false) {
     DecodePlan d;
     const int group = Hq / Hkv;
@@ -60,7 +70,16 @@ inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits
     d.shares = d.cluster = 1;
     d.whole = false;
     d.slot_mode = kDecodeSlotTile;
+    d.in_turn = shared && units > cap && units < kDecodeTurnUnits && unit_bytes <= kTurnBytes;
+    d.turn = 0;
     long long counters = 0;
+    if (d.in_turn) {
+        d.shares = 0;
+        d.slots = 0, d.splits = 1;  // no partial results: room for the counter
+        d.turn = cap;
+        d.n_ctas = (int)std::min<long long>(units, decode_max_ctas());
+        return d;
+    }
     if (n_splits > 0) {
         const int want = std::min(std::min(n_splits, n_128), 64), per = (n_128 + want - 1) / want;
         d.slots = d.shares = (n_128 + per - 1) / per;
@@ -126,6 +145,8 @@ inline int decode_fill(const DecodePlan& d, DecodeParams& p, CUtensorMap& tk, CU
     p.cluster = d.cluster;
     p.whole = d.whole;
     p.slot_mode = d.slot_mode;
+    p.turn = d.turn;
+    p.units = B * p.units_per_seq;
     p.scale = softmax_scale > 0.f ? softmax_scale : 1.f / sqrtf((float)D);
     p.scale_log2 = p.scale * 1.4426950408889634f;
     p.lens = lens;
@@ -168,7 +189,8 @@ constexpr int kPrefetchCtas = 128;
 // (Behind a shared prompt's kernel the loads themselves begin that early.)
 template <int MODE, int D, int NH>
 int launch_decode_heads(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p, int n_ctas, cudaStream_t st) {
-    if (MODE != kDecodeShared && n_ctas >= kPrefetchCtas) return launch_decode_pf<D, NH, MODE != kDecodeShared ? 2 : 0, MODE>(tk, tv, p, n_ctas, st);
+    constexpr bool behind_prompts = MODE == kDecodeShared || MODE == kDecodeSharedTurn;
+    if (!behind_prompts && n_ctas >= kPrefetchCtas) return launch_decode_pf<D, NH, behind_prompts ? 0 : 2, MODE>(tk, tv, p, n_ctas, st);
     return launch_decode_pf<D, NH, 0, MODE>(tk, tv, p, n_ctas, st);
 }
 template <int MODE>

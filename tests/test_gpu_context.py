@@ -92,6 +92,62 @@ def test_decode_shared(G, n, P, L, Hq, Hkv, D, plens, lens, slack):
     assert torch.equal(o2, o)
 
 
+@pytest.mark.parametrize("G,n,P,L,Hq,Hkv,D", [
+    (1, 20000, 4, 2, 4, 4, 64),        # hundreds of units of a sequence's own rows for each CTA
+    (64, 2, 256, 64, 16, 4, 64),       # more tiles of the prompts' rows than SMs
+    (36, 16, 200, 100, 16, 4, 128),    # almost as many
+    (8, 16, 2000, 300, 24, 1, 64),
+    (1, 320, 200, 3500, 8, 1, 64),     # long units
+    (2, 75, 900, 1, 4, 4, 128),
+])
+@pytest.mark.parametrize("ragged", [True, False])
+def test_shared_prompts_of_many_sequences(G, n, P, L, Hq, Hkv, D, ragged):
+    """more units of (sequence, KV head) than CTAs: against the formula, twice, and as a graph between whose replays other calls run"""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    B, J, scale = G * n, Hq // Hkv, 1 / math.sqrt(D)
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(BF16)
+
+    q, kp, vp, k, v = rand(B, Hq, D), rand(G, Hkv, P, D), rand(G, Hkv, P, D), rand(B, Hkv, L, D), rand(B, Hkv, L, D)
+    plens = torch.randint(0, P + 1, (G,), generator=g, device="cuda", dtype=I32)
+    lens = torch.randint(1, L + 1, (B,), generator=g, device="cuda", dtype=I32) if ragged else None
+    o, lse = torch.full_like(q, NAN), torch.full((B, Hq), NAN, device="cuda")
+
+    def call(o, lse):
+        m.flash_attn_decode_shared(q, kp, vp, k, v, o, lse, B, G, P, L, Hq, Hkv, D, plens, lens)
+
+    call(o, lse)
+    m.device_status()
+    for b0 in range(0, B, 200):  # in float64, some sequences at a time
+        b = torch.arange(b0, min(b0 + 200, B), device="cuda")
+        i = b // n
+        kk, vv = torch.cat([kp[i], k[b]], 2).double(), torch.cat([vp[i], v[b]], 2).double()
+        qq = q[b].double().view(len(b), Hkv, J, D)
+        at = torch.arange(P + L, device="cuda")
+        own = (lens if ragged else torch.full((B,), L, device="cuda"))[b]
+        seen = torch.where(at < P, at < plens[i, None], at - P < own[:, None])[:, None, None]
+        s = (qq @ kk.transpose(-1, -2) * scale).masked_fill(~seen, -math.inf)
+        wl = s.logsumexp(-1)
+        p = (s - wl[..., None]).exp()
+        wo, mag, e = p @ vv, p @ vv.abs(), score_error(qq, kk, scale)
+        err = (o[b].double().view_as(wo) - wo).abs()
+        assert (err <= HALF_STEP * wo.abs() + (HALF_STEP + 2 * e + 2.0**-14) * mag).all()
+        assert ((lse[b].double().view_as(wl) - wl).abs() <= 2 * e + 2.0**-20 * (1 + wl.abs())).all()
+    og, lg = torch.full_like(o, NAN), torch.full_like(lse, NAN)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(og, lg)
+        call(og, lg)
+    for _ in range(2):
+        og.fill_(NAN), lg.fill_(NAN)
+        graph.replay()
+        o2, l2 = torch.full_like(o, NAN), torch.full_like(lse, NAN)
+        call(o2, l2)
+        assert torch.equal(og, o) and torch.equal(lg, lse) and torch.equal(o2, o) and torch.equal(l2, lse)
+    m.device_status()
+
+
 def test_shared_prompts_with_far_apart_scores():
     """the prompt's keys outweigh the sequence's own by e^60, and the other way round"""
     G, n, P, L, H, D = 1, 4, 300, 40, 2, 64
