@@ -49,12 +49,28 @@ PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool 
     d.units = (long long)G * Hkv * d.n_chunks * d.tiles;
     const int all = (P + kPrefixKeys - 1) / kPrefixKeys;
     const double keys = (double)G * P * d.tiles, own = (double)B * (L + kUnitKeys);
-    d.splits = std::max(1, std::min(all, (int)(sms * keys / (keys + own) / d.units + 0.5)));
-    d.grid = d.units * d.splits;
+    const auto deal = [&](int splits) {
+        d.splits = splits;
+        d.grid = d.units * splits;
+        const int left = d.grid < sms ? sms - (int)d.grid : sms;
+        d.decode = decode_plan(B, L, Hq, Hkv, D, 0, ragged, std::min(2 * left, kDecodeMaxCtas), true, splits);
+        if (d.grid >= sms) d.decode.turn = d.decode.n_ctas;  // all of them start as the prompts' CTAs end
+    };
+    const int most = std::max(1, std::min(all, (int)(sms * keys / (keys + own) / d.units + 0.5)));
+    deal(most);
+    // Where the decode has few units, their joins with many splits are a chain of their own: so many tiles of keys a split as make the two
+    // shortest together, about 0.9 us a tile and 0.7 us a round.  (1 x 16 16000 4 8/1 128, with 123 / 62 / 31 / 15 splits: 44.5 / 15.3 / 15.1 /
+    // 17.3; 1 x 24 5000 10 16/2 64, 38 / 19 / 10: 14.4 / 11.6 / 14.6; 4 x 4 3000 64 16/4 64, 8 / 4 / 2: 11.0 / 12.1 / 16.0.)
+    const auto cost = [&](int per) { return 9 * per + 7 * decode_join_rounds(d.decode.G, D, d.decode.cluster, d.splits); };
+    if (d.decode.shares > 0) {
+        int per = (all + most - 1) / most, best = most, least = cost(per);
+        for (per += 1; 9 * per < least; per += 1 + per / 8) {
+            deal((all + per - 1) / per);
+            if (cost(per) < least) least = cost(per), best = d.splits;
+        }
+        deal(best);
+    }
     d.slots = (size_t)d.units * d.splits;
-    const int left = d.grid < sms ? sms - (int)d.grid : sms;
-    d.decode = decode_plan(B, L, Hq, Hkv, D, 0, ragged, std::min(2 * left, kDecodeMaxCtas), true);
-    if (d.grid >= sms) d.decode.turn = d.decode.n_ctas;  // all of them start as the prompts' CTAs end
     d.decode_bytes = round256((size_t)B * Hq * d.decode.splits * (size_t)(D + 2) * sizeof(float));
     d.bytes = d.decode_bytes + (d.slots * 128 + (size_t)B * Hq) * (D + 2) * sizeof(float);
     return d;

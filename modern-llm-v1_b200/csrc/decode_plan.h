@@ -49,6 +49,10 @@ constexpr long long kRangesBytes = 16ll << 20;
 constexpr int kSaturatingCtas = 60;
 constexpr long long kTurnBytes = 3ll << 18;
 
+// Rounds of loads in which the CTAs of a unit's cluster join it with the prompt's results (decode_add_prefix): about 0.7 us each, so a
+// cluster that saves two of them is worth its own 1 us (1 prompt x 12 samples, P=3220 L=3 8/1 D=128, 26 splits: 18.6 -> 11.3 us).
+inline int decode_join_rounds(int G, int D, int cluster, int prompt_splits) { return (G * (D / 2) / cluster + 127) / 128 * ((prompt_splits + 7) / 8); }
+
 // cap: CTAs that may run at once, or 0: as many as fit the device.
 //
 // Behind shared prompts (`shared`, cap: CTAs on the SMs that the prompts' kernel leaves) the CTAs wait for the prompts' kernel at their ends.
@@ -58,7 +62,7 @@ constexpr long long kTurnBytes = 3ll << 18;
 // 64 45.0 / 28.3; 2 x 128 3000 250 32/8 128 97.0 / 61.1; 16 x 4 4000 256 16/8 64 75.1 / 41.6; 8 x 8 1000 100 16/16 64 114.7 / 31.3; units of
 // 512 KB 4 x 40 1000 2000 16/4 64 54.1 / 50.5; of 1 MB 2 x 20 2000 2000 32/8 128 57.9 / 58.7, 1 x 300 1000 4000 8/1 64 52.9 / 57.2; equal
 // lengths, whole units dealt beforehand / in turn: 4 x 64 8192 256 16/4 128 57.3 / 51.6, 1 x 64 16384 256 16/4 128 27.7 / 27.8.)
-inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits, bool ragged, int cap = 0, bool shared = false) {
+inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits, bool ragged, int cap = 0, bool shared = false, int prompt_splits = 0) {
     DecodePlan d;
     const int group = Hq / Hkv;
     if (cap <= 0) cap = decode_max_ctas();
@@ -92,7 +96,9 @@ inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits
     } else {
         d.slots = (int)std::min<long long>(n_all, (2 * cap + units - 1) / units);
         if (n_all > 1) counters = std::min<long long>(tiles, cap);  // (a single tile is never shared)
-        while (d.cluster < kDecodeMaxCluster && units * d.cluster * 2 <= (shared ? cap / 2 : sm_count()) && n_all > 2 * d.cluster) d.cluster *= 2;
+        while (d.cluster < kDecodeMaxCluster && units * d.cluster * 2 <= (shared ? cap / 2 : sm_count()) &&
+               (n_all > 2 * d.cluster || decode_join_rounds(d.G, D, d.cluster, prompt_splits) > decode_join_rounds(d.G, D, d.cluster * 2, prompt_splits) + 1))
+            d.cluster *= 2;
         d.shares = d.cluster;
         const long long ctas = units * d.cluster, last = ctas % cap ? ctas % cap : cap;
         const long long idle = last < kSaturatingCtas ? unit_bytes / d.cluster * (kSaturatingCtas - last) : 0;

@@ -99,10 +99,13 @@ def test_decode_shared(G, n, P, L, Hq, Hkv, D, plens, lens, slack):
     (8, 16, 2000, 300, 24, 1, 64),
     (1, 320, 200, 3500, 8, 1, 64),     # long units
     (2, 75, 900, 1, 4, 4, 128),
+    (1, 12, 3220, 3, 8, 1, 128),       # few units, many splits of the prompt: clusters whose CTAs have no rows of their own
+    (1, 16, 16000, 4, 8, 1, 128),
+    (1, 1, 16000, 1, 4, 1, 128),
 ])
 @pytest.mark.parametrize("ragged", [True, False])
 def test_shared_prompts_of_many_sequences(G, n, P, L, Hq, Hkv, D, ragged):
-    """more units of (sequence, KV head) than CTAs: against the formula, twice, and as a graph between whose replays other calls run"""
+    """the deals of whole units: against the formula, twice, and as a graph between whose replays other calls run"""
     g = torch.Generator(device="cuda").manual_seed(n)
     B, J, scale = G * n, Hq // Hkv, 1 / math.sqrt(D)
 
