@@ -1062,7 +1062,10 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             }
         }
     }
-    if (p.cluster <= 1) return;
+    if (p.cluster <= 1) {
+        if (SHARED && tid == 0) grid_dep_wait();  // whoever waits for this kernel's end waits for the prompts' too, also behind a failure
+        return;
+    }
     // ---- the cluster's partial results: this CTA finishes its slice of the outputs.  A CTA without tiles sends weight zero, one
     // that has failed a negative row sum, upon which nobody writes the unit; nobody leaves before everybody's stores have landed.
     if (!sent) {
@@ -1089,7 +1092,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             m = fmaxf(m, ml[c].x);
             good = good && !(ml[c].y < 0.f);
         }
-        if (!good) return;  // a CTA has failed (and said so for every head)
+        if (!good) break;  // a CTA has failed (and said so for every head)
         float a0 = 0.f, a1 = 0.f, l = 0.f;
 #pragma unroll
         for (int c = 0; c < kDecodeMaxCluster; ++c) {
@@ -1101,6 +1104,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         write_rows(g, d2 * 2, a0, a1, m, l);
     }
+    if (SHARED && tid == 0) grid_dep_wait();
 }
 
 }  // namespace b200attn
