@@ -189,7 +189,8 @@ __device__ __forceinline__ uint64_t make_sdesc_plain(uint32_t smem_addr, uint32_
 // a dQ pass that writes only dQ and the row vectors, loads K, V and the first Q and dO before
 // that.  grid_dep_launch() is called where the next kernel is short or known: in the dQ pass
 // (after its own wait, so everything older is complete), in the one-pass backward's row-vector
-// kernel, in the decode and in the append of one token.  The forward, the dK/dV pass and the
+// kernel, in the decode and in the append of one token, in the prompts' kernel in front of a decode (after its own wait), and in
+// the kernels of the keys' weights.  The forward, the dK/dV pass and the
 // backward of one tile call it late, by their producer warps once their last loads are issued, and
 // only where the host says so (`early` in their parameters, see spread_smem in b200attn_api.cu).
 // From their very beginning a dependent grid would be queued behind a kernel for its whole run
@@ -499,7 +500,7 @@ __device__ __forceinline__ void reg_dealloc() {
 // Optional phase timestamps for tuning (compiled in only with -DB200ATTN_PROBE): the first
 // CTA of a launch records clock64() at numbered points into a device array.
 #ifdef B200ATTN_PROBE
-__device__ long long g_probe[512];
+static __device__ long long g_probe[512];
 #define B200ATTN_STAMP(cond, idx)                                                      \
     do {                                                                               \
         if ((cond) && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && (idx) < 512) \
@@ -507,8 +508,8 @@ __device__ long long g_probe[512];
     } while (0)
 // Per-CTA trace: SM id and begin/end times (ns) of the first 2048 CTAs of a launch, kept per kernel
 // (k = 0 forward, 1 dQ pass, 2 dK/dV pass).
-__device__ unsigned long long g_trace[8192 * 3];
-__device__ long long g_trace_clk[8192 * 2];  // clock64() at the same two points
+static __device__ unsigned long long g_trace[8192 * 3];
+static __device__ long long g_trace_clk[8192 * 2];  // clock64() at the same two points
 __device__ __forceinline__ unsigned long long b200attn_globaltimer() {
     unsigned long long t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
