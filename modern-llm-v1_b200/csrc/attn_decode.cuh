@@ -162,10 +162,10 @@ __host__ __device__ __forceinline__ int decode_len(const DecodeParams& p, int b)
 }
 // A whole unit
 template <int KEYS>
-__device__ __forceinline__ void decode_walk_unit(const DecodeParams& p, DecodeWalk& w, int unit) {
+__device__ __forceinline__ void decode_walk_unit(const DecodeParams& p, DecodeWalk& w, int unit, int len = 0) {
     w.b = int(fastdiv(unit, p.div_units));
     w.u = unit - w.b * p.units_per_seq;
-    w.len = decode_len(p, w.b);
+    w.len = len ? len : decode_len(p, w.b);
     w.n_tiles = (w.len + KEYS - 1) / KEYS;
     w.t = w.j0 = w.cta0 = 0;
     w.t_end = w.total = w.n_tiles;
@@ -616,13 +616,15 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     uint64_t* bar_full = bars;              // [NST]
     uint64_t* bar_free = bars + NST;        // [NST]
     uint64_t* bar_q = bars + 2 * NST;       // [2] the q rows of a piece have landed   (phase: piece / 2)
-    uint64_t* bar_q_free = bar_q + 2;       // [2] they are in registers               (phase: piece / 2)
+    uint64_t* bar_q_free = bar_q + 2;       // [2] the piece has ended                 (phase: piece / 2); its q rows are in registers long
+                                            // before, but a fence of their own costs 450 clocks a piece
     uint64_t* bar_part = bar_q_free + 2;    // the shared piece at the range's beginning has been stored
     volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_part + 1);
     volatile int* last_flag = abort_flag + 1;
     volatile int* fail_flag = abort_flag + 2;
     volatile int* epoch = abort_flag + 3;
     volatile int* turn_unit = abort_flag + 4;                            // [2] kDecodeSharedTurn: the unit whose q rows lie in buffer 0 / 1, or -1: no more
+    volatile int* turn_len = abort_flag + 6;                             // [2] and its sequence's length
     int* turn_list = reinterpret_cast<int*>(sXMl);                       // (there are no clusters then)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -690,7 +692,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                         if (!ok) break;
                     }
                     if (elect_one()) {
-                        if (TURN) turn_unit[n & 1] = unit;
+                        if (TURN) turn_unit[n & 1] = unit, turn_len[n & 1] = w.len;
                         mbar_arrive_expect_tx(&bar_q[n & 1], G * D * 2);
                         bulk_load_1d(sQ + (n & 1) * Cfg::kQBytes, p.q + (size_t(w.b) * p.Hq + h0) * D, G * D * 2, &bar_q[n & 1]);
                     }
@@ -813,12 +815,14 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     for (int n = 0; TURN || w.t < w.t_end; ++n) {
         if (ok) ok = mbar_wait_warp(&bar_q[n & 1], (n >> 1) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_LOAD);
         if constexpr (TURN) {
-            ok = decode_bar_ok(ok);
-            if (!ok) break;
-            const int unit = turn_unit[n & 1];
-            if (unit < 0) break;
-            decode_walk_unit<KEYS>(p, w, unit);
-            if (tid == 0 && defer) turn_list[listed] = unit;
+            // (a warp that has given up has no unit; it meets the others at the barrier of the piece's end, or at this one)
+            const int unit = ok ? turn_unit[n & 1] : 0;
+            if (unit < 0) {
+                ok = decode_bar_ok(ok);
+                break;
+            }
+            if (ok) decode_walk_unit<KEYS>(p, w, unit, turn_len[n & 1]);
+            if (ok && tid == 0 && defer) turn_list[listed] = unit;
         }
         const int tiles = decode_piece(w);
         DecodeState<D, NH> st;
@@ -832,8 +836,6 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
                 for (int ks = 0; ks < KS; ks += 2)  // matrices 0-3: head-dim chunks 2ks .. 2ks+3 of heads nh * 8 .. + 8
                     ldsm_x4(q_base + (nh * 8 + (lane & 7)) * Cfg::kQRow + (ks * 2 + (lane >> 3)) * 16, bq[ks][nh][0], bq[ks][nh][1],
                             bq[ks + 1][nh][0], bq[ks + 1][nh][1]);
-            fence_proxy_async_smem();
-            mbar_arrive(&bar_q_free[n & 1]);
         }
         const int kw = warp * (KEYS / 4);  // this warp's keys inside a tile
         for (int i = 0; i < tiles; ++i, ++j) {
@@ -867,10 +869,14 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             // ---- mask keys beyond the cache length (a unit's last tile only)
             const int tile_key = (w.j0 + i) * KEYS;
             if (tile_key + KEYS > w.len) {
-                if (MODE != kDecodePlain) {  // this warp's V rows of them
-                    for (int r = kw; r < kw + KEYS / 4; ++r)
-                        if (tile_key + r >= w.len && lane < D / 8)
-                            *reinterpret_cast<uint4*>(sKV + s * 2 * Cfg::kTileBytes + Cfg::kTileBytes + swz_off(r, lane, Cfg::kBoxBytes)) = make_uint4(0u, 0u, 0u, 0u);
+                if (MODE != kDecodePlain) {  // this warp's V rows of them, 512 bytes at a time
+                    constexpr int C = D / 8;
+#pragma unroll
+                    for (int r0 = 0; r0 < KEYS / 4; r0 += 32 / C) {
+                        const int r = kw + r0 + lane / C;
+                        if (tile_key + r >= w.len)
+                            *reinterpret_cast<uint4*>(sKV + s * 2 * Cfg::kTileBytes + Cfg::kTileBytes + swz_off(r, lane % C, Cfg::kBoxBytes)) = make_uint4(0u, 0u, 0u, 0u);
+                    }
                     __syncwarp();
                 }
 #pragma unroll
@@ -966,6 +972,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             // every piece's loads are waited for, nothing is written
             if (p.cluster > 1) break;  // (one piece)
             fence_proxy_async_smem();
+            mbar_arrive(&bar_q_free[n & 1]);
             mbar_arrive(&bar_free[s_last]);
             if constexpr (!TURN) decode_walk_next<KEYS>(p, w, tiles);
             continue;
@@ -1033,6 +1040,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         }
         // the scratch was written and read with ordinary accesses; the stage goes back to TMA
         fence_proxy_async_smem();
+        mbar_arrive(&bar_q_free[n & 1]);
         mbar_arrive(&bar_free[s_last]);
         named_bar_sync(1, 128);  // sMl and the flag are rewritten at the next piece's end
         if constexpr (TURN) {

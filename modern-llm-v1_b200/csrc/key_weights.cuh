@@ -6,8 +6,8 @@
 //
 // One new token per sequence: the decode kernel leaves its scores (kDecodeScores) and decode_weights_kernel, behind it, has only to
 // take the exponentials against the final lse: 4 G bytes a key written and read through L2 beside the 4 D of its K and V rows, instead
-// of a second pass over K.  Measured on B200 against the decode alone, us: B=1 L=1500 16/4 D=128 9.3 and 6.2, B=32 L<=4096 16/4 D=64 24.2 and
-// 19.5: the second launch and the scores.
+// of a second pass over K.  Measured on B200 against the decode alone, us: B=1 L=1500 16/4 D=128 8.7 and 6.1, B=32 L<=4096 16/4 D=64 22.1 and
+// 18.4: the second launch and the scores.
 //
 // A chunk of new tokens: key_weights_kernel computes S^T = K Q^T by tiles of 128 keys (lanes of tensor memory) and 128 query rows
 // (columns), so that a key's sum runs inside a thread and needs no exchange.
