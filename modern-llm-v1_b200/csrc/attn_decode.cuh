@@ -532,63 +532,72 @@ __device__ __forceinline__ void decode_join_unit(const DecodeParams& p, const De
     }
 }
 
-// The same for the n units of a list, in kDecodeSharedTurn.  Of prompts in one or two splits, four elements' loads are issued together.
-template <int D, int KEYS>
+// The same for the n units of a list, in kDecodeSharedTurn: two elements' loads of four splits are issued together.  (Four of two for
+// prompts in one or two splits as well: 58.3 us instead of 61.7 where 2048 units join a prompt in one split, and 0.1 to 0.6 more nearly everywhere else,
+// the variants' registers being the whole kernel's.)
+template <int D>
 __device__ __forceinline__ void decode_join_units(const DecodeParams& p, const int* list, int n, int tid) {
     const DecodePrefix& x = p.prefix;
     const int per = p.G * (D / 4), total = n * per;
-    DecodeWalk w;
-    if (x.splits > 2) {
-        for (int k = 0; k < n; ++k) {
-            decode_walk_unit<KEYS>(p, w, list[k]);
-            decode_join_unit<D>(p, w, tid);
-        }
-        return;
-    }
     const int status = *reinterpret_cast<volatile int*>(p.status);
-    constexpr int E = 4;
+    constexpr int E = 2, N = 4;
+#pragma unroll 1
     for (int i0 = tid; i0 < total; i0 += 128 * E) {
-        float4 own[E], po[E][2];
-        float2 ml[E], pml[E][2];
-        size_t at[E];
-        int col[E];
+        float4 a[E];
+        float2 ml[E];
+        size_t at[E], slot0[E];
+        int col[E], row[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = min(i0 + e * 128, total - 1), k = i / per, r = i - k * per, c = r / p.G, g = r - c * p.G;
             const int unit = list[k], b = int(fastdiv(unit, p.div_units)), u = unit - b * p.units_per_seq;
             const int hk = int(fastdiv(u, p.div_chunks)), j = (u - hk * p.n_chunks) * p.G + g;
             at[e] = size_t(b) * p.Hq + hk * p.group + j, col[e] = c;
-            own[e] = __ldcg(reinterpret_cast<const float4*>(x.own_o + at[e] * D) + c);
+            a[e] = __ldcg(reinterpret_cast<const float4*>(x.own_o + at[e] * D) + c);
             ml[e] = __ldcg(x.own_ml + at[e]);
-            int row;
-            const size_t slot0 = decode_prefix_row(x, b, hk, j, &row);
+            slot0[e] = decode_prefix_row(x, b, hk, j, &row[e]);
+        }
+#pragma unroll 1
+        for (int s0 = 0; s0 < x.splits; s0 += N) {
+            float4 po[E][N];
+            float2 pml[E][N];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const size_t slot = slot0 + min(s, x.splits - 1);
-                pml[e][s] = __ldcg(x.ml + slot * 128 + row);
-                po[e][s] = __ldcg(reinterpret_cast<const float4*>(x.o + (slot * (D / 4) + c) * 512 + row * 4));
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int s = 0; s < N; ++s) {  // (splits that are not there: the last one's)
+                    const size_t slot = slot0[e] + min(s0 + s, x.splits - 1);
+                    pml[e][s] = __ldcg(x.ml + slot * 128 + row[e]);
+                    po[e][s] = __ldcg(reinterpret_cast<const float4*>(x.o + (slot * (D / 4) + col[e]) * 512 + row[e] * 4));
+                }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                float m = ml[e].x;
+#pragma unroll
+                for (int s = 0; s < N; ++s) {
+                    if (s0 + s >= x.splits) pml[e][s] = make_float2(-INFINITY, 0.f);
+                    m = fmaxf(m, pml[e][s].x);
+                }
+                const float f = ml[e].x == -INFINITY ? 1.f : ex2_approx((ml[e].x - m) * p.scale_log2);  // (as in decode_add_prefix)
+                ml[e] = make_float2(m, ml[e].y * f);
+                a[e].x *= f, a[e].y *= f, a[e].z *= f, a[e].w *= f;
+#pragma unroll
+                for (int s = 0; s < N; ++s) {
+                    const bool any = !(pml[e][s].x == -INFINITY && pml[e][s].y == 0.f);
+                    const float fs = pml[e][s].x == -INFINITY ? 1.f : ex2_approx((pml[e][s].x - m) * p.scale_log2);
+                    ml[e].y += fs * pml[e][s].y;
+                    a[e].x += any ? fs * po[e][s].x : 0.f;
+                    a[e].y += any ? fs * po[e][s].y : 0.f;
+                    a[e].z += any ? fs * po[e][s].z : 0.f;
+                    a[e].w += any ? fs * po[e][s].w : 0.f;
+                }
             }
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             if (i0 + e * 128 >= total || status != 0) break;
-            if (x.splits < 2) pml[e][1] = make_float2(-INFINITY, 0.f);
-            const float m = fmaxf(ml[e].x, fmaxf(pml[e][0].x, pml[e][1].x));
-            const float f = ml[e].x == -INFINITY ? 1.f : ex2_approx((ml[e].x - m) * p.scale_log2);
-            float l = ml[e].y * f, a[4] = {own[e].x * f, own[e].y * f, own[e].z * f, own[e].w * f};
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const bool any = !(pml[e][s].x == -INFINITY && pml[e][s].y == 0.f);
-                const float fs = pml[e][s].x == -INFINITY ? 1.f : ex2_approx((pml[e][s].x - m) * p.scale_log2);
-                l += fs * pml[e][s].y;
-                a[0] += any ? fs * po[e][s].x : 0.f;
-                a[1] += any ? fs * po[e][s].y : 0.f;
-                a[2] += any ? fs * po[e][s].z : 0.f;
-                a[3] += any ? fs * po[e][s].w : 0.f;
-            }
-            const float inv = 1.f / l;
-            reinterpret_cast<uint2*>(p.o)[at[e] * (D / 4) + col[e]] = make_uint2(pack_bf16x2(a[0] * inv, a[1] * inv), pack_bf16x2(a[2] * inv, a[3] * inv));
-            if (p.lse && col[e] == 0) p.lse[at[e]] = m * p.scale + logf(l);
+            const float inv = 1.f / ml[e].y;
+            reinterpret_cast<uint2*>(p.o)[at[e] * (D / 4) + col[e]] = make_uint2(pack_bf16x2(a[e].x * inv, a[e].y * inv), pack_bf16x2(a[e].z * inv, a[e].w * inv));
+            if (p.lse && col[e] == 0) p.lse[at[e]] = ml[e].x * p.scale + logf(ml[e].y);
         }
     }
 }
@@ -1046,7 +1055,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if constexpr (TURN) {
             if (defer && ++listed == kDecodeTurnList) {  // (from here on the prompts' results are there)
                 grid_dep_wait();
-                decode_join_units<D, KEYS>(p, turn_list, listed, tid);
+                decode_join_units<D>(p, turn_list, listed, tid);
                 listed = 0;
                 defer = false;
             }
@@ -1057,7 +1066,7 @@ attn_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     if constexpr (TURN) {
         if (ok && listed > 0) {  // the units that this CTA has finished; none behind a failure
             grid_dep_wait();
-            decode_join_units<D, KEYS>(p, turn_list, listed, tid);
+            decode_join_units<D>(p, turn_list, listed, tid);
         }
     } else if constexpr (MODE == kDecodeShared) {
         if (p.prefix.own_o && ok && !failed) {  // the units that this CTA has finished

@@ -33,12 +33,15 @@ struct PrefixPlan {
     size_t decode_bytes, bytes;  // of the workspace: the decode's own, all
     size_t slots;
 };
-// The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others, and both are bound by HBM or, when
-// short, by latency: SMs are shared out by the keys to be gone through, once for every tile of a prompt's rows, and kUnitKeys more for each
-// unit of the decode's, its beginning and end.  (1 prompt x 64 samples, P=16384 L=256 16/4 D=128, all lengths the same, us with 0 / 128 / 192 /
-// 256 of them: 27.5 / 28.5 / 27.7 / 29.7; L=64: 39.4 / 27.8 / 26.9 / 27.9; 1 x 16 16000 100 32/8 128: 42.8 / 25.3 / 23.3 / 23.2; 8 x 16 2000 1
-// 16/4 64, the first token behind the prompts: 67.9 / 21.6 / 21.6 / 21.6.)
-constexpr int kUnitKeys = 192;
+// The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others.  SMs are shared out so that the
+// longer of the two, and the join behind it, is shortest.  What a CTA takes, in us, from timing calls with every number of splits:
+constexpr double kPrefixStart = 4.0, kUnitStart = 2.0, kDecodeTile = 0.95;  // a prompt's CTA without its tiles, a decode's unit without its tiles, one of those (32 KB)
+constexpr double prefix_tile(int D) { return D == 64 ? 0.95 : 1.1; }
+constexpr double kJoinRound = 0.7;
+// (us with so many splits; G prompts x n samples, P, L, heads, D, lengths up to L.  8 x 16 2000 300 16/4 64: 1 22.0, 2 18.4, 3 21.7, 4 22.1;
+// the same with L=1: 20.8, 15.7, 19.4, 19.8; 2 x 57 2432 6 16/4 64: 2 16.7, 4 14.5, 6 17.9, 8 18.2; 1 x 128 8000 100 16/4 64: 3 25.6, 5 20.7, 6 22.5,
+// 8 25.9; 4 x 16 8000 200 16/4 128: 3 30.1, 5 25.2, 6 25.9, 8 32.9.  By the keys to be gone through alone, as before, it took 1, 1, 3, 5 and 5; as it is
+// 2, 2, 4, 5 and 7.)
 PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool ragged) {
     PrefixPlan d;
     const int group = Hq / Hkv, n = B / G, sms = sm_count();
@@ -48,28 +51,31 @@ PrefixPlan prefix_plan(int B, int G, int P, int L, int Hq, int Hkv, int D, bool 
     d.tiles = (n + d.seqs - 1) / d.seqs;
     d.units = (long long)G * Hkv * d.n_chunks * d.tiles;
     const int all = (P + kPrefixKeys - 1) / kPrefixKeys;
-    const double keys = (double)G * P * d.tiles, own = (double)B * (L + kUnitKeys);
+    const long long decode_units = (long long)B * Hkv * (group / decode_heads_per_cta(group));
+    const int keys = decode_tile_keys(D);
+    const double unit = kUnitStart + kDecodeTile * (ragged ? 0.5 + 0.5 * L / keys : (double)((L + keys - 1) / keys));
+    // `splits` of the keys, and what that takes
     const auto deal = [&](int splits) {
         d.splits = splits;
         d.grid = d.units * splits;
-        const int left = d.grid < sms ? sms - (int)d.grid : sms;
-        d.decode = decode_plan(B, L, Hq, Hkv, D, 0, ragged, std::min(2 * left, kDecodeMaxCtas), true, splits);
+        const int left = d.grid < sms ? sms - (int)d.grid : sms, cap = std::min(2 * left, kDecodeMaxCtas);
+        d.decode = decode_plan(B, L, Hq, Hkv, D, 0, ragged, cap, true, splits);
         if (d.grid >= sms) d.decode.turn = d.decode.n_ctas;  // all of them start as the prompts' CTAs end
+        const double prompts = kPrefixStart + prefix_tile(D) * ((all + splits - 1) / splits);
+        if (d.decode.shares > 0) return prompts + kJoinRound * decode_join_rounds(d.decode.G, D, d.decode.cluster, splits);
+        const long long units = (decode_units + cap - 1) / cap;
+        return std::max(prompts, unit * (double)decode_units / cap) + kJoinRound * (double)((units * d.decode.G * (D / 4) + 255) / 256) * ((splits + 3) / 4);
     };
-    const int most = std::max(1, std::min(all, (int)(sms * keys / (keys + own) / d.units + 0.5)));
-    deal(most);
-    // Where the decode has few units, their joins with many splits are a chain of their own: so many tiles of keys a split as make the two
-    // shortest together, about 0.9 us a tile and 0.7 us a round.  (1 x 16 16000 4 8/1 128, with 123 / 62 / 31 / 15 splits: 44.5 / 15.3 / 15.1 /
-    // 17.3; 1 x 24 5000 10 16/2 64, 38 / 19 / 10: 14.4 / 11.6 / 14.6; 4 x 4 3000 64 16/4 64, 8 / 4 / 2: 11.0 / 12.1 / 16.0.)
-    const auto cost = [&](int per) { return 9 * per + 7 * decode_join_rounds(d.decode.G, D, d.decode.cluster, d.splits); };
-    if (d.decode.shares > 0) {
-        int per = (all + most - 1) / most, best = most, least = cost(per);
-        for (per += 1; 9 * per < least; per += 1 + per / 8) {
-            deal((all + per - 1) / per);
-            if (cost(per) < least) least = cost(per), best = d.splits;
-        }
-        deal(best);
+    int per = (int)std::max<long long>(1, std::min<long long>(all, (all * d.units + sms - 1) / sms)), best = (all + per - 1) / per;  // tiles of keys a split
+    if (best * d.units >= sms && per < all) best = (all + per) / (per + 1), ++per;
+    double least = deal(best);
+    for (per += 1 + per / 8; per < all + 1 + all / 8 && kPrefixStart + prefix_tile(D) * std::min(per, all) < least * 1.03; per += 1 + per / 8) {
+        const int splits = (all + per - 1) / per;
+        const double t = deal(splits);
+        if (t <= least * 1.03) best = splits;  // (of about equal ones the one that leaves the decode more SMs)
+        least = std::min(least, t);
     }
+    deal(best);
     d.slots = (size_t)d.units * d.splits;
     d.decode_bytes = round256((size_t)B * Hq * d.decode.splits * (size_t)(D + 2) * sizeof(float));
     d.bytes = d.decode_bytes + (d.slots * 128 + (size_t)B * Hq) * (D + 2) * sizeof(float);

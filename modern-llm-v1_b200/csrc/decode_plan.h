@@ -58,10 +58,10 @@ inline int decode_join_rounds(int G, int D, int cluster, int prompt_splits) { re
 // Behind shared prompts (`shared`, cap: CTAs on the SMs that the prompts' kernel leaves) the CTAs wait for the prompts' kernel at their ends.
 // More units than those CTAs, of at most kTurnBytes: each takes a whole unit, then the next that nobody has taken, and so do the CTAs that
 // start on the SMs which the prompts' kernel frees.  Longer units are dealt in ranges among cap CTAs, which come out more even.  (us, units of
-// different lengths up to L, ranges / in turn; G prompts x n samples, P, L, heads, D: 8 x 16 2000 300 16/4 64 25.7 / 21.7; 16 x 16 500 300 8/4
-// 64 45.0 / 28.3; 2 x 128 3000 250 32/8 128 97.0 / 61.1; 16 x 4 4000 256 16/8 64 75.1 / 41.6; 8 x 8 1000 100 16/16 64 114.7 / 31.3; units of
-// 512 KB 4 x 40 1000 2000 16/4 64 54.1 / 50.5; of 1 MB 2 x 20 2000 2000 32/8 128 57.9 / 58.7, 1 x 300 1000 4000 8/1 64 52.9 / 57.2; equal
-// lengths, whole units dealt beforehand / in turn: 4 x 64 8192 256 16/4 128 57.3 / 51.6, 1 x 64 16384 256 16/4 128 27.7 / 27.8.)
+// different lengths up to L, ranges / in turn, as both were at first; G prompts x n samples, P, L, heads, D: 8 x 16 2000 300 16/4 64 25.7 / 21.7;
+// 16 x 16 500 300 8/4 64 45.0 / 28.3; 2 x 128 3000 250 32/8 128 97.0 / 61.1; 16 x 4 4000 256 16/8 64 75.1 / 41.6; 8 x 8 1000 100 16/16 64 114.7 / 31.3;
+// units of 512 KB 4 x 40 1000 2000 16/4 64 54.1 / 50.5; of 1 MB 2 x 20 2000 2000 32/8 128 57.9 / 58.7, 1 x 300 1000 4000 8/1 64 52.9 / 57.2; equal
+// lengths, whole units dealt beforehand / in turn: 4 x 64 8192 256 16/4 128 57.3 / 51.6.)
 inline DecodePlan decode_plan(int B, int L, int Hq, int Hkv, int D, int n_splits, bool ragged, int cap = 0, bool shared = false, int prompt_splits = 0) {
     DecodePlan d;
     const int group = Hq / Hkv;
