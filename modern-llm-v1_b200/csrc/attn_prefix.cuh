@@ -21,8 +21,8 @@
 // (512 columns), per softmax: S 128 with P over each half's scores, O D.
 //
 // Measured on B200, us per call, this kernel and the decode behind (G prompts, n sequences each, 16/4 heads):
-//   G=8 n=16 P<=2000 L<=300 D=64: one softmax 28.3, two, thread = row 27.0, thread = row and half 25.3, the decode's units in turn 21.7
-//   G=1 n=64 P=16384 L=256 D=128: one softmax 31.5, two, thread = row and half 27.4, with the decode's units in turn 27.8 (67 MB: 2.4 TB/s)
+//   G=8 n=16 P<=2000 L<=300 D=64: one softmax 28.3, two, thread = row 27.0, thread = row and half 25.3; with the decode's units in turn 21.7, two splits 17.4
+//   G=1 n=64 P=16384 L=256 D=128: one softmax 31.5, two, thread = row and half 27.4, as it is 26.9 (67 MB: 2.5 TB/s)
 //   G=1 n=8 P=500 L=12 6/2 D=64: 6.9, 7.0 and 7.2 (the two launches' latency)
 // Measured and dropped: tiles of 64 keys with P beside S (Q K^T takes 64 clocks a step for half the keys); two tiles of rows in a CTA, every K and
 // V tile used twice, 31.5 where two CTAs that each read them take 27.4 (the partial results of 256 rows are as many bytes as 256 keys, and
