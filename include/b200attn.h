@@ -275,7 +275,8 @@ int b200attn_rope_norm_bwd_qk(const void* dyq, const void* dyk, int y_layout, co
  *   pos: [B, T] (device, int32) the tokens' positions, or NULL: token t has position t.  cos_t, sin_t: [n_pos, R / 2] FP32, 16-byte
  *   aligned.  A token whose position is not in [0, n_pos) is skipped (its outputs are not written) and sets the device status word to 106.
  *   gamma_q and gamma_k: the QK-norm behind the rotation, with rstd_* [B, H, T] written (forward) or read (backward); both NULL:
- *   no norm, and then rstd_*, d_gamma_* and, in the backward, xq and xk are not used and may be NULL.
+ *   no norm, and then rstd_*, d_gamma_* and, in the backward, xq and xk are not used and may be NULL.  (gamma_*, d_gamma_* and rstd_*
+ *   may begin at any float.)
  *
  * Layouts, types and d_gamma (accumulated into, in a fixed order) as for b200attn_rope_norm_fwd / _bwd; the workspace, of
  * b200attn_rope_norm_bwd_workspace_bytes(D), is only needed with the norm.
@@ -305,8 +306,8 @@ int b200attn_rotary_bwd(const void* dyq, const void* dyk, int y_layout, const vo
  * b200attn_kv_append with those rotations, for caches whose rows and positions part ways (behind a shared prompt, after an
  * eviction).  The n_new tokens of sequence b get the positions pos[b] + t and the cache rows rows[b] + t; pos and rows are [B]
  * (device, int32) or NULL: pos0 and row0 for every sequence.  positions: [B, Hkv, L_cap] int32, where the k rows' positions are
- * noted, or NULL.  gamma_q and gamma_k may both be NULL (no norm).  A sequence whose rows exceed L_cap (status word 105) or whose
- * positions exceed the tables (106) is skipped.
+ * noted, or NULL.  gamma_q and gamma_k may both be NULL (no norm); else they are 16-byte aligned, as the tables are.  A sequence
+ * whose rows exceed L_cap (status word 105) or whose positions exceed the tables (106) is skipped.
  */
 int b200attn_kv_append_rotary(const void* xq, const void* xk, const void* xv, int x_dtype, void* q_out, void* kcache,
                               void* vcache, int* positions, const float* gamma_q, const float* gamma_k,

@@ -63,7 +63,10 @@ kv_rotary_kernel(const __grid_constant__ KvRotaryParams p) {
             raw.load(which == 0 ? p.xq : which == 1 ? p.xk : p.xv, static_cast<long long>(r) * D, rl.at, rl.more);
             raw.r.get(v);
             if (NORM && which != 2) {
-                rotary_gamma(which == 0 ? p.gamma_q : p.gamma_k, rl.at, rl.more, gm);
+                // (16-byte aligned, as b200attn_kv_append_rotary asks: this is loaded with every row)
+                const float* const gamma = (which == 0 ? p.gamma_q : p.gamma_k) + rl.at;
+                const float4 ga = *reinterpret_cast<const float4*>(gamma), gb = *reinterpret_cast<const float4*>(gamma + rl.more);
+                gm[0] = ga.x, gm[1] = ga.y, gm[2] = ga.z, gm[3] = ga.w, gm[4] = gb.x, gm[5] = gb.y, gm[6] = gb.z, gm[7] = gb.w;
             }
         }
         // (a position that the tables do not have reads their first rows: t < n_new <= n_pos was checked by the host)

@@ -95,10 +95,11 @@ __device__ __forceinline__ void rotary_store8(void* base, long long row, int at,
         *reinterpret_cast<uint2*>(ptr + more) = make_uint2(rn_pack_bf16x2(v[4], v[5]), rn_pack_bf16x2(v[6], v[7]));
     }
 }
-// gamma of the lane's elements
+// gamma of the lane's elements, one by one: it may begin at any float of a buffer that holds all of a model's parameters.  (Once per
+// warp, in front of its rows.)
 __device__ __forceinline__ void rotary_gamma(const float* gamma, int at, int more, float (&g)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(gamma + at), b = *reinterpret_cast<const float4*>(gamma + at + more);
-    g[0] = a.x, g[1] = a.y, g[2] = a.z, g[3] = a.w, g[4] = b.x, g[5] = b.y, g[6] = b.z, g[7] = b.w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) g[e] = gamma[at + e], g[e + 4] = gamma[at + more + e];
 }
 
 // The position of a lane's token; a token whose position the tables do not have is dropped (live = false).
