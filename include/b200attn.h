@@ -342,7 +342,9 @@ int b200attn_kv_append_rotary(const void* xq, const void* xk, const void* xv, in
  *   overlap weights and positions, which are only read.
  *
  * Sums are FP32 and in a fixed order: a call repeats bit for bit.  Workspaces: at least ..._workspace_bytes(...), 256-byte aligned, without
- * initialisation; calls that may overlap need workspaces of their own.  Nothing is written while the device status word is set.
+ * initialisation; calls that may overlap need workspaces of their own.  Nothing is written while the device status word is set.  (Where
+ * another stream's kernel sets the word, or another thread clears it, while a call runs, that call may have written some of its
+ * outputs, some (batch, KV head) pairs of an evicted cache for instance, and not others.)
  */
 int b200attn_decode_shared(const void* q, const void* kprefix, const void* vprefix, const void* kcache, const void* vcache,
                            void* o, float* lse, const int* prefix_lens, const int* lens, int B, int G, int P, int P_cap,

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv_evict_kernel(const EvictP
     int* s_from = s_hist + kEvictBins;                     // [kEvictWindow] rows that move, in order
     int* s_to = s_from + kEvictWindow;                     // [kEvictWindow] free places, in order
     uint32_t* s_key = reinterpret_cast<uint32_t*>(s_to + kEvictWindow);  // [n]
-    __shared__ int s_max[kEvictWarps], s_pick[3][3];
+    __shared__ int s_max[kEvictWarps], s_pick[3][3], s_status;
     __shared__ int2 s_red[5][kEvictWarps];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -111,15 +111,17 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv_evict_kernel(const EvictP
     int* const pos_out = p.pos_out + base;
     grid_dep_wait();
     if (LIST) grid_dep_launch();
-    const int status = *reinterpret_cast<const volatile int*>(p.status);  // (looked at where something is written: no round trip of its own)
+    // The status word, which other streams and the host may change at any time: a CTA goes by what one thread has read once, since rows
+    // are listed and moved by all threads together.  (Looked at where something is written: no round trip of its own.)
+    const int status = *reinterpret_cast<const volatile int*>(p.status);
     const int n = p.lens ? max(0, min(__ldg(p.lens + unit / p.Hkv), p.L)) : p.L;
     const int left = min(n, p.keep);
     // this CTA's share of the rows whose weight and position it writes
     const int r0 = int((long long)p.L_cap * rank / ranks), r1 = int((long long)p.L_cap * (rank + 1) / ranks);
     if (n <= p.keep) {
-        if (status != 0) return;
-        for (int i = r0 + tid; i < r1; i += kEvictThreads) w_out[i] = i < n ? __ldg(w + i) : 0.f, pos_out[i] = i < n ? __ldg(pos + i) : -1;
         if (LIST && tid == 0) p.n_moves[unit] = 0;
+        if (__syncthreads_or(status != 0)) return;
+        for (int i = r0 + tid; i < r1; i += kEvictThreads) w_out[i] = i < n ? __ldg(w + i) : 0.f, pos_out[i] = i < n ? __ldg(pos + i) : -1;
         return;
     }
 
@@ -146,6 +148,7 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv_evict_kernel(const EvictP
     }
     for (int o = 16; o > 0; o >>= 1) newest = max(newest, __shfl_xor_sync(0xffffffffu, newest, o));
     if (lane == 0) s_max[warp] = newest;
+    if (tid == 0) s_status = status;
     for (int i = tid; i < kEvictBins; i += kEvictThreads) s_hist[i] = 0;
     __syncthreads();
     newest = s_max[lane];
@@ -218,7 +221,10 @@ __global__ void __launch_bounds__(kEvictThreads, 1) kv_evict_kernel(const EvictP
     });
     const int2 at0 = evict_warps_before(holes, moves, s_red[4], &total);  // as many moves as free places
 
-    if (status != 0) return;
+    if (s_status != 0) {
+        if (LIST && tid == 0) p.n_moves[unit] = 0;
+        return;
+    }
     // ---- this CTA's share of the moves, a window at a time; with the first, the weights and positions that do not move
     const int m0 = int((long long)total * rank / ranks), m1 = int((long long)total * (rank + 1) / ranks);
     bool first_window = true;
@@ -257,9 +263,11 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictParams
     __shared__ int2 s_move[kMoveRows];
     const int tid = threadIdx.x, unit = int(blockIdx.x) / p.blocks, e0 = (int(blockIdx.x) - unit * p.blocks) * kMoveRows;
     grid_dep_wait();
-    const int status = *reinterpret_cast<const volatile int*>(p.status), m = min(kMoveRows, __ldcg(p.n_moves + unit) - e0);
+    // (Not a second look at the status word: what is listed is moved, as the weights and positions have been, and a unit that was not
+    // selected has no moves.)
+    const int m = min(kMoveRows, __ldcg(p.n_moves + unit) - e0);
     if (tid < kMoveRows && e0 + tid < p.most) s_move[tid] = __ldcg(p.moves + size_t(unit) * p.most + e0 + tid);  // (some may not be set)
-    if (m <= 0 || status != 0) return;
+    if (m <= 0) return;
     __syncthreads();
     const size_t base = size_t(unit) * p.L_cap * D;
     evict_move<D, kMoveThreads / 32, 8>(p.k + base, p.v + base, m, tid >> 5, tid & 31, [&](int e) { return s_move[e]; });
