@@ -308,12 +308,21 @@ int b200attn_rotary_bwd(const void* dyq, const void* dyk, int y_layout, const vo
  * (device, int32) or NULL: pos0 and row0 for every sequence.  positions: [B, Hkv, L_cap] int32, where the k rows' positions are
  * noted, or NULL.  gamma_q and gamma_k may both be NULL (no norm); else they are 16-byte aligned, as the tables are.  A sequence
  * whose rows exceed L_cap (status word 105) or whose positions exceed the tables (106) is skipped.
+ *
+ * b200attn_kv_append_weights: the same for a cache whose keys' weights are kept (b200attn_decode_weights, b200attn_key_weights): the new
+ * rows' weights [B, Hkv, L_cap] FP32 become 0, so that a row which another token has held before (one that was taken back, padding)
+ * begins without its weight.
  */
 int b200attn_kv_append_rotary(const void* xq, const void* xk, const void* xv, int x_dtype, void* q_out, void* kcache,
                               void* vcache, int* positions, const float* gamma_q, const float* gamma_k,
                               const float* cos_t, const float* sin_t, int n_pos, int R, int pairs, const int* pos,
                               int pos0, const int* rows, int row0, int B, int n_new, int L_cap, int Hq, int Hkv, int D,
                               float eps, void* stream);
+int b200attn_kv_append_weights(const void* xq, const void* xk, const void* xv, int x_dtype, void* q_out, void* kcache,
+                               void* vcache, int* positions, float* weights, const float* gamma_q, const float* gamma_k,
+                               const float* cos_t, const float* sin_t, int n_pos, int R, int pairs, const int* pos,
+                               int pos0, const int* rows, int row0, int B, int n_new, int L_cap, int Hq, int Hkv, int D,
+                               float eps, void* stream);
 
 /*
  * Sampling from long contexts (the reference keeps no cache at all, llm/apps/infer_modern_gpt.cu:253-255).

@@ -68,6 +68,7 @@ SYMBOLS = (
     "b200attn_rotary_fwd",
     "b200attn_rotary_bwd",
     "b200attn_kv_append_rotary",
+    "b200attn_kv_append_weights",
     "b200attn_decode_shared",
     "b200attn_decode_shared_workspace_bytes",
     "b200attn_decode_weights",
@@ -172,6 +173,8 @@ def load() -> ctypes.CDLL:
     L.b200attn_rotary_bwd.restype = i
     L.b200attn_kv_append_rotary.argtypes = [vp] * 3 + [i] + [vp] * 8 + [i] * 3 + [vp, i, vp, i] + [i] * 6 + [f, vp]
     L.b200attn_kv_append_rotary.restype = i
+    L.b200attn_kv_append_weights.argtypes = [vp] * 3 + [i] + [vp] * 9 + [i] * 3 + [vp, i, vp, i] + [i] * 6 + [f, vp]
+    L.b200attn_kv_append_weights.restype = i
     L.b200attn_decode_shared.argtypes = [vp] * 9 + [i] * 9 + [f, vp, sz, vp]
     L.b200attn_decode_shared.restype = i
     L.b200attn_decode_shared_workspace_bytes.argtypes = [i] * 7

@@ -859,11 +859,11 @@ bool heads_ok(const char* fn, int Hq, int Hkv, int D) {
 }
 
 // xq, xk, xv, gamma_q, gamma_k, q_out, kcache, vcache, positions, cos, sin, rotary_dim, pairs (a number), pos, pos0, rows, row0, B, L_cap,
-// Hq, Hkv, D, eps
+// Hq, Hkv, D, eps, weights or None
 PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const char* fn = "KVCache.append";
     B200ATTN_TRY
-    if (!arg_count(n, 23)) return nullptr;
+    if (!arg_count(n, 24)) return nullptr;
     ScalarType xt;
     int xd;
     if (!x_dtype(fn, a[0], &xt, &xd)) return nullptr;
@@ -873,7 +873,7 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if ((a[3] == Py_None) != (a[4] == Py_None)) return value_error("%s: gamma_q and gamma_k belong together", fn);
     Items items;
     items.add(a[6], "K cache", bf), items.add(a[7], "V cache", bf), items.add(a[0], "xq", xt), items.add(a[1], "xk", xt), items.add(a[2], "xv", xt);
-    items.add(a[5], "q_out", bf), items.add(a[3], "gamma_q", f), items.add(a[4], "gamma_k", f), items.add(a[8], "positions", i32);
+    items.add(a[5], "q_out", bf), items.add(a[3], "gamma_q", f), items.add(a[4], "gamma_k", f), items.add(a[8], "positions", i32), items.add(a[23], "weights", f);
     items.add(a[9], "cos", f), items.add(a[10], "sin", f), items.add(a[13], "pos", i32), items.add(a[15], "rows", i32);
     int rp[2], pos0, row0, d[5];
     if (!items.check(fn) || !ints(a + 11, 2, rp) || !ints(a + 14, 1, &pos0) || !ints(a + 16, 1, &row0) || !ints(a + 17, 5, d)) return nullptr;
@@ -897,13 +897,15 @@ PyObject* append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (eps == -1.0 && PyErr_Occurred()) return nullptr;
     const Call c(a[6]);
     void *xq = ptr(a[0]), *xk = ptr(a[1]), *xv = ptr(a[2]), *qo = ptr(a[5]), *k = ptr(a[6]), *v = ptr(a[7]), *st = c.st();
-    float *gq = opt_ptr<float>(a[3]), *gk = opt_ptr<float>(a[4]), *cs = opt_ptr<float>(a[9]), *sn = opt_ptr<float>(a[10]);
+    float *gq = opt_ptr<float>(a[3]), *gk = opt_ptr<float>(a[4]), *cs = opt_ptr<float>(a[9]), *sn = opt_ptr<float>(a[10]), *w = opt_ptr<float>(a[23]);
     int *ps = opt_ptr<int>(a[8]), *pos = opt_ptr<int>(a[13]), *rows = opt_ptr<int>(a[15]);
     int rc;
     {
         const NoGil no_gil;
-        rc = b200attn_kv_append_rotary(xq, xk, xv, xd, qo, k, v, ps, gq, gk, cs, sn, int(n_pos), rp[0], rp[1], pos, pos0, rows, row0, B, int(n_new),
-                                       L_cap, Hq, Hkv, D, static_cast<float>(eps), st);
+        rc = w ? b200attn_kv_append_weights(xq, xk, xv, xd, qo, k, v, ps, w, gq, gk, cs, sn, int(n_pos), rp[0], rp[1], pos, pos0, rows, row0, B,
+                                            int(n_new), L_cap, Hq, Hkv, D, static_cast<float>(eps), st)
+               : b200attn_kv_append_rotary(xq, xk, xv, xd, qo, k, v, ps, gq, gk, cs, sn, int(n_pos), rp[0], rp[1], pos, pos0, rows, row0, B,
+                                           int(n_new), L_cap, Hq, Hkv, D, static_cast<float>(eps), st);
     }
     return finish(rc, fn);
     B200ATTN_CATCH

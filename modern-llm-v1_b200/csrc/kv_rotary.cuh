@@ -4,7 +4,8 @@
 // is noted where the cache keeps positions.
 //
 //   q rows [B, n_new, Hq, D]  -> rotated at pos + t (norm) -> BF16 q_out [B, Hq, n_new, D]
-//   k rows [B, n_new, Hkv, D] -> rotated at pos + t (norm) -> BF16 kcache[b, h, row + t, :],  positions[b, h, row + t] = pos + t
+//   k rows [B, n_new, Hkv, D] -> rotated at pos + t (norm) -> BF16 kcache[b, h, row + t, :],  positions[b, h, row + t] = pos + t,
+//                                                             weights[b, h, row + t] = 0: whatever token the row held before
 //   v rows                    -> BF16 vcache[b, h, row + t, :]
 //
 // The same deal of rows to lanes as kv_append_kernel: latency at one token, HBM bytes for a prompt.  The row arithmetic is rotary.cuh's,
@@ -19,6 +20,7 @@ namespace b200attn {
 struct KvRotaryParams : KvAppendParams {
     const int* rows;  // [B] first cache row per sequence, or nullptr: row0
     int* positions;   // [B, Hkv, L_cap] or nullptr
+    float* weights;   // the same
     int row0, n_pos, R;
 };
 
@@ -100,6 +102,7 @@ kv_rotary_kernel(const __grid_constant__ KvRotaryParams p) {
         } else {
             rotary_store8<false, HALF>(p.kcache, at * D, rl.at, rl.more, rot);
             if (p.positions && li == 0) p.positions[at] = int(pos);
+            if (p.weights && li == 0) p.weights[at] = 0.f;
         }
     }
 }

@@ -108,6 +108,47 @@ int launch_kv_rotary(const KvRotaryParams& p, cudaStream_t st) {
     return B200ATTN_OK;
 }
 
+int kv_append_rotary_run(const void* xq, const void* xk, const void* xv, int x_dtype, void* q_out, void* kcache, void* vcache, int* positions,
+                         float* weights, const float* gamma_q, const float* gamma_k, const float* cos_t, const float* sin_t, int n_pos, int R,
+                         int pairs, const int* pos, int pos0, const int* rows, int row0, int B, int n_new, int L_cap, int Hq, int Hkv, int D,
+                         float eps, void* stream) {
+    if (B <= 0 || n_new <= 0 || pos0 < 0 || row0 < 0 || L_cap <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || n_pos <= 0) return B200ATTN_ERR_INVALID_ARG;
+    if (Hq % Hkv != 0 || (long long)(rows ? 0 : row0) + n_new > L_cap || (long long)(pos ? 0 : pos0) + n_new > n_pos) return B200ATTN_ERR_INVALID_ARG;
+    if (x_dtype != B200ATTN_DTYPE_BF16 && x_dtype != B200ATTN_DTYPE_F32) return B200ATTN_ERR_INVALID_ARG;
+    int rc = rotary_check_pairs(D, R, pairs);
+    if (rc) return rc;
+    if (!xq || !xk || !xv || !q_out || !kcache || !vcache || !cos_t || !sin_t || (gamma_q != nullptr) != (gamma_k != nullptr))
+        return B200ATTN_ERR_INVALID_ARG;
+    for (const void* a : {xq, xk, xv, (const void*)q_out, (const void*)kcache, (const void*)vcache, (const void*)gamma_q, (const void*)gamma_k,
+                          (const void*)cos_t, (const void*)sin_t})
+        if (!aligned16(a)) return B200ATTN_ERR_ALIGNMENT;
+    const long long rows_q = (long long)B * n_new * Hq, rows_kv = (long long)B * n_new * Hkv;
+    if (rows_q + 2 * rows_kv >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
+    KvRotaryParams p = {};
+    p.status = status_ptr(&rc);
+    if (!p.status) return rc;
+    p.pos = pos, p.pos0 = pos0, p.rows = rows, p.row0 = row0, p.positions = positions, p.weights = weights, p.n_pos = n_pos, p.R = R;
+    p.xq = xq, p.xk = xk, p.xv = xv;
+    p.q_out = static_cast<uint16_t*>(q_out);
+    p.kcache = static_cast<uint16_t*>(kcache);
+    p.vcache = static_cast<uint16_t*>(vcache);
+    p.gamma_q = gamma_q, p.gamma_k = gamma_k, p.cos_t = cos_t, p.sin_t = sin_t;
+    p.B = B, p.n_new = n_new, p.L_cap = L_cap, p.Hq = Hq, p.Hkv = Hkv;
+    p.rows_q = (unsigned)rows_q, p.rows_kv = (unsigned)rows_kv;
+    p.div_hq = fastdiv_make((unsigned)Hq), p.div_hkv = fastdiv_make((unsigned)Hkv), p.div_n = fastdiv_make((unsigned)n_new);
+    p.eps = eps;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool f32 = x_dtype == B200ATTN_DTYPE_F32, half = pairs == B200ATTN_PAIRS_HALF, norm = gamma_q != nullptr;
+    using std::integral_constant;
+    const integral_constant<bool, true> yes;
+    const integral_constant<bool, false> no;
+    auto go = [&](auto d, auto f, auto h, auto n) { return launch_kv_rotary<d.value, f.value, h.value, n.value>(p, st); };
+    auto by_norm = [&](auto d, auto f, auto h) { return norm ? go(d, f, h, yes) : go(d, f, h, no); };
+    auto by_half = [&](auto d, auto f) { return half ? by_norm(d, f, yes) : by_norm(d, f, no); };
+    auto by_type = [&](auto d) { return f32 ? by_half(d, yes) : by_half(d, no); };
+    return D == 64 ? by_type(integral_constant<int, 64>()) : by_type(integral_constant<int, 128>());
+}
+
 }  // namespace
 
 extern "C" int b200attn_rotary_table(int T, int R, double base, int scaling, double factor, double trained, double turns_fast,
@@ -158,39 +199,15 @@ extern "C" int b200attn_kv_append_rotary(const void* xq, const void* xk, const v
                                          int* positions, const float* gamma_q, const float* gamma_k, const float* cos_t, const float* sin_t,
                                          int n_pos, int R, int pairs, const int* pos, int pos0, const int* rows, int row0, int B, int n_new,
                                          int L_cap, int Hq, int Hkv, int D, float eps, void* stream) {
-    if (B <= 0 || n_new <= 0 || pos0 < 0 || row0 < 0 || L_cap <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || n_pos <= 0) return B200ATTN_ERR_INVALID_ARG;
-    if (Hq % Hkv != 0 || (long long)(rows ? 0 : row0) + n_new > L_cap || (long long)(pos ? 0 : pos0) + n_new > n_pos) return B200ATTN_ERR_INVALID_ARG;
-    if (x_dtype != B200ATTN_DTYPE_BF16 && x_dtype != B200ATTN_DTYPE_F32) return B200ATTN_ERR_INVALID_ARG;
-    int rc = rotary_check_pairs(D, R, pairs);
-    if (rc) return rc;
-    if (!xq || !xk || !xv || !q_out || !kcache || !vcache || !cos_t || !sin_t || (gamma_q != nullptr) != (gamma_k != nullptr))
-        return B200ATTN_ERR_INVALID_ARG;
-    for (const void* a : {xq, xk, xv, (const void*)q_out, (const void*)kcache, (const void*)vcache, (const void*)gamma_q, (const void*)gamma_k,
-                          (const void*)cos_t, (const void*)sin_t})
-        if (!aligned16(a)) return B200ATTN_ERR_ALIGNMENT;
-    const long long rows_q = (long long)B * n_new * Hq, rows_kv = (long long)B * n_new * Hkv;
-    if (rows_q + 2 * rows_kv >= (1LL << 31)) return B200ATTN_ERR_TOO_LARGE;
-    KvRotaryParams p = {};
-    p.status = status_ptr(&rc);
-    if (!p.status) return rc;
-    p.pos = pos, p.pos0 = pos0, p.rows = rows, p.row0 = row0, p.positions = positions, p.n_pos = n_pos, p.R = R;
-    p.xq = xq, p.xk = xk, p.xv = xv;
-    p.q_out = static_cast<uint16_t*>(q_out);
-    p.kcache = static_cast<uint16_t*>(kcache);
-    p.vcache = static_cast<uint16_t*>(vcache);
-    p.gamma_q = gamma_q, p.gamma_k = gamma_k, p.cos_t = cos_t, p.sin_t = sin_t;
-    p.B = B, p.n_new = n_new, p.L_cap = L_cap, p.Hq = Hq, p.Hkv = Hkv;
-    p.rows_q = (unsigned)rows_q, p.rows_kv = (unsigned)rows_kv;
-    p.div_hq = fastdiv_make((unsigned)Hq), p.div_hkv = fastdiv_make((unsigned)Hkv), p.div_n = fastdiv_make((unsigned)n_new);
-    p.eps = eps;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool f32 = x_dtype == B200ATTN_DTYPE_F32, half = pairs == B200ATTN_PAIRS_HALF, norm = gamma_q != nullptr;
-    using std::integral_constant;
-    const integral_constant<bool, true> yes;
-    const integral_constant<bool, false> no;
-    auto go = [&](auto d, auto f, auto h, auto n) { return launch_kv_rotary<d.value, f.value, h.value, n.value>(p, st); };
-    auto by_norm = [&](auto d, auto f, auto h) { return norm ? go(d, f, h, yes) : go(d, f, h, no); };
-    auto by_half = [&](auto d, auto f) { return half ? by_norm(d, f, yes) : by_norm(d, f, no); };
-    auto by_type = [&](auto d) { return f32 ? by_half(d, yes) : by_half(d, no); };
-    return D == 64 ? by_type(integral_constant<int, 64>()) : by_type(integral_constant<int, 128>());
+    return kv_append_rotary_run(xq, xk, xv, x_dtype, q_out, kcache, vcache, positions, nullptr, gamma_q, gamma_k, cos_t, sin_t, n_pos, R, pairs,
+                                pos, pos0, rows, row0, B, n_new, L_cap, Hq, Hkv, D, eps, stream);
+}
+
+extern "C" int b200attn_kv_append_weights(const void* xq, const void* xk, const void* xv, int x_dtype, void* q_out, void* kcache, void* vcache,
+                                          int* positions, float* weights, const float* gamma_q, const float* gamma_k, const float* cos_t,
+                                          const float* sin_t, int n_pos, int R, int pairs, const int* pos, int pos0, const int* rows, int row0,
+                                          int B, int n_new, int L_cap, int Hq, int Hkv, int D, float eps, void* stream) {
+    if (!weights) return B200ATTN_ERR_INVALID_ARG;
+    return kv_append_rotary_run(xq, xk, xv, x_dtype, q_out, kcache, vcache, positions, weights, gamma_q, gamma_k, cos_t, sin_t, n_pos, R, pairs,
+                                pos, pos0, rows, row0, B, n_new, L_cap, Hq, Hkv, D, eps, stream);
 }

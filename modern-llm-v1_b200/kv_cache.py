@@ -147,7 +147,8 @@ class KVCache:
     def set_lengths(self, lengths) -> None:
         """Gives every sequence its own length (e.g. after a padded prompt batch went through `append` /
         `attend` / `advance` with the longest prompt's length): rows at and beyond a sequence's length are
-        treated as not yet written."""
+        treated as not yet written.  With track_weights those rows' weights become 0 and their positions -1; what their tokens gave to the
+        rows that stay remains."""
         host = [int(x) for x in lengths]
         if len(host) != self.B or min(host) < 0 or max(host) > self.L_cap:
             raise ValueError("KVCache.set_lengths: need B lengths in [0, L_cap]")
@@ -157,12 +158,17 @@ class KVCache:
         self.length = max(host)
         self.lengths = torch.tensor(host, dtype=torch.int32, device=self.device)
         self._lens_next = self.lengths + 1
+        if self.track_weights:
+            gone = torch.arange(self.L_cap, device=self.device) >= self.lengths[:, None, None]
+            for w, p in zip(self.weights, self.positions):
+                w.masked_fill_(gone, 0.0)
+                p.masked_fill_(gone, -1)
 
     def append(self, layer: int, xq, xk, xv, gamma_q, gamma_k, q_out) -> None:
         """xq [B, n_new, Hq, D], xk / xv [B, n_new, Hkv, D] (the projection outputs, FP32 or BF16, all the
         same type) are the n_new tokens after the `length` cached ones.  Writes q_out [B, Hq, n_new, D] BF16
         (rotated, normalised, times gamma_q) and the tokens' rows of this layer's K (same chain with gamma_k)
-        and V (converted to BF16).  Except in a cache with the reference's rotation and nothing else, gamma_q and gamma_k may both be
+        and V (converted to BF16); with track_weights these rows begin without weight.  Except in a cache with the reference's rotation and nothing else, gamma_q and gamma_k may both be
         None: no norm."""
         if self._plain:
             _lib.host().kv_append(self, layer, xq, xk, xv, gamma_q, gamma_k, q_out)
@@ -175,7 +181,8 @@ class KVCache:
             raise ValueError("KVCache.append: one token per sequence once the lengths differ")
         _lib.host().append_rotary(xq, xk, xv, gamma_q, gamma_k, q_out, self._kl[layer], self._vl[layer],
                                   self.positions[layer] if self.track_weights else None, self.cos, self.sin, self._R, self._pairs, pos, pos0,
-                                  rows, self.length, self.B, self.L_cap, self.Hq, self.Hkv, self.D, self.eps)
+                                  rows, self.length, self.B, self.L_cap, self.Hq, self.Hkv, self.D, self.eps,
+                                  self.weights[layer] if self.track_weights else None)
 
     def _layer_ok(self, what, layer):
         if not 0 <= layer < self.n_layers:
