@@ -46,24 +46,25 @@ class KVCache:
     _shift, _pos, _evicted, _prompts = 0, None, False, None
 
     def __init__(self, n_layers: int, B: int, Hq: int, Hkv: int, D: int, L_cap: int, device="cuda",
-                 rope_base: float = 10000.0, eps: float = 1e-5, *, rotary_dim=None, pairs="interleaved", scaling="none",
+                 rope_base=None, eps=None, *, rotary_dim=None, pairs="interleaved", scaling="none",
                  factor: float = 1.0, trained=None, T_max=None, prefix=None, track_weights: bool = False):
+        """rope_base is 10000 and eps 1e-5 where they are left out, or what the prompts' cache has (`prefix`)."""
         if min(n_layers, B, Hq, Hkv, D, L_cap) <= 0 or Hq % Hkv != 0:
             raise ValueError("KVCache: sizes must be positive and Hq a multiple of Hkv")
         if D not in (64, 128):
             raise ValueError("KVCache: d_h must be 64 or 128")
         _lib.load()  # fail now, not at the first token, when the CUDA library is missing
         self.n_layers, self.B, self.Hq, self.Hkv, self.D, self.L_cap = n_layers, B, Hq, Hkv, D, L_cap
-        self.eps = float(eps)
+        self.eps = 1e-5 if eps is None else float(eps)
         self.device = torch.device(device)
         self.k = torch.zeros((n_layers, B, Hkv, L_cap, D), dtype=torch.bfloat16, device=self.device)
         self.v = torch.zeros_like(self.k)
         self.prefix, self.track_weights = prefix, bool(track_weights)
         own = (rotary_dim, pairs, scaling) != (None, "interleaved", "none")
         if prefix is None:
-            self._rotary_setup(rope_base, rotary_dim, pairs, scaling, factor, trained, T_max, own)
+            self._rotary_setup(10000.0 if rope_base is None else rope_base, rotary_dim, pairs, scaling, factor, trained, T_max, own)
         else:
-            self._prefix_setup(prefix, own, T_max)
+            self._prefix_setup(prefix, own, T_max, rope_base, eps, factor, trained)
         if self.track_weights:
             if prefix is not None:
                 raise ValueError("KVCache: a cache that continues shared prompts keeps no weights")
@@ -102,9 +103,10 @@ class KVCache:
             return make_rope_cache(T, self.D, self._base, device=self.device)
         return make_rotary_cache(T, self._R, self._base, scaling, factor, trained, device=self.device)
 
-    def _prefix_setup(self, prefix, own, T_max):
-        if own or T_max is not None:
-            raise ValueError("KVCache: a cache that continues prompts rotates as theirs does")
+    def _prefix_setup(self, prefix, own, T_max, base, eps, factor, trained):
+        given = [(base, prefix._base), (eps, prefix.eps), (None if factor == 1.0 else factor, prefix._scaled[1]), (trained, prefix._scaled[2])]
+        if own or T_max is not None or any(x is not None and x != theirs for x, theirs in given):
+            raise ValueError("KVCache: a cache that continues prompts rotates and normalises as theirs does")
         if (prefix.n_layers, prefix.Hq, prefix.Hkv, prefix.D) != (self.n_layers, self.Hq, self.Hkv, self.D) or prefix.prefix is not None:
             raise ValueError("KVCache: prefix must be a cache of prompts with the same layers and heads")
         if prefix.track_weights:
@@ -112,7 +114,7 @@ class KVCache:
         if self.B % prefix.B != 0:
             raise ValueError("KVCache: B must be a multiple of the number of prompts")
         self._R, self._pairs, self._scaled, self._base, self._reference = prefix._R, prefix._pairs, prefix._scaled, prefix._base, prefix._reference
-        self._plain = False
+        self._plain, self.eps = False, prefix.eps
         self.cos, self.sin = self._tables(prefix.L_cap + self.L_cap)
 
     def reset(self) -> None:
