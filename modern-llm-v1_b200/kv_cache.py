@@ -44,6 +44,7 @@ class KVCache:
     # the reference's rotation, a cache of its own, no weights
     _plain, prefix, track_weights = True, None, False
     _shift, _pos, _evicted, _prompts = 0, None, False, None
+    _changes = 0  # times that the tokens which count have changed
 
     def __init__(self, n_layers: int, B: int, Hq: int, Hkv: int, D: int, L_cap: int, device="cuda",
                  rope_base=None, eps=None, *, rotary_dim=None, pairs="interleaved", scaling="none",
@@ -119,6 +120,7 @@ class KVCache:
 
     def reset(self) -> None:
         """Forgets every token (the buffers keep their bytes; rows >= length are never read)."""
+        self._changes += 1
         self.length = 0
         self.lengths = self._lens_next = self._lengths_host = None
         self._shift, self._pos, self._evicted, self._prompts = 0, None, False, None
@@ -133,10 +135,10 @@ class KVCache:
         if self.prefix is not None and self._prompts is None:
             if self.prefix.length == 0:
                 raise ValueError("KVCache: the prompts are empty")
-            self._shift, self._prompts = self.prefix.length, (self.prefix.length, self.prefix.lengths)
+            self._shift, self._prompts = self.prefix.length, self.prefix._changes
             if self.prefix.lengths is not None:
                 self._pos = self.prefix.lengths.repeat_interleave(self.B // self.prefix.B)
-        elif self.prefix is not None and (self.prefix.length != self._prompts[0] or self.prefix.lengths is not self._prompts[1]):
+        elif self.prefix is not None and self.prefix._changes != self._prompts:
             raise ValueError("KVCache: the prompts have changed since their first continuation (reset this cache)")
         return self.length + self._shift, self._pos, self.lengths
 
@@ -156,6 +158,7 @@ class KVCache:
             raise ValueError("KVCache.set_lengths: need B lengths in [0, L_cap]")
         if self._evicted or self.prefix is not None:
             raise ValueError("KVCache.set_lengths: not after an eviction, nor behind shared prompts")
+        self._changes += 1
         self._lengths_host = host
         self.length = max(host)
         self.lengths = torch.tensor(host, dtype=torch.int32, device=self.device)
@@ -237,6 +240,7 @@ class KVCache:
                                  recent, self.lengths, self.L_cap)
             self._spare = (self.weights[i], self.positions[i])
             self.weights[i], self.positions[i] = w2, p2
+        self._changes += 1
         self._evicted = True
         if self.lengths is None:
             self._shift += self.length - keep
@@ -252,6 +256,7 @@ class KVCache:
         """Call once per step, after every layer has appended and attended."""
         if n_new <= 0 or self.length + n_new > self.L_cap:
             raise ValueError("KVCache.advance: n_new out of range")
+        self._changes += 1
         self.length += n_new
         if self.lengths is not None:
             self._lengths_host = [x + n_new for x in self._lengths_host]

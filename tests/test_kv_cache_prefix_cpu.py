@@ -25,3 +25,28 @@ def test_a_rotation_of_its_own_is_refused():
         own = new(prefix=prompts, **kw)
         assert own.cos.shape == (16, 32) and (own.cos[:8] == prompts.cos).all() and (own.sin[:8] == prompts.sin).all()
     assert (new().cos == new(rope_base=10000.0).cos).all()
+
+
+@pytest.mark.parametrize("how", ["refilled", "same lengths again", "longer and back"])
+def test_prompts_that_have_changed_are_noticed(how):
+    """also where they have the same length as before"""
+    prompts = new()
+    prompts.advance(5)
+    samples = new(prefix=prompts)
+    assert samples.next_position == 5
+    samples.advance()
+    assert samples.next_position == 6
+    if how == "refilled":
+        prompts.reset()
+        prompts.advance(5)
+    elif how == "same lengths again":
+        prompts.set_lengths([5, 5])
+    else:
+        prompts.advance(1)
+        prompts.reset()
+        prompts.advance(5)
+    with pytest.raises(ValueError, match="prompts have changed"):
+        samples.next_position
+    samples.reset()
+    at = samples.next_position
+    assert at == 5 if how != "same lengths again" else at.tolist() == [5, 5]
