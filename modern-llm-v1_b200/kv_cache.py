@@ -12,8 +12,8 @@ prompts of different lengths); from then on `append` and `attend` take one token
 sequence's own position.
 
 For long contexts a cache can also
-  - rotate in other layouts (`pairs`, `rotary_dim`), with scaled frequencies (`scaling`, `factor`, `trained`) and without the
-    QK-norm (gammas None), see rotary.py;
+  - rotate in other layouts (`pairs`, `rotary_dim`), with scaled frequencies (`scaling`, `factor`, `trained`, `turns_fast`,
+    `turns_slow`) and without the QK-norm (gammas None), see rotary.py;
   - continue prompts that several of its sequences share (`prefix`: a KVCache that holds them; sequence b continues prompt
     b // (B // prefix.B)): the prompts' keys and values are kept and read once, not once per sequence;
   - keep the attention weight that each cached key has received and its position (`track_weights`), and cut itself down by it
@@ -48,8 +48,10 @@ class KVCache:
 
     def __init__(self, n_layers: int, B: int, Hq: int, Hkv: int, D: int, L_cap: int, device="cuda",
                  rope_base=None, eps=None, *, rotary_dim=None, pairs="interleaved", scaling="none",
-                 factor: float = 1.0, trained=None, T_max=None, prefix=None, track_weights: bool = False):
-        """rope_base is 10000 and eps 1e-5 where they are left out, or what the prompts' cache has (`prefix`)."""
+                 factor: float = 1.0, trained=None, T_max=None, prefix=None, track_weights: bool = False, turns_fast=None,
+                 turns_slow=None):
+        """rope_base is 10000 and eps 1e-5 where they are left out, or what the prompts' cache has (`prefix`); turns_fast and
+        turns_slow are make_rotary_cache's, for "parts"."""
         if min(n_layers, B, Hq, Hkv, D, L_cap) <= 0 or Hq % Hkv != 0:
             raise ValueError("KVCache: sizes must be positive and Hq a multiple of Hkv")
         if D not in (64, 128):
@@ -61,11 +63,12 @@ class KVCache:
         self.k = torch.zeros((n_layers, B, Hkv, L_cap, D), dtype=torch.bfloat16, device=self.device)
         self.v = torch.zeros_like(self.k)
         self.prefix, self.track_weights = prefix, bool(track_weights)
+        turns = (turns_fast, turns_slow)
         own = (rotary_dim, pairs, scaling) != (None, "interleaved", "none")
         if prefix is None:
-            self._rotary_setup(10000.0 if rope_base is None else rope_base, rotary_dim, pairs, scaling, factor, trained, T_max, own)
+            self._rotary_setup(10000.0 if rope_base is None else rope_base, rotary_dim, pairs, scaling, factor, trained, turns, T_max, own)
         else:
-            self._prefix_setup(prefix, own, T_max, rope_base, eps, factor, trained)
+            self._prefix_setup(prefix, own, T_max, rope_base, eps, factor, trained, turns)
         if self.track_weights:
             if prefix is not None:
                 raise ValueError("KVCache: a cache that continues shared prompts keeps no weights")
@@ -84,7 +87,7 @@ class KVCache:
         self._lens_next = None  # lengths + 1: what the decode kernel reads while the newest token is being attended
         self._lengths_host = None
 
-    def _rotary_setup(self, base, rotary_dim, pairs, scaling, factor, trained, T_max, own):
+    def _rotary_setup(self, base, rotary_dim, pairs, scaling, factor, trained, turns, T_max, own):
         R = self.D if rotary_dim is None else int(rotary_dim)
         if pairs not in ("interleaved", "half"):
             raise ValueError("KVCache: pairs must be interleaved or half")
@@ -93,19 +96,20 @@ class KVCache:
         T = self.L_cap if T_max is None else int(T_max)
         if T < self.L_cap:
             raise ValueError("KVCache: T_max is less than the capacity")
-        self._R, self._pairs, self._scaled, self._base = R, _lib.PAIRS_HALF if pairs == "half" else _lib.PAIRS_INTERLEAVED, (scaling, factor, trained), base
+        self._R, self._pairs, self._base = R, _lib.PAIRS_HALF if pairs == "half" else _lib.PAIRS_INTERLEAVED, base
+        fast, slow = (default if x is None else float(x) for x, default in zip(turns, (32.0, 1.0)))
+        self._scaled = (scaling, factor, trained, fast, slow)
         self._reference = not own
         self._plain = not own and not self.track_weights and T_max is None  # the reference's rotation, rows are positions
         self.cos, self.sin = self._tables(T)
 
     def _tables(self, T):
-        scaling, factor, trained = self._scaled
         if self._reference:  # the reference's rotation has its values, of angles in 32 bits
             return make_rope_cache(T, self.D, self._base, device=self.device)
-        return make_rotary_cache(T, self._R, self._base, scaling, factor, trained, device=self.device)
+        return make_rotary_cache(T, self._R, self._base, *self._scaled, device=self.device)
 
-    def _prefix_setup(self, prefix, own, T_max, base, eps, factor, trained):
-        given = [(base, prefix._base), (eps, prefix.eps), (None if factor == 1.0 else factor, prefix._scaled[1]), (trained, prefix._scaled[2])]
+    def _prefix_setup(self, prefix, own, T_max, base, eps, factor, trained, turns):
+        given = [(base, prefix._base), (eps, prefix.eps), *zip((None if factor == 1.0 else factor, trained, *turns), prefix._scaled[1:])]
         if own or T_max is not None or any(x is not None and x != theirs for x, theirs in given):
             raise ValueError("KVCache: a cache that continues prompts rotates and normalises as theirs does")
         if (prefix.n_layers, prefix.Hq, prefix.Hkv, prefix.D) != (self.n_layers, self.Hq, self.Hkv, self.D) or prefix.prefix is not None:
