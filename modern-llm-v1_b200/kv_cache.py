@@ -150,7 +150,7 @@ class KVCache:
     def next_position(self):
         """The position of the next token: an int, or int32 [B] on the device where the sequences differ."""
         pos0, pos, rows = self._place()
-        return pos if pos is not None else pos0 if rows is None else rows + self._shift
+        return pos.clone() if pos is not None else pos0 if rows is None else rows + self._shift
 
     def set_lengths(self, lengths) -> None:
         """Gives every sequence its own length (e.g. after a padded prompt batch went through `append` /

@@ -50,3 +50,16 @@ def test_prompts_that_have_changed_are_noticed(how):
     samples.reset()
     at = samples.next_position
     assert at == 5 if how != "same lengths again" else at.tolist() == [5, 5]
+
+
+def test_positions_that_were_asked_for_stay_what_they_were():
+    """also after the next token: the cache counts on in a tensor of its own"""
+    prompts = new()
+    prompts.advance(5)
+    prompts.set_lengths([5, 3])
+    samples = new(prefix=prompts)
+    at = samples.next_position
+    samples.advance()
+    assert at.tolist() == [5, 3]
+    at.zero_()
+    assert samples.next_position.tolist() == [6, 4]
