@@ -442,6 +442,9 @@ __device__ __forceinline__ int decode_count(unsigned long long* word, unsigned l
 // on who takes it.
 constexpr int kDecodeTurnBits = 24;
 constexpr int kDecodeTurnUnits = (1 << kDecodeTurnBits) - kDecodeMaxCtas;
+// The answer to ask number n, and whether it is the last of all
+__host__ __device__ __forceinline__ int decode_asked_unit(const DecodeParams& p, int n) { return n + p.turn < p.units ? n + p.turn : -1; }
+__host__ __device__ __forceinline__ bool decode_last_ask(const DecodeParams& p, int n, int n_ctas) { return n + p.turn == p.units + n_ctas - 1; }
 __device__ __forceinline__ int decode_next_unit(const DecodeParams& p, unsigned epoch, bool first, int n_ctas) {
     const unsigned long long tag = ((p.tag >> kDecodeCountBits) + epoch) << kDecodeTurnBits;
     int n = -1;
@@ -450,13 +453,12 @@ __device__ __forceinline__ int decode_next_unit(const DecodeParams& p, unsigned 
         if ((seen >> kDecodeTurnBits) != (tag >> kDecodeTurnBits) && atomicCAS(p.counters, seen, tag + 1) == seen) n = 0;
     }
     if (n < 0) n = int(atomicAdd(p.counters, 1ull) - tag);
-    n += p.turn;
-    if (n == p.units + n_ctas - 1) *p.counters = tag;
-    return n < p.units ? n : -1;
+    if (decode_last_ask(p, n, n_ctas)) *p.counters = tag;
+    return decode_asked_unit(p, n);
 }
 
 // Where the prompt's partial results of head j of the group (of sequence b, KV head hk) lie: its row in the first split's slot
-__device__ __forceinline__ size_t decode_prefix_row(const DecodePrefix& x, int b, int hk, int j, int* row) {
+__host__ __device__ __forceinline__ size_t decode_prefix_row(const DecodePrefix& x, int b, int hk, int j, int* row) {
     const int prompt = int(fastdiv(b, x.div_n)), seq = b - prompt * int(x.div_n.d);
     const int chunk = int(fastdiv(j, x.div_heads)), tile = int(fastdiv(seq, x.div_seqs));
     *row = (seq - tile * int(x.div_seqs.d)) * int(x.div_heads.d) + j - chunk * int(x.div_heads.d);

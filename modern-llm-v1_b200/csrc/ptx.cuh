@@ -241,8 +241,12 @@ inline FastDiv fastdiv_make(unsigned d) {
     f.shr = p - 32;
     return f;
 }
-__device__ __forceinline__ unsigned fastdiv(unsigned n, const FastDiv& f) {
+__host__ __device__ __forceinline__ unsigned fastdiv(unsigned n, const FastDiv& f) {
+#ifdef __CUDA_ARCH__
     return f.d == 1 ? n : (__umulhi(n, f.mul) >> f.shr);
+#else
+    return f.d == 1 ? n : unsigned((unsigned long long)n * f.mul >> 32) >> f.shr;
+#endif
 }
 
 // ---------------------------------------------------------------------------
