@@ -125,10 +125,11 @@ struct KeyWeightsCfg {
 };
 constexpr int kKeyWeightsThreads = (kKeyWeightsGroups * 4 + 3) * 32;
 
-// Units of a (batch, KV head) in front of key tile kt: tile i is seen by n_qt - max(0, i - full_kt) tiles of tokens
+// Units of a (batch, KV head) in front of key tile kt: tile i is seen by n_qt - max(0, i - full_kt) tiles of tokens.  (All units are fewer
+// than 2^31, so that kt n_qt, of which at most half is taken off, and m (m - 1) are below 2^32: unsigned.)
 __host__ __device__ __forceinline__ int key_weights_before(const KeyWeightsParams& p, int kt) {
-    const int m = kt > p.full_kt ? kt - p.full_kt : 0;
-    return (kt * p.n_qt - m * (m - 1) / 2) * p.n_hc;
+    const unsigned m = kt > p.full_kt ? kt - p.full_kt : 0;
+    return int((unsigned(kt) * unsigned(p.n_qt) - m * (m - 1) / 2) * unsigned(p.n_hc));
 }
 struct KeyWeightsItem {
     int bh, kt;        // batch * Hkv + KV head, tile of keys

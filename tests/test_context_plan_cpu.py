@@ -168,8 +168,40 @@ static int shared(Rng& rng) {
     return 0;
 }
 
-int main() {
+// chunks whose units are counted up to the last of 31 bits: the numbers on the way to a count are larger
+static int longest(Rng& rng) {
+    g_sms = 148;
+    int most = 0;
+    for (int i = 0; i < 200; ++i) {
+        KeyWeightsParams p = {};
+        const int pos0 = rng(0, 1) ? 0 : rng.log(1, 60000000), T = i < 4 ? 8388480 - i * 1000000 : rng.log(100000, 8388480), group = rng(0, 3) ? 1 : rng(1, 8);
+        key_weights_plan(p, 1, T, pos0, group, 1);
+        const long long total = key_weights_total(p, 1);
+        if (total >= (1ll << 31)) continue;
+        key_weights_deal(p, int(total));
+        auto before = [&](int kt) {
+            const long long m = std::max(0, kt - p.full_kt);
+            return ((long long)kt * p.n_qt - m * (m - 1) / 2) * p.n_hc;
+        };
+        for (int e = 0; e < 2000; ++e) {
+            const int kt = e < 8 ? p.n_kt - e : rng(0, p.n_kt);
+            CHECK(kt < 0 || key_weights_before(p, kt) == before(kt));
+        }
+        for (int c : {0, 1, p.n_ctas / 2, p.n_ctas - 2, p.n_ctas - 1})
+            for (int u : {key_weights_range(p, c), key_weights_range(p, c + 1) - 1}) {
+                const KeyWeightsItem it = key_weights_item(p, u);
+                CHECK(it.bh == 0 && it.kt >= 0 && it.kt < p.n_kt && it.start == before(it.kt) && it.units == before(it.kt + 1) - before(it.kt));
+                CHECK(it.start <= u && u < it.start + it.units && key_weights_cta(p, u) == c);
+            }
+        most = std::max(most, p.total);
+    }
+    CHECK(most > (1 << 30));
+    return 0;
+}
+
+int main(int argc, char**) {
     Rng rng{std::mt19937(3)};
+    if (argc > 1) return longest(rng);
     for (int i = 0; i < 1000; ++i)
         if (key_weights(rng)) return 1;
     for (int i = 0; i < 1000; ++i)
@@ -192,3 +224,8 @@ def test_the_plans_that_ship(driver):
     out = subprocess.run([driver], capture_output=True, text=True, timeout=600)
     assert out.returncode == 0, out.stdout
     assert all(int(n) > 100 for n in out.stdout.split()), out.stdout  # deals of every kind were among them
+
+
+def test_the_longest_chunks(driver):
+    out = subprocess.run([driver, "longest"], capture_output=True, text=True, timeout=600)
+    assert out.returncode == 0, out.stdout
