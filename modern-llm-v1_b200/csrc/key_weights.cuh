@@ -212,7 +212,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         for (int i = tid; i < NST * Cfg::kTileBytes / 16; i += NG * 128) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
     }
-    if (tid < 128) sTok[tid] = tid % p.tokens;
+    if (tid < 128) sTok[tid] = tid < cols ? tid % p.tokens : INT_MAX / 2;  // (no token: behind all that count)
     grid_dep_wait();
     if (tid == 0) {
         const int failed = *reinterpret_cast<volatile int*>(p.status);
@@ -231,6 +231,10 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         *hc = in_item - q * p.n_hc;
         return p.n_qt - 1 - q;
     };
+    // A tile's first token.  The last tile ends with the last token, whatever it has in common with the tile in front (the lse of which counts
+    // those tokens once): every column is a query row then, where rows of zeros would score NaN with a key that holds an infinity.
+    const int last_tile = p.T - p.tokens;
+    auto tile_token = [&](int qt) { return min(qt * p.tokens, last_tile); };
 
     if (*abort_flag != 0) {
         // an earlier kernel has failed
@@ -258,7 +262,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     mbar_arrive_expect_tx(&bar_q_full[s], cols * D * 2);
 #pragma unroll
                     for (int bx = 0; bx < Cfg::kBoxes; ++bx)
-                        tma_load_4d(sQ + s * Cfg::kTileBytes + bx * Cfg::kBoxBytes, &tmQ, &bar_q_full[s], bx * 64, qt * p.tokens, hk * p.group + hc * p.heads, b);
+                        tma_load_4d(sQ + s * Cfg::kTileBytes + bx * Cfg::kBoxBytes, &tmQ, &bar_q_full[s], bx * 64, tile_token(qt), hk * p.group + hc * p.heads, b);
                 }
                 __syncwarp();
             }
@@ -313,9 +317,9 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int qt = unit_qt(in_item, &hc);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int t = qt * p.tokens + t_col[c];
+                const int t = tile_token(qt) + t_col[c];
                 // 2^(x - inf) = 0
-                v[c] = lane + 32 * c < cols && t < T ? __ldg(rows + size_t(hc * p.heads + h_col[c]) * p.T + t) * -kLog2e : -INFINITY;
+                v[c] = lane + 32 * c < cols && t >= qt * p.tokens && t < T ? __ldg(rows + size_t(hc * p.heads + h_col[c]) * p.T + t) * -kLog2e : -INFINITY;
             }
             if (++in_item == it.units) {
                 const int bh = it.bh;
@@ -352,11 +356,12 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const int first = u0 + i - it.start, m = min(it.units - first, n - i);
             float acc = 0.f;
             const int k_lim = it.kt * 128 + key - p.pos0;  // tokens below it do not see the key
-            const int rows = p.rows ? __ldg(p.rows + it.bh / p.Hkv) : INT_MAX;
+            const int rows = p.rows ? __ldg(p.rows + it.bh / p.Hkv) : p.T;
             for (int e = (wg - i % NG + NG) % NG; e < m; e += NG) {
                 int hc;
-                const int k = i + e, t_first = unit_qt(first + e, &hc) * p.tokens, lim = k_lim - t_first;
-                const bool padding = t_first + p.tokens > rows;  // some query rows do not count: whatever they hold
+                const int k = i + e, t_first = tile_token(unit_qt(first + e, &hc)), lim = k_lim - t_first;
+                // chunks that end behind it have columns that do not count: whatever their rows hold, and the key
+                const int padding = t_first + p.tokens > rows ? 0 : cols;
                 const bool diagonal = lim + 127 - key > 0;  // whether any key of the tile is unseen by the unit's first token
                 const float* lse = sLse + (wg * 2 + (k / NG & 1)) * 128;
                 ok = mbar_wait_warp(&bar_s_full[wg], uint32_t(k / NG) & 1, abort_flag, p.status, DEV_WAIT_TIMEOUT_MMA);
@@ -365,7 +370,7 @@ key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 uint64_t sum2[2] = {0ull, 0ull};
                 uint32_t v[2][16];
                 auto chunk = [&](int c, uint32_t (&v)[16]) {
-                    if (padding) {
+                    if (c * 16 + 16 > padding) {
 #pragma unroll
                         for (int x = 0; x < 16; ++x)
                             if (t_first + sTok[c * 16 + x] >= rows) v[x] = 0u;
