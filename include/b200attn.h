@@ -237,7 +237,8 @@ int b200attn_decode_ragged(const void* q, const void* kcache, const void* vcache
  *
  * x: B*T*H rows of D elements, BF16 or FP32 (x_dtype), in either layout (x_layout; BTHD is the projection
  * output read in place).  y: BF16 in y_layout (what b200attn_fwd takes).  rstd: FP32 [B, H, T], the row order of
- * the reference's rstd vector.  gamma: FP32 [D].  cos_t, sin_t: FP32 [T, D/2] device tables with the values of
+ * the reference's rstd vector.  gamma: FP32 [D] (gamma, rstd and d_gamma may begin at any float).  cos_t, sin_t: FP32 [T, D/2] device
+ * tables, 16-byte aligned, with the values of
  * make_rope_cache (llm/src/model/rope.cu:112-128); b200attn_rope_table fills host copies of them.
  * Backward: dy BF16 in y_layout; dx in x's type and layout (overwritten); d_gamma FP32 [D] is ACCUMULATED into,
  * as in the reference (llm/src/model/rmsnorm.h:17), but in a fixed order (no atomics: bit-reproducible).

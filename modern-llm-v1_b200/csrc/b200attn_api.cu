@@ -605,6 +605,7 @@ int rope_norm_run(bool backward, const RopeNormTensor* t, int n_tensors, int x_d
         p[i].eps = eps;
     }
     if (!cos_t || !sin_t) return B200ATTN_ERR_INVALID_ARG;
+    if (!aligned16(cos_t) || !aligned16(sin_t)) return B200ATTN_ERR_ALIGNMENT;
     if (backward && (!workspace || workspace_bytes < b200attn_rope_norm_bwd_workspace_bytes(D) ||
                      (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
         return B200ATTN_ERR_WORKSPACE;
