@@ -41,10 +41,17 @@ def kv_evict(kcache, vcache, weights, positions, weights_out, positions_out, B, 
 
 
 class KVCache:
-    # the reference's rotation, a cache of its own, no weights
-    _plain, prefix, track_weights = True, None, False
-    _shift, _pos, _evicted, _prompts = 0, None, False, None
-    _changes = 0  # times that the tokens which count have changed
+    def __new__(cls, *args, **kwargs):
+        """The reference's rotation, a cache of its own, no weights.  (What every append, attend and advance asks are attributes of the
+        instance alone: one that the class has as well costs a lookup of some 20 ns.)"""
+        self = super().__new__(cls)
+        self._plain = self._alone = True
+        self.prefix, self.track_weights = None, False
+        self._shift = 0  # a token's position minus its row, where all sequences agree
+        self._pos = None  # else: the next token's position per sequence [B] int32 on the device
+        self._evicted, self._prompts = False, None
+        self._changes = 0  # times that the tokens which count have changed
+        return self
 
     def __init__(self, n_layers: int, B: int, Hq: int, Hkv: int, D: int, L_cap: int, device="cuda",
                  rope_base=None, eps=None, *, rotary_dim=None, pairs="interleaved", scaling="none",
@@ -63,6 +70,7 @@ class KVCache:
         self.k = torch.zeros((n_layers, B, Hkv, L_cap, D), dtype=torch.bfloat16, device=self.device)
         self.v = torch.zeros_like(self.k)
         self.prefix, self.track_weights = prefix, bool(track_weights)
+        self._alone = prefix is None and not self.track_weights
         turns = (turns_fast, turns_slow)
         own = (rotary_dim, pairs, scaling) != (None, "interleaved", "none")
         if prefix is None:
@@ -79,9 +87,6 @@ class KVCache:
             self._spare = pairs_[-1]
         # the layers' own tensors, for the calls that take them
         self._kl, self._vl = list(self.k.unbind(0)), list(self.v.unbind(0))
-        self._shift = 0  # a token's position minus its row, where all sequences agree
-        self._pos = None  # else: the next token's position per sequence [B] int32 on the device
-        self._evicted = False
         self.length = 0  # tokens held by every layer (the longest sequence's, once lengths differ)
         self.lengths = None  # per-sequence lengths [B] int32 on the device, once set_lengths was called
         self._lens_next = None  # lengths + 1: what the decode kernel reads while the newest token is being attended
@@ -177,11 +182,10 @@ class KVCache:
         """xq [B, n_new, Hq, D], xk / xv [B, n_new, Hkv, D] (the projection outputs, FP32 or BF16, all the
         same type) are the n_new tokens after the `length` cached ones.  Writes q_out [B, Hq, n_new, D] BF16
         (rotated, normalised, times gamma_q) and the tokens' rows of this layer's K (same chain with gamma_k)
-        and V (converted to BF16); with track_weights these rows begin without weight.  Except in a cache with the reference's rotation and nothing else, gamma_q and gamma_k may both be
-        None: no norm."""
+        and V (converted to BF16); with track_weights these rows begin without weight.  Except in a cache with the reference's
+        rotation and nothing else, gamma_q and gamma_k may both be None: no norm."""
         if self._plain:
-            _lib.host().kv_append(self, layer, xq, xk, xv, gamma_q, gamma_k, q_out)
-            return
+            return (_lib._host or _lib.host()).kv_append(self, layer, xq, xk, xv, gamma_q, gamma_k, q_out)
         self._layer_ok("append", layer)
         pos0, pos, rows = self._place()
         if rows is not None and pos is None:
@@ -205,11 +209,10 @@ class KVCache:
         Behind shared prompts: one token, over the prompt and the sequence's own tokens.  With track_weights the keys' weights grow by
         what these tokens give them; new_lens (int32 [B] on the device) says how many of the n_new tokens of each sequence are
         tokens and not padding, where the prompts of a batch differ in length (`set_lengths` follows)."""
+        if self._alone and new_lens is None:
+            return (_lib._host or _lib.host()).kv_attend(self, layer, q, ctx, lse, n_new, softmax_scale)
         if new_lens is not None and (not self.track_weights or n_new == 1):
             raise ValueError("KVCache.attend: new_lens is for several tokens at once, with track_weights")
-        if self.prefix is None and not self.track_weights:
-            _lib.host().kv_attend(self, layer, q, ctx, lse, n_new, softmax_scale)
-            return
         self._layer_ok("attend", layer)
         if n_new <= 0 or self.length + n_new > self.L_cap:
             raise ValueError("KVCache.attend: n_new out of range")
