@@ -268,7 +268,7 @@ int b200attn_rope_norm_bwd_qk(const void* dyq, const void* dyk, int y_layout, co
                               size_t workspace_bytes, void* stream);
 
 /*
- * Rotary positions in every layout, for q and k in one launch each way (the reference has one: all of the head, neighbouring pairs,
+ * Rotary positions in other layouts, for q and k in one launch each way (the reference has one: all of the head, neighbouring pairs,
  * the token's index as its position, the norm always, llm/src/model/rope.cu:25-65; that one is b200attn_rope_norm_fwd_qk).
  *
  *   The first R of a head's D elements turn (R a multiple of 16, at most D); a pair is (x[2i], x[2i+1]) with
@@ -353,8 +353,8 @@ int b200attn_kv_append_weights(const void* xq, const void* xk, const void* xv, i
  *
  * Sums are FP32 and in a fixed order: a call repeats bit for bit.  Workspaces: at least ..._workspace_bytes(...), 256-byte aligned, without
  * initialisation; calls that may overlap need workspaces of their own.  Nothing is written while the device status word is set.  (Where
- * another stream's kernel sets the word, or another thread clears it, while a call runs, that call may have written some of its
- * outputs, some (batch, KV head) pairs of an evicted cache for instance, and not others.)
+ * another stream's kernel sets the word, or another thread clears it, while a call runs, what that call leaves in its outputs, an evicted
+ * cache's rows and the weights among them, is undefined.)
  */
 int b200attn_decode_shared(const void* q, const void* kprefix, const void* vprefix, const void* kcache, const void* vcache,
                            void* o, float* lse, const int* prefix_lens, const int* lens, int B, int G, int P, int P_cap,

@@ -12,7 +12,7 @@
 // read the prompt through L2.  What a single online softmax cannot do is keep up: product, scores out of tensor memory, maximum,
 // exponentials, P back and the next product are a chain of 3300 clocks, in which an SM's share of HBM brings 64 KB, a tile at D = 128.  So
 // a CTA runs two of them, taking its tiles in turn, each with S and O of its own; the two results are joined through shared memory at
-// the end.  Up to 64 rows the second softmax has them in lanes 64 .. 127, so that each has two of the SM's four schedulers for itself.
+// the end, and a tile takes 1440 clocks at D = 64 and 2180 at D = 128.  Up to 64 rows the second softmax has them in lanes 64 .. 127, so that each has two of the SM's four schedulers for itself.
 // P goes over S's columns, which leaves room for 128 keys and two softmaxes at both head dimensions.
 //
 // Roles (576 threads): warps 0-7 the one softmax, 8-15 the other; thread = row and half of the tile's keys (two warps share a row's maximum
@@ -21,9 +21,9 @@
 // (512 columns), per softmax: S 128 with P over each half's scores, O D.
 //
 // Measured on B200, us per call, this kernel and the decode behind (G prompts, n sequences each, 16/4 heads):
-//   G=8 n=16 P<=2000 L<=300 D=64: one softmax 28.3, two, thread = row 27.0, thread = row and half 25.3; with the decode's units in turn 21.7, two splits 17.4
-//   G=1 n=64 P=16384 L=256 D=128: one softmax 31.5, two, thread = row and half 27.4, as it is 26.9 (67 MB: 2.5 TB/s)
-//   G=1 n=8 P=500 L=12 6/2 D=64: 6.9, 7.0 and 7.2 (the two launches' latency)
+//   G=8 n=16 P<=2000 L<=300 D=64: one softmax 28.3, two, thread = row 27.0, thread = row and half 25.3; with the decode's units in turn 21.7, two splits 16.6 to 17.5
+//   G=1 n=64 P=16384 L=256 D=128: one softmax 31.5, two, thread = row and half 27.4, as it is 26.1 (67 MB: 2.6 TB/s)
+//   G=1 n=8 P=500 L=12 6/2 D=64: 6.9, 7.0 and 7.0 to 7.5 (the two launches' latency)
 // Measured and dropped: tiles of 64 keys with P beside S (Q K^T takes 64 clocks a step for half the keys); two tiles of rows in a CTA, every K and
 // V tile used twice, 31.5 where two CTAs that each read them take 27.4 (the partial results of 256 rows are as many bytes as 256 keys, and
 // twice as many shares have to be joined); its results added up over a cluster through distributed shared memory (35: clusters of four

@@ -29,7 +29,8 @@ struct PrefixPlan {
     size_t slots;
 };
 // The two kernels run side by side, the prompts' one CTA per SM and the decode two on each of the others.  SMs are shared out so that the
-// longer of the two, and the join behind it, is shortest.  What a CTA takes, in us, from timing calls with every number of splits:
+// longer of the two, and the join behind it, is shortest; of a decode in shares of units only the join is counted, as if it were always done
+// when the prompts are.  What a CTA takes, in us, from timing calls with every number of splits:
 constexpr double kPrefixStart = 4.0, kUnitStart = 2.0, kDecodeTile = 0.95;  // a prompt's CTA without its tiles, a decode's unit without its tiles, one of those (32 KB)
 constexpr double prefix_tile(int D) { return D == 64 ? 0.95 : 1.1; }
 constexpr double kJoinRound = 0.7;

@@ -6,8 +6,8 @@
 //
 // One new token per sequence: the decode kernel leaves its scores (kDecodeScores) and decode_weights_kernel, behind it, has only to
 // take the exponentials against the final lse: 4 G bytes a key written and read through L2 beside the 4 D of its K and V rows, instead
-// of a second pass over K.  Measured on B200 against the decode alone, us: B=1 L=1500 16/4 D=128 8.7 and 6.1, B=32 L<=4096 16/4 D=64 22.1 and
-// 18.4: the second launch and the scores.
+// of a second pass over K.  Measured on B200 against the decode alone, us: B=1 L=1500 16/4 D=128 8.6 and 6.0, B=32 L<=4096 16/4 D=64 22.2 to 24.3
+// and 18.4: the second launch and the scores.
 //
 // A chunk of new tokens: key_weights_kernel computes S^T = K Q^T by tiles of 128 keys (lanes of tensor memory) and 128 query rows
 // (columns), so that a key's sum runs inside a thread and needs no exchange.
@@ -95,11 +95,11 @@ __global__ void __launch_bounds__(kDecodeWeightsThreads) decode_weights_kernel(c
 // of an item, a ring of Q tiles); warp 17 issues the products; warp 18 brings the columns' lse.  TMEM: four score buffers of 128 columns,
 // one per group.
 // What bounds it: 128 x 128 exponentials a unit at 16 a clock, 1024 clocks, where the products take 256 (D = 64) or 512.  A quarter of them
-// goes to the FMA pipes; a unit then takes some 1150 clocks, the special-function units at 57 %, the issue slots at 55 %, what is left
-// being the latency of four warps a scheduler.  Measured on B200, us per call: B=1 T=4000 16/4 D=64 68.7 with two groups of four warps that
-// fetched the lse themselves and joined their sums at every item's end, 61 with four groups, 54 with the lse brought by a warp of its
-// own, 49.6 with sums joined by the kernel behind; B=2, 500 tokens behind 3000, 16/4 D=128 35.7 -> 26.3, some 9 of them the two launches, the
-// first loads and the second kernel.
+// goes to the FMA pipes; a unit then takes 1280 clocks, the special-function units at 52 % (D = 64) and 44 %, the issue slots at 58 and 53 %,
+// what is left being the latency of four warps a scheduler.  Measured on B200, us per call: B=1 T=4000 16/4 D=64 68.7 with two groups of four
+// warps that fetched the lse themselves and joined their sums at every item's end, 61 with four groups, 54 with the lse brought by a warp of
+// its own, 51.5 with sums joined by the kernel behind, 52.6 with every column a query row (infinities); B=2, 500 tokens behind 3000, 16/4
+// D=128 35.7 -> 27.5, some 9 of them the two launches, the first loads and the second kernel.
 struct KeyWeightsParams {
     const float* lse;   // [B, Hq, T]
     const int* rows;    // [B] or nullptr: of the T query rows those that count (a padded batch)

@@ -11,10 +11,10 @@
 // (histograms in shared memory), numbers the free places and the rows to move, and
 //   LIST = false  moves its share of them (p.ranks CTAs per unit, each of which selects for itself): few units
 //   LIST = true   leaves them in the workspace for kv_move_kernel, whose CTAs take 128 moves each, whichever unit they are of
-// What bounds it: the moved bytes where units are many and long (B=32 L<=6000 keep=2500 4 heads D=128: 28 us, 13 of them the selection's
-// chain on one SM per unit, the rest 80 MB of moves at 5 TB/s; 45 us with one kernel whose CTAs had a unit each, 39 with four CTAs a
-// unit), else that chain: status and length, the inputs, three histograms and two sweeps, about 1 us each (one sequence, L=2048 2 heads
-// D=64: 8.3 us).
+// What bounds it: the moved bytes where units are many and long (B=32 L<=6000 keep=2500 4 heads D=128: 30 to 32 us; cold and one at a time
+// the selection's chain on one SM per unit takes 16 of them and 80 MB of moves 17.5; 45 us with one kernel whose CTAs had a unit each, 39 with
+// four CTAs a unit), else that chain: status and length, the inputs, three histograms and two sweeps, about 1 us each (one sequence, L=2048
+// 2 heads D=64: 8.1 us).
 #pragma once
 
 #include <limits.h>

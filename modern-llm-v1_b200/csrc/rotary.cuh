@@ -1,5 +1,6 @@
-// Rotary positions in every layout a model may have been trained with, on the way into the attention kernels and back: pairs of
-// neighbours or of the two halves, the first R of a head's D elements, a position per token, with or without the QK-norm behind.
+// Rotary positions in other layouts than the reference's, on the way into the attention kernels and back: pairs of neighbours or of the
+// two halves, the first R of a head's D elements, a position per token, with the QK-norm behind the rotation (where the reference has it)
+// or without.  A norm in front of the rotation is not among them: with a gamma that differs within a pair the two do not commute.
 // (rope_norm.cuh is the reference's one form of it: all of the head, neighbours, the norm always, llm/src/model/rope.cu:25-65.)
 //
 //   the pair i < R / 2 of a row at position p is  (a, b) = (x[2i], x[2i+1])  or  (x[i], x[i + R/2])
@@ -12,8 +13,9 @@
 // heads, so that a token's cosines and sines stay in registers.  Where the halves are paired a lane's 8 elements are four pairs, two
 // pieces of four R / 2 apart (R is a multiple of 16); behind R they are two pieces side by side.  (Eight elements in a row, with the
 // partners by shuffle, took twice the registers for the tables and 8 to 16 shuffles a row: backward with the norm, BF16 B=4 T=8192 16/4
-// D=128, 122.8 us instead of 105.8.)  Measured, q and k together: that backward 4.8 TB/s (interleaved 100 us); FP32 forward with the norm,
-// B=16 T=1024 16/4 D=64 R=32, 23.4 us, 5.4 TB/s; one token 4 us, a launch.  More rows in flight (3 or 4 instead of 2), 2 or 4 CTAs per SM
+// D=128, 122.8 us instead of 106.)  Measured, q and k together: that backward 4.8 TB/s (interleaved 100 us); FP32 forward with the norm,
+// B=16 T=1024 16/4 D=64 R=32, 23.4 us, 5.4 TB/s; without the norm B=4 T=8192 16/4 D=128 BF16 58.0 us forward and 58.3 back (5.8 TB/s), FP32
+// R=64 82.5 and 86.9 (6.1, 5.8); one token 4 us, a launch.  More rows in flight (3 or 4 instead of 2), 2 or 4 CTAs per SM
 // instead of 3: all slower (102.6 -> 105 to 130).
 #pragma once
 
@@ -96,7 +98,8 @@ __device__ __forceinline__ void rotary_store8(void* base, long long row, int at,
     }
 }
 // gamma of the lane's elements, one by one: it may begin at any float of a buffer that holds all of a model's parameters.  (Once per
-// warp, in front of its rows.)
+// warp, in front of its rows; against 16-byte loads only the backward of FP32 half pairs takes longer, by a spill: B=4 T=4096 16/4 D=128
+// 72.2 us instead of 71.5.)
 __device__ __forceinline__ void rotary_gamma(const float* gamma, int at, int more, float (&g)[8]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) g[e] = gamma[at + e], g[e + 4] = gamma[at + more + e];

@@ -1,8 +1,9 @@
-"""Rotary positions of every layout for q and k, forward and backward (csrc/rotary.cuh).
+"""Rotary positions in other layouts for q and k, forward and backward (csrc/rotary.cuh).
 
 rope_norm.py has the reference's one form (all of a head, neighbouring pairs, the token's index, the norm always).  Models trained
 elsewhere differ: pairs of the head's halves, only part of the head, positions of their own per token (padded or packed batches),
-no QK-norm, and frequencies scaled for contexts longer than those trained on.  The caller allocates every tensor; outputs are
+no QK-norm, and frequencies scaled for contexts longer than those trained on.  A QK-norm is behind the rotation, as the reference has it;
+a model with the norm in front of it (and a gamma that differs within a pair) normalises first and passes no gammas here.  The caller allocates every tensor; outputs are
 overwritten except ``d_gamma_*``, which are accumulated into as in rope_qknorm_backward.  Bad arguments raise ValueError, CUDA
 failures RuntimeError; there is no CPU or PyTorch fallback.
 """
